@@ -431,6 +431,56 @@ int triposplat_b200_q_kv_rmsnorm_sdpa_split(const float* q, const float* kv, con
                                             const float* k_gamma, int B, int Lq, int Lk, int H,
                                             void* out_split);
 
+/* ---------------------------------------------------------------- training operators ---
+ * No reference counterpart (the CPU project only samples).  dtype: 0 fp32, 1 bf16, 2 fp16;
+ * sums, statistics and parameters are fp32 whatever the tensors' type.  `strides` are host
+ * arrays of element strides; the last dimension is contiguous.  Extra status codes as above;
+ * -3 also for an unknown dtype / kind / layout.  All are deterministic (no atomics). */
+
+/* z = x + residual_scale * gate[b] * post_weight * post(y),
+ * h = pre_weight * pre(z) * (1 + scale[b]) + shift[b];  x, y, z, h [B, L, C], C <= 8192.
+ * post, pre: 0 none (pre: h is not written), 1 LayerNorm, 2 RMSNorm; gate, scale, shift
+ * [B, C] and the weights [C] may be null (scale and shift together); stats [B * L, 4], 16-byte
+ * aligned, for the backward pass.  strides: x batch, row, y batch, row; z, h contiguous. */
+int triposplat_b200_norm_gate(const void* x, const void* y, const int64_t* strides, const float* gate,
+                              const float* scale, const float* shift, const float* pre_weight,
+                              const float* post_weight, void* z, void* h, float* stats, int dtype,
+                              int B, int64_t L, int C, int pre, int post, float residual_scale,
+                              float eps);
+/* Gradients of the same from dz and dh (one of them may be null).  strides: batch, row of x, y,
+ * dz, dh; dx, dy contiguous; each parameter gradient may be null. */
+int triposplat_b200_norm_gate_backward(const void* dz, const void* dh, const void* x, const void* y,
+                                       const int64_t* strides, const float* stats, const float* gate,
+                                       const float* scale, const float* pre_weight,
+                                       const float* post_weight, void* dx, void* dy, float* dgate,
+                                       float* dscale, float* dshift, float* dpre_weight,
+                                       float* dpost_weight, int dtype, int B, int64_t L, int C, int pre,
+                                       int post, float residual_scale);
+
+/* Rotary positions with several axes: x [B, L, H, D] (D even, <= 256), positions [L, axes] of
+ * numbers (position_type 0 int32, 1 int64, 2 fp32; position_batch_stride elements between batch
+ * entries' tables, 0 = shared), axis_pairs (host, 1 to 4 counts, P = their sum <= D / 2),
+ * inv_freq [P].  layout 0: pair p is (2p, 2p+1); 1: (p, P+p).  gamma [H, D] or null: the
+ * rotated vector r becomes r * sqrt(D) / max(|r|, 1e-12) * gamma.  strides: batch, token, head
+ * of x, then of y; y may be x. */
+int triposplat_b200_axis_rope(const void* x, const void* positions, const float* inv_freq,
+                              const float* gamma, void* y, const int64_t* strides, int dtype,
+                              int position_type, int64_t position_batch_stride, int B, int64_t L, int H,
+                              int D, const int* axis_pairs, int axes, int layout);
+/* dx (and with gamma, where asked for, dgamma [H, D]) of the same; x is read only with gamma.
+ * strides: batch, token, head of dy, x, dx; dx may be dy. */
+int triposplat_b200_axis_rope_backward(const void* dy, const void* x, const void* positions,
+                                       const float* inv_freq, const float* gamma, void* dx, float* dgamma,
+                                       const int64_t* strides, int dtype, int position_type,
+                                       int64_t position_batch_stride, int B, int64_t L, int H, int D,
+                                       const int* axis_pairs, int axes, int layout);
+
+/* norm = 2-norm of all gradients together; each is scaled by min(1, max_norm / (norm + 1e-6)),
+ * in place or into outs[i].  grads, outs (null: in place), sizes, dtypes are host arrays of
+ * `count` entries; norm is one device float. */
+int triposplat_b200_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t* sizes,
+                                   const int* dtypes, int count, float max_norm, float* norm);
+
 /* ---- Tensor-parallel reduction over NVLink peer memory (no reference counterpart) ----
  * ipc_alloc: cudaMalloc'd, zeroed buffer plus its 64-byte CUDA IPC handle; ipc_open maps a
  * handle of another process of the node; ipc_close / ipc_free release them.

@@ -113,6 +113,12 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "triposplat_timestep_embedding_f32_avx512": ([VP] * 3 + [I] * 4, I),
     "triposplat_pcd_position_embedding_f32_avx512": ([VP] * 3 + [I64] + [I] * 5, I),
     "triposplat_mul_inplace_f32_avx512": ([VP, VP, I64, I], I),
+    # training operators
+    "triposplat_b200_norm_gate": ([VP] * 11 + [I, I, I64, I, I, I, F, F], I),
+    "triposplat_b200_norm_gate_backward": ([VP] * 17 + [I, I, I64, I, I, I, F], I),
+    "triposplat_b200_axis_rope": ([VP] * 6 + [I, I, I64, I, I64, I, I, VP, I, I], I),
+    "triposplat_b200_axis_rope_backward": ([VP] * 8 + [I, I, I64, I, I64, I, I, VP, I, I], I),
+    "triposplat_b200_clip_grad_norm": ([VP] * 4 + [I, F, VP], I),
     "triposplat_repo_phasor_f32_avx512": ([VP, VP, VP, I, VP, VP, I, VP, VP, I, VP, I64, I], I),
 }
 
@@ -137,8 +143,14 @@ def _load(path: str) -> ctypes.CDLL:
     return lib
 
 
-def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
+@lru_cache(maxsize=16)
+def _load_named(path, from_env: str | None) -> ctypes.CDLL:
     return _load(str(library_path(path)))
+
+
+def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
+    # resolving the path takes longer than a small kernel runs, so it is done once per name
+    return _load_named(path, os.environ.get("TRIPOSPLAT_B200_LIBRARY"))
 
 
 def bind(lib: ctypes.CDLL, name: str, args, res=I):
@@ -152,7 +164,8 @@ def use_current_stream(lib: ctypes.CDLL) -> None:
     """Queue the library's next launches on PyTorch's current CUDA stream."""
     import torch
 
-    lib.triposplat_b200_set_stream(ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    # the raw handle: torch.cuda.current_stream() spends several microseconds on its Stream object
+    lib.triposplat_b200_set_stream(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def check_status(lib: ctypes.CDLL) -> None:

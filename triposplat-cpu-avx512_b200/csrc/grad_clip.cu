@@ -1,0 +1,216 @@
+// Global gradient norm over many tensors, and clipping:
+//   n = sqrt(sum of g^2) ;  c = min(1, max_norm / (n + 1e-6)) ;  out = g * c   (out may be g)
+//
+// Bound by HBM: the norm needs every gradient before the first can be scaled, so each is
+// read twice (the second read comes out of L2 where the set fits it) and written once.
+// Tensors are cut into chunks of 8192 elements.  Two launches per group of up to 768 tensors:
+// the first writes one fp64 partial sum of squares per block, the second adds all partial sums
+// in a fixed order (every block for itself: no atomics, the same bits on every run, and
+// nothing comes back to the host) and scales.  Squares are summed in fp64 from the thread on, so
+// that no gradient a 32-bit type holds overflows or vanishes in its square.
+//
+// The table of tensors travels in the launch's parameters (25 KB of the 32 KB they may take, 2 KB
+// for up to 64 tensors), so a call uploads nothing and keeps nothing.
+#include <stdint.h>
+
+#include "common.cuh"
+#include "runtime.h"
+#include "vecio.cuh"
+
+namespace tsb {
+namespace clip {
+
+constexpr int kGroup = 768;      // tensors per launch
+constexpr int kFew = 64;         // table size where a call has no more tensors than this
+constexpr int kChunk = 8192;     // elements per unit of work
+constexpr int kThreads = 256;
+
+template <int N>
+struct Table {
+  const void* in[N];
+  void* out[N];                  // scale only
+  int64_t size[N];
+  int64_t first[N + 1];          // chunk number at which each tensor starts
+  uint8_t dtype[N];
+  int n;
+};
+static_assert(sizeof(Table<kGroup>) <= 32764 - 64, "kernel parameters");
+
+// A chunk of one tensor: its first element's number and its length.
+struct Chunk {
+  int tensor, n;
+  int64_t at;
+};
+
+template <int N>
+__device__ __forceinline__ Chunk chunk_of(const Table<N>& t, int64_t u) {
+  int lo = 0, hi = t.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.first[mid] <= u) lo = mid;
+    else hi = mid - 1;
+  }
+  const int64_t at = (u - t.first[lo]) * kChunk;
+  return {lo, (int)min((int64_t)kChunk, t.size[lo] - at), at};
+}
+
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double sm[kThreads / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double s = 0.0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) s += sm[w];
+  return s;
+}
+
+// 16-byte accesses where the chunk starts on a 16-byte boundary, single elements otherwise
+template <class T>
+__device__ __forceinline__ double chunk_squares(const T* p, int n, double acc) {
+  constexpr int V = 16 / sizeof(T);
+  int done = 0;
+  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    done = n / V * V;
+#pragma unroll 4
+    for (int e = threadIdx.x * V; e < done; e += kThreads * V) {
+      float v[V];
+      load_vec<T, V>(p + e, v);
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc = fma((double)v[k], (double)v[k], acc);
+    }
+  }
+  for (int e = done + threadIdx.x; e < n; e += kThreads) {
+    const double v = (double)to_f32(p[e]);
+    acc = fma(v, v, acc);
+  }
+  return acc;
+}
+
+template <class T>
+__device__ __forceinline__ void chunk_scale(const T* p, T* o, int n, float c) {
+  constexpr int V = 16 / sizeof(T);
+  int done = 0;
+  if (((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(o)) & 15) == 0) {
+    done = n / V * V;
+#pragma unroll 4
+    for (int e = threadIdx.x * V; e < done; e += kThreads * V) {
+      float v[V];
+      load_vec<T, V>(p + e, v);
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] *= c;
+      store_vec<T, V>(o + e, v);
+    }
+  }
+  for (int e = done + threadIdx.x; e < n; e += kThreads) o[e] = from_f32<T>(to_f32(p[e]) * c);
+}
+
+template <int N>
+__global__ void __launch_bounds__(kThreads) square_sum_k(const __grid_constant__ Table<N> t, double* part) {
+  double acc = 0.0;
+  for (int64_t u = blockIdx.x; u < t.first[t.n]; u += gridDim.x) {
+    const Chunk c = chunk_of(t, u);
+    const void* p = t.in[c.tensor];
+    if (t.dtype[c.tensor] == kF32) acc = chunk_squares(static_cast<const float*>(p) + c.at, c.n, acc);
+    else if (t.dtype[c.tensor] == kBF16)
+      acc = chunk_squares(static_cast<const __nv_bfloat16*>(p) + c.at, c.n, acc);
+    else acc = chunk_squares(static_cast<const __half*>(p) + c.at, c.n, acc);
+  }
+  acc = block_sum(acc);
+  if (threadIdx.x == 0) part[blockIdx.x] = acc;
+}
+
+template <int N>
+__global__ void __launch_bounds__(kThreads) scale_k(const __grid_constant__ Table<N> t, const double* part,
+                                                    int parts, float max_norm, float* norm) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < parts; i += kThreads) s += part[i];
+  const float total = (float)sqrt(block_sum(s));
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
+  // NaN stays NaN, an infinite norm scales by zero: as a division and a minimum give them
+  const float q = max_norm / (total + 1.0e-6f);
+  const float f = q > 1.0f ? 1.0f : q;
+  for (int64_t u = blockIdx.x; u < t.first[t.n]; u += gridDim.x) {
+    const Chunk c = chunk_of(t, u);
+    const void* p = t.in[c.tensor];
+    void* o = t.out[c.tensor];
+    if (f == 1.0f && o == p) continue;
+    if (t.dtype[c.tensor] == kF32)
+      chunk_scale(static_cast<const float*>(p) + c.at, static_cast<float*>(o) + c.at, c.n, f);
+    else if (t.dtype[c.tensor] == kBF16)
+      chunk_scale(static_cast<const __nv_bfloat16*>(p) + c.at, static_cast<__nv_bfloat16*>(o) + c.at, c.n, f);
+    else chunk_scale(static_cast<const __half*>(p) + c.at, static_cast<__half*>(o) + c.at, c.n, f);
+  }
+}
+
+// Tensors [from, to) of a call through one launch of either kernel.
+template <int N>
+static void launch(const void* const* grads, void* const* outs, const int64_t* sizes, const int* dtypes,
+                   int from, int to, bool scale, double* part, int parts, int blocks, float max_norm,
+                   float* norm, cudaStream_t stream) {
+  Table<N> t;
+  t.n = 0;
+  t.first[0] = 0;
+  for (int i = from; i < to; ++i) {
+    if (sizes[i] == 0) continue;
+    t.in[t.n] = grads[i];
+    t.out[t.n] = outs ? outs[i] : const_cast<void*>(grads[i]);
+    t.size[t.n] = sizes[i];
+    t.dtype[t.n] = (uint8_t)dtypes[i];
+    t.first[t.n + 1] = t.first[t.n] + (sizes[i] + kChunk - 1) / kChunk;
+    ++t.n;
+  }
+  LaunchScope scope(kKElementwise, stream);
+  if (scale) scale_k<N><<<blocks, kThreads, 0, stream>>>(t, part, parts, max_norm, norm);
+  else square_sum_k<N><<<blocks, kThreads, 0, stream>>>(t, part);
+}
+
+}  // namespace clip
+}  // namespace tsb
+
+extern "C" {
+
+int triposplat_b200_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t* sizes,
+                                   const int* dtypes, int count, float max_norm, float* norm) {
+  using namespace tsb;
+  using namespace tsb::clip;
+  if (!norm || (count > 0 && (!grads || !sizes || !dtypes))) return kNullPointer;
+  if (count < 0 || !(max_norm >= 0.0f)) return kBadDims;
+  int64_t chunks = 0;
+  for (int i = 0; i < count; ++i) {
+    if (sizes[i] < 0) return kBadDims;
+    if (dtypes[i] < kF32 || dtypes[i] > kF16) return kBadRange;
+    if (sizes[i] > 0 && (!grads[i] || (outs && !outs[i]))) return kNullPointer;
+    const uintptr_t low = dtype_size(dtypes[i]) - 1;
+    if ((reinterpret_cast<uintptr_t>(grads[i]) & low) || (outs && (reinterpret_cast<uintptr_t>(outs[i]) & low)))
+      return kBadAlignment;
+    chunks += (sizes[i] + kChunk - 1) / kChunk;
+  }
+  const int st = entry_check();
+  if (st != kOk) return st;
+  if (!is_device_pointer(norm)) return kNotDevicePointer;
+  for (int i = 0; i < count; ++i)
+    if (sizes[i] > 0 && (!is_device_pointer(grads[i]) || (outs && !is_device_pointer(outs[i]))))
+      return kNotDevicePointer;
+  cudaStream_t stream = current_stream();
+  const int groups = count > kGroup ? (count + kGroup - 1) / kGroup : 1;
+  const int64_t cap = (int64_t)sm_count() * 8;
+  const int blocks = (int)(chunks < 1 ? 1 : (chunks < cap ? chunks : cap));
+  double* part = static_cast<double*>(workspace((size_t)groups * blocks * sizeof(double), stream));
+  if (!part) return kWorkspace;
+  for (int pass = 0; pass < 2; ++pass)
+    for (int g = 0; g < groups; ++g) {
+      const int from = g * kGroup, to = count - from < kGroup ? count : from + kGroup;
+      double* p = pass == 0 ? part + (size_t)g * blocks : part;
+      if (to - from <= kFew)
+        launch<kFew>(grads, outs, sizes, dtypes, from, to, pass == 1, p, groups * blocks, blocks, max_norm,
+                     g == 0 ? norm : nullptr, stream);
+      else
+        launch<kGroup>(grads, outs, sizes, dtypes, from, to, pass == 1, p, groups * blocks, blocks, max_norm,
+                       g == 0 ? norm : nullptr, stream);
+    }
+  return launch_status();
+}
+
+}  // extern "C"

@@ -1,0 +1,489 @@
+// Norms before and after a block, fused with the block's gate, residual scale and modulation:
+//   z = x + rho * gate[b] * w_post * post(y)
+//   h = w_pre * pre(z) * (1 + scale[b]) + shift[b]
+// post in {none, layer, rms}, pre in {none, layer, rms}; layer(v) = (v - mean) * r with
+// r = 1 / sqrt(mean((v - mean)^2) + eps), rms(v) = v / sqrt(mean(v^2) + eps).
+//
+// Backward, with m = post(y), n = pre(z) (rebuilt from x, y and four saved numbers per row, so
+// that 16-bit tensors add no rounding between the two directions):
+//   dn = dh (1 + scale) w_pre ;  dz' = dz + r_n (dn - [layer] mean(dn) - n mean(dn n)) = dx
+//   dm = dz' rho gate w_post  ;  dy = r_m (dm - [layer] mean(dm) - m mean(dm m))   (none: dm)
+//   S0 = sum dh, S1 = sum dh n, S2 = sum dz' m over a batch entry's rows, per column:
+//   dshift = S0, dscale = w_pre S1, dgate = rho w_post S2,
+//   dw_pre = sum_b (1 + scale) S1, dw_post = sum_b rho gate S2
+// so three column sums carry all five parameter gradients.  Each row group adds its rows in
+// order in registers and writes one partial row; a second kernel adds the partial rows in a
+// fixed order: no atomics, the same bits on every run.
+//
+// Bound by HBM: every tensor is read or written once.  A row is held in registers (8 or 16
+// elements per thread) by one warp (up to 256 columns) or one block, statistics are taken
+// in two passes over the registers (mean, then centred squares) in fp32.
+#include <stdint.h>
+
+#include <initializer_list>
+
+#include "common.cuh"
+#include "runtime.h"
+#include "vecio.cuh"
+
+namespace tsb {
+namespace ng {
+
+enum Kind : int { kNone = 0, kLayer = 1, kRms = 2 };
+constexpr int kMaxThreads = 512;   // per row: 8 columns each up to 4096, 16 beyond
+constexpr int kMaxColumns = 8192;
+
+struct Args {
+  const void *x, *y, *dz, *dh;             // T; dz and dh only in the backward pass
+  int64_t xb, xl, yb, yl, zb, zl, hb, hl;  // element strides (batch, row) of x, y, dz, dh
+  const float *gate, *scale, *shift, *wpre, *wpost;  // [B, C], [B, C], [B, C], [C], [C] or null
+  void *out0, *out1;                       // z, h or dx, dy: [B, L, C] contiguous
+  float* stats;                            // [B * L, 4]: mean, r of post; mean, r of pre
+  float* part;                             // [B, groups, 3, C] partial column sums
+  int64_t L;
+  int B, C, pre, post, groups;
+  float rho, eps;
+};
+
+// Sum over a row's threads: one warp, or the whole block (`sm` [2][32] float2, alternated by
+// `turn`, so one barrier per sum is enough).
+__device__ __forceinline__ float2 row_sum(float2 v, float2 (*sm)[32], int& turn) {
+  v.x = warp_sum(v.x);
+  v.y = warp_sum(v.y);
+  if (blockDim.x == 32) return v;
+  float2* s = sm[turn];
+  turn ^= 1;
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float2 r = make_float2(0.0f, 0.0f);
+  for (unsigned w = 0; w < blockDim.x / 32; ++w) {
+    r.x += s[w].x;
+    r.y += s[w].y;
+  }
+  return r;
+}
+
+// mean (0 for rms) and r of a row held in registers; elements past C are zero and stay out of
+// the centred sum through `valid`
+template <int VEC, int NI>
+__device__ __forceinline__ float2 row_stats(const float (&v)[NI][VEC], int kind, int C, float eps,
+                                            float2 (*sm)[32], int& turn) {
+  float mean = 0.0f;
+  if (kind == kLayer) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s += v[i][e];
+    mean = row_sum(make_float2(s, 0.0f), sm, turn).x / (float)C;
+  }
+  float q = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float d = v[i][e] - mean;
+      if (c + e < C) q = fmaf(d, d, q);
+    }
+  }
+  q = row_sum(make_float2(q, 0.0f), sm, turn).x;
+  return make_float2(mean, 1.0f / sqrtf(q / (float)C + eps));
+}
+
+template <class T, int VEC, int NI>
+__device__ __forceinline__ void load_row(const T* p, int C, float (&v)[NI][VEC]) {
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
+    if (c < C) {
+      load_vec<T, VEC>(p + c, v[i]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[i][e] = 0.0f;
+    }
+  }
+}
+
+template <class T, int VEC, int NI>
+__device__ __forceinline__ void store_row(T* p, int C, const float (&v)[NI][VEC]) {
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
+    if (c < C) store_vec<T, VEC>(p + c, v[i]);
+  }
+}
+
+// per-column fp32 parameter (null: `other`)
+template <int VEC>
+__device__ __forceinline__ void load_par(const float* p, int c, float other, float (&v)[VEC]) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = other;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) v[e] = __ldg(p + c + e);
+}
+
+template <class T, int VEC, int NI>
+__global__ void __launch_bounds__(kMaxThreads) norm_gate_k(const Args a) {
+  __shared__ float2 sm[2][32];
+  int turn = 0;
+  const int64_t rows = (int64_t)a.B * a.L;
+  for (int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; r < rows;
+       r += (int64_t)gridDim.x * blockDim.y) {
+    const int64_t b = r / a.L, l = r - b * a.L;
+    float z[NI][VEC], m[NI][VEC];
+    load_row<T, VEC, NI>(static_cast<const T*>(a.y) + b * a.yb + l * a.yl, a.C, m);
+    load_row<T, VEC, NI>(static_cast<const T*>(a.x) + b * a.xb + l * a.xl, a.C, z);
+    float2 sp = make_float2(0.0f, 1.0f), sn = make_float2(0.0f, 1.0f);
+    if (a.post != kNone) sp = row_stats<VEC, NI>(m, a.post, a.C, a.eps, sm, turn);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
+      if (c >= a.C) continue;
+      float g[VEC], w[VEC];
+      load_par<VEC>(a.gate ? a.gate + b * a.C : nullptr, c, 1.0f, g);
+      load_par<VEC>(a.wpost, c, 1.0f, w);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        z[i][e] = fmaf((m[i][e] - sp.x) * sp.y * w[e], g[e] * a.rho, z[i][e]);
+    }
+    store_row<T, VEC, NI>(static_cast<T*>(a.out0) + r * a.C, a.C, z);
+    if (a.pre != kNone) {
+      sn = row_stats<VEC, NI>(z, a.pre, a.C, a.eps, sm, turn);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
+        if (c >= a.C) continue;
+        float s[VEC], t[VEC], w[VEC];
+        load_par<VEC>(a.scale ? a.scale + b * a.C : nullptr, c, 0.0f, s);
+        load_par<VEC>(a.shift ? a.shift + b * a.C : nullptr, c, 0.0f, t);
+        load_par<VEC>(a.wpre, c, 1.0f, w);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          z[i][e] = fmaf((z[i][e] - sn.x) * sn.y * w[e], 1.0f + s[e], t[e]);
+      }
+      store_row<T, VEC, NI>(static_cast<T*>(a.out1) + r * a.C, a.C, z);
+    }
+    if (threadIdx.x == 0)
+      *reinterpret_cast<float4*>(a.stats + 4 * r) = make_float4(sp.x, sp.y, sn.x, sn.y);
+  }
+}
+
+// Row group g of batch entry blockIdx.y takes the entry's rows [g * chunk, (g + 1) * chunk).
+template <class T, int VEC, int NI>
+__global__ void __launch_bounds__(kMaxThreads) norm_gate_bwd_k(const Args a) {
+  __shared__ float2 sm[2][32];
+  int turn = 0;
+  const int b = blockIdx.y, g = blockIdx.x * blockDim.y + threadIdx.y;
+  const int64_t chunk = (a.L + a.groups - 1) / a.groups;
+  const int64_t l1 = min(a.L, (g + 1) * chunk);
+  const float inv_c = 1.0f / (float)a.C;
+  float a0[NI][VEC], a1[NI][VEC], a2[NI][VEC];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) a0[i][e] = a1[i][e] = a2[i][e] = 0.0f;
+  for (int64_t l = g * chunk; l < l1; ++l) {
+    const int64_t r = b * a.L + l;
+    float n[NI][VEC], m[NI][VEC], d[NI][VEC];
+    load_row<T, VEC, NI>(static_cast<const T*>(a.y) + b * a.yb + l * a.yl, a.C, m);
+    load_row<T, VEC, NI>(static_cast<const T*>(a.x) + b * a.xb + l * a.xl, a.C, n);
+    const float4 st = __ldg(reinterpret_cast<const float4*>(a.stats + 4 * r));
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
+      if (c >= a.C) continue;
+      float gt[VEC], w[VEC];
+      load_par<VEC>(a.gate ? a.gate + (int64_t)b * a.C : nullptr, c, 1.0f, gt);
+      load_par<VEC>(a.wpost, c, 1.0f, w);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        m[i][e] = (m[i][e] - st.x) * st.y;
+        n[i][e] = (fmaf(m[i][e] * w[e], gt[e] * a.rho, n[i][e]) - st.z) * st.w;
+      }
+    }
+    if (a.pre != kNone && a.dh != nullptr) {
+      load_row<T, VEC, NI>(static_cast<const T*>(a.dh) + b * a.hb + l * a.hl, a.C, d);
+      float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
+        if (c >= a.C) continue;
+        float sc[VEC], w[VEC];
+        load_par<VEC>(a.scale ? a.scale + (int64_t)b * a.C : nullptr, c, 0.0f, sc);
+        load_par<VEC>(a.wpre, c, 1.0f, w);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          a0[i][e] += d[i][e];
+          a1[i][e] = fmaf(d[i][e], n[i][e], a1[i][e]);
+          d[i][e] *= (1.0f + sc[e]) * w[e];
+          s.x += d[i][e];
+          s.y = fmaf(d[i][e], n[i][e], s.y);
+        }
+      }
+      s = row_sum(s, sm, turn);
+      const float mean = a.pre == kLayer ? s.x * inv_c : 0.0f, dot = s.y * inv_c;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) d[i][e] = st.w * (d[i][e] - mean - n[i][e] * dot);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) d[i][e] = 0.0f;
+    }
+    if (a.dz != nullptr) {
+      load_row<T, VEC, NI>(static_cast<const T*>(a.dz) + b * a.zb + l * a.zl, a.C, n);
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) d[i][e] += n[i][e];
+    }
+    store_row<T, VEC, NI>(static_cast<T*>(a.out0) + r * a.C, a.C, d);
+    float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
+      if (c >= a.C) continue;
+      float gt[VEC], w[VEC];
+      load_par<VEC>(a.gate ? a.gate + (int64_t)b * a.C : nullptr, c, 1.0f, gt);
+      load_par<VEC>(a.wpost, c, 1.0f, w);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        a2[i][e] = fmaf(d[i][e], m[i][e], a2[i][e]);
+        d[i][e] *= gt[e] * a.rho * w[e];
+        s.x += d[i][e];
+        s.y = fmaf(d[i][e], m[i][e], s.y);
+      }
+    }
+    if (a.post != kNone) {
+      s = row_sum(s, sm, turn);
+      const float mean = a.post == kLayer ? s.x * inv_c : 0.0f, dot = s.y * inv_c;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) d[i][e] = st.y * (d[i][e] - mean - m[i][e] * dot);
+    }
+    store_row<T, VEC, NI>(static_cast<T*>(a.out1) + r * a.C, a.C, d);
+  }
+  if (a.part == nullptr || g >= a.groups) return;
+  float* p = a.part + ((int64_t)b * a.groups + g) * 3 * a.C;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if (c + e < a.C) {
+        p[c + e] = a0[i][e];
+        p[a.C + c + e] = a1[i][e];
+        p[2 * a.C + c + e] = a2[i][e];
+      }
+  }
+}
+
+struct ReduceArgs {
+  const float *part, *gate, *scale, *wpre, *wpost;
+  float *dgate, *dscale, *dshift, *dwpre, *dwpost;  // nullable
+  int B, C, groups;
+  float rho;
+};
+
+// 32 columns per block, 32 threads per column; partial rows added in a fixed order.
+__global__ void __launch_bounds__(1024) norm_gate_reduce_k(const ReduceArgs a) {
+  __shared__ float sm[3][32][33];
+  const int c = blockIdx.x * 32 + threadIdx.x, y = threadIdx.y;
+  float wp = 0.0f, wq = 0.0f;
+  for (int b = 0; b < a.B; ++b) {
+    float s[3] = {0.0f, 0.0f, 0.0f};
+    if (c < a.C) {
+      const float* p = a.part + (int64_t)b * a.groups * 3 * a.C + c;
+#pragma unroll 4
+      for (int g = y; g < a.groups; g += 32) {
+#pragma unroll
+        for (int q = 0; q < 3; ++q) s[q] += p[((int64_t)g * 3 + q) * a.C];
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) sm[q][threadIdx.x][y] = s[q];
+    __syncthreads();
+    if (y < 3) {  // warp y adds quantity y, one column per lane
+      float t = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) t += sm[y][threadIdx.x][j];
+      sm[y][threadIdx.x][32] = t;
+    }
+    __syncthreads();
+    if (y == 0 && c < a.C) {
+      const float s0 = sm[0][threadIdx.x][32], s1 = sm[1][threadIdx.x][32], s2 = sm[2][threadIdx.x][32];
+      const int64_t bc = (int64_t)b * a.C + c;
+      if (a.dshift) a.dshift[bc] = s0;
+      if (a.dscale) a.dscale[bc] = s1 * (a.wpre ? a.wpre[c] : 1.0f);
+      if (a.dgate) a.dgate[bc] = s2 * a.rho * (a.wpost ? a.wpost[c] : 1.0f);
+      wp = fmaf(1.0f + (a.scale ? a.scale[bc] : 0.0f), s1, wp);
+      wq = fmaf(a.rho * (a.gate ? a.gate[bc] : 1.0f), s2, wq);
+    }
+    __syncthreads();
+  }
+  if (y == 0 && c < a.C) {
+    if (a.dwpre) a.dwpre[c] = wp;
+    if (a.dwpost) a.dwpost[c] = wq;
+  }
+}
+
+// 16-byte accesses where every row of every tensor starts on a 16-byte boundary, single
+// elements otherwise (odd widths, sliced views)
+static bool vec_ok(const Args& a, int size) {
+  const int64_t n = 16 / size;
+  auto bad = [&](const void* p, int64_t sb, int64_t sl) {
+    return p && ((reinterpret_cast<uintptr_t>(p) & 15) || sb % n || sl % n);
+  };
+  if (a.C % n) return false;
+  return !(bad(a.x, a.xb, a.xl) || bad(a.y, a.yb, a.yl) || bad(a.dz, a.zb, a.zl) || bad(a.dh, a.hb, a.hl) ||
+           bad(a.out0, 0, 0) || bad(a.out1, 0, 0));
+}
+
+struct Shape {
+  dim3 block;
+  bool wide;  // 16 elements per thread
+};
+
+static Shape shape_of(int C) {
+  Shape s;
+  s.wide = C > 8 * kMaxThreads;
+  const int per = s.wide ? 16 : 8;
+  const int t = ((C + per - 1) / per + 31) / 32 * 32;
+  s.block = t == 32 ? dim3(32, 4) : dim3(t, 1);
+  return s;
+}
+
+template <class T, int VEC>
+static void launch_fwd(const Args& a, const Shape& s, unsigned grid, cudaStream_t st) {
+  if (s.wide) norm_gate_k<T, VEC, 16 / VEC><<<grid, s.block, 0, st>>>(a);
+  else norm_gate_k<T, VEC, 8 / VEC><<<grid, s.block, 0, st>>>(a);
+}
+template <class T, int VEC>
+static void launch_bwd(const Args& a, const Shape& s, dim3 grid, cudaStream_t st) {
+  if (s.wide) norm_gate_bwd_k<T, VEC, 16 / VEC><<<grid, s.block, 0, st>>>(a);
+  else norm_gate_bwd_k<T, VEC, 8 / VEC><<<grid, s.block, 0, st>>>(a);
+}
+
+// whether a tensor's pointer is not a multiple of its element's size
+static bool misaligned(const void* p, int size) { return reinterpret_cast<uintptr_t>(p) & (size - 1); }
+
+static int check(const Args& a, int dtype) {
+  if (a.B <= 0 || a.B > 65535 || a.L <= 0 || a.C <= 0 || a.C > kMaxColumns) return kBadDims;
+  if (dtype < kF32 || dtype > kF16 || a.pre < kNone || a.pre > kRms || a.post < kNone || a.post > kRms)
+    return kBadRange;
+  if ((a.scale == nullptr) != (a.shift == nullptr)) return kNullPointer;
+  if (a.pre == kNone && (a.scale || a.wpre)) return kBadRange;
+  for (const void* p : {a.x, a.y, a.dz, a.dh, static_cast<const void*>(a.out0), static_cast<const void*>(a.out1)})
+    if (misaligned(p, dtype_size(dtype))) return kBadAlignment;
+  for (const float* p : {a.gate, a.scale, a.shift, a.wpre, a.wpost})
+    if (misaligned(p, 4)) return kBadAlignment;
+  if (misaligned(a.stats, 16)) return kBadAlignment;
+  return kOk;
+}
+
+}  // namespace ng
+}  // namespace tsb
+
+extern "C" {
+
+int triposplat_b200_norm_gate(const void* x, const void* y, const int64_t* strides, const float* gate,
+                              const float* scale, const float* shift, const float* pre_weight,
+                              const float* post_weight, void* z, void* h, float* stats, int dtype,
+                              int B, int64_t L, int C, int pre, int post, float residual_scale,
+                              float eps) {
+  using namespace tsb;
+  if (!x || !y || !strides || !z || !stats || (pre != ng::kNone && !h)) return kNullPointer;
+  ng::Args a{};
+  a.x = x; a.y = y;
+  a.xb = strides[0]; a.xl = strides[1]; a.yb = strides[2]; a.yl = strides[3];
+  a.gate = gate; a.scale = scale; a.shift = shift; a.wpre = pre_weight; a.wpost = post_weight;
+  a.out0 = z; a.out1 = pre == ng::kNone ? nullptr : h; a.stats = stats;
+  a.L = L; a.B = B; a.C = C; a.pre = pre; a.post = post; a.rho = residual_scale; a.eps = eps;
+  int st = ng::check(a, dtype);
+  if (st != kOk) return st;
+  st = entry_check();
+  if (st != kOk) return st;
+  for (const void* p : {x, y, static_cast<const void*>(z), static_cast<const void*>(a.out1),
+                        static_cast<const void*>(stats), static_cast<const void*>(gate),
+                        static_cast<const void*>(scale), static_cast<const void*>(shift),
+                        static_cast<const void*>(pre_weight), static_cast<const void*>(post_weight)})
+    if (p && !is_device_pointer(p)) return kNotDevicePointer;
+  const ng::Shape s = ng::shape_of(C);
+  const int64_t blocks = ((int64_t)B * L + s.block.y - 1) / s.block.y;
+  const int64_t cap = (int64_t)sm_count() * (2048 / (s.block.x * s.block.y)) * 4;
+  const unsigned grid = (unsigned)(blocks < cap ? blocks : cap);
+  const bool vec = ng::vec_ok(a, dtype_size(dtype));
+  cudaStream_t stream = current_stream();
+  LaunchScope scope(kKElementwise, stream);
+  if (dtype == kF32) vec ? ng::launch_fwd<float, 4>(a, s, grid, stream) : ng::launch_fwd<float, 1>(a, s, grid, stream);
+  else if (dtype == kBF16)
+    vec ? ng::launch_fwd<__nv_bfloat16, 8>(a, s, grid, stream) : ng::launch_fwd<__nv_bfloat16, 1>(a, s, grid, stream);
+  else vec ? ng::launch_fwd<__half, 8>(a, s, grid, stream) : ng::launch_fwd<__half, 1>(a, s, grid, stream);
+  return launch_status();
+}
+
+int triposplat_b200_norm_gate_backward(const void* dz, const void* dh, const void* x, const void* y,
+                                       const int64_t* strides, const float* stats, const float* gate,
+                                       const float* scale, const float* pre_weight,
+                                       const float* post_weight, void* dx, void* dy, float* dgate,
+                                       float* dscale, float* dshift, float* dpre_weight,
+                                       float* dpost_weight, int dtype, int B, int64_t L, int C, int pre,
+                                       int post, float residual_scale) {
+  using namespace tsb;
+  if (!x || !y || !strides || !stats || !dx || !dy || (!dz && !dh)) return kNullPointer;
+  ng::Args a{};
+  a.x = x; a.y = y; a.dz = dz; a.dh = dh;
+  a.xb = strides[0]; a.xl = strides[1]; a.yb = strides[2]; a.yl = strides[3];
+  a.zb = strides[4]; a.zl = strides[5]; a.hb = strides[6]; a.hl = strides[7];
+  a.gate = gate; a.scale = scale; a.shift = scale; a.wpre = pre_weight; a.wpost = post_weight;
+  a.out0 = dx; a.out1 = dy; a.stats = const_cast<float*>(stats);
+  a.L = L; a.B = B; a.C = C; a.pre = pre; a.post = post; a.rho = residual_scale;
+  int st = ng::check(a, dtype);
+  if (st != kOk) return st;
+  if (pre == ng::kNone && dh) return kBadRange;
+  st = entry_check();
+  if (st != kOk) return st;
+  for (const void* p : {dz, dh, x, y, static_cast<const void*>(stats), static_cast<const void*>(gate),
+                        static_cast<const void*>(scale), static_cast<const void*>(pre_weight),
+                        static_cast<const void*>(post_weight), static_cast<const void*>(dx),
+                        static_cast<const void*>(dy), static_cast<const void*>(dgate),
+                        static_cast<const void*>(dscale), static_cast<const void*>(dshift),
+                        static_cast<const void*>(dpre_weight), static_cast<const void*>(dpost_weight)})
+    if (p && !is_device_pointer(p)) return kNotDevicePointer;
+  const ng::Shape s = ng::shape_of(C);
+  cudaStream_t stream = current_stream();
+  // row groups per batch entry: about 512 threads per SM in flight, one row per group at least
+  const int64_t want = ((int64_t)sm_count() * (512 / s.block.x > 0 ? 512 / s.block.x : 1) + B - 1) / B;
+  a.groups = (int)(want < L ? want : L);
+  const bool sums = dgate || dscale || dshift || dpre_weight || dpost_weight;
+  if (sums) {
+    a.part = static_cast<float*>(workspace((size_t)B * a.groups * 3 * C * sizeof(float), stream));
+    if (!a.part) return kWorkspace;
+  }
+  const dim3 grid((a.groups + s.block.y - 1) / s.block.y, B);
+  const bool vec = ng::vec_ok(a, dtype_size(dtype));
+  {
+    LaunchScope scope(kKElementwise, stream);
+    if (dtype == kF32)
+      vec ? ng::launch_bwd<float, 4>(a, s, grid, stream) : ng::launch_bwd<float, 1>(a, s, grid, stream);
+    else if (dtype == kBF16)
+      vec ? ng::launch_bwd<__nv_bfloat16, 8>(a, s, grid, stream) : ng::launch_bwd<__nv_bfloat16, 1>(a, s, grid, stream);
+    else vec ? ng::launch_bwd<__half, 8>(a, s, grid, stream) : ng::launch_bwd<__half, 1>(a, s, grid, stream);
+  }
+  if (sums) {
+    const ng::ReduceArgs ra{a.part, gate, scale, pre_weight, post_weight, dgate, dscale, dshift, dpre_weight,
+                            dpost_weight, B, C, a.groups, residual_scale};
+    LaunchScope scope(kKElementwise, stream);
+    ng::norm_gate_reduce_k<<<(C + 31) / 32, dim3(32, 32), 0, stream>>>(ra);
+  }
+  return launch_status();
+}
+
+}  // extern "C"
