@@ -475,6 +475,25 @@ int triposplat_b200_axis_rope_backward(const void* dy, const void* x, const void
                                        int64_t position_batch_stride, int B, int64_t L, int H, int D,
                                        const int* axis_pairs, int axes, int layout);
 
+/* Exact attention O = softmax(Q K^T / 8 + key_bias) V for training, head_dim 64, fp32 tensors of
+ * any strides with a contiguous last dimension.  strides: batch, head, row of q, k, v; key_bias
+ * [bias_batches, bias_heads, Lk] contiguous (1 or B, 1 or H) or null; out_blhd [B, Lq, H, 64];
+ * stats [B, H, Lq, 2] for the backward pass.  A key whose bias is -inf does not exist (its K and
+ * V may hold anything); a row without keys is zeros.  The scores' accuracy is that of
+ * triposplat_sdpa_f32_avx512_exact_q8t512. */
+int triposplat_b200_attention_forward(const float* q, const float* k, const float* v,
+                                      const int64_t* strides, const float* key_bias, int bias_batches,
+                                      int bias_heads, float* out_blhd, float* stats, int B, int H,
+                                      int Lq, int Lk);
+/* Its gradients from dout, with the probabilities recomputed.  strides: batch, head, row of dout,
+ * q, k, v, out, dq, dk, dv; dbias (shaped as key_bias) may be null.  Work space (library-owned): the
+ * split planes of q, dout, k, v (as many bytes as the tensors) and a few vectors. */
+int triposplat_b200_attention_backward(const float* dout, const float* q, const float* k,
+                                       const float* v, const float* out, const float* stats,
+                                       const int64_t* strides, const float* key_bias,
+                                       int bias_batches, int bias_heads, float* dq, float* dk,
+                                       float* dv, float* dbias, int B, int H, int Lq, int Lk);
+
 /* norm = 2-norm of all gradients together; each is scaled by min(1, max_norm / (norm + 1e-6)),
  * in place or into outs[i].  grads, outs (null: in place), sizes, dtypes are host arrays of
  * `count` entries; norm is one device float. */

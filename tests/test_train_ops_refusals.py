@@ -58,3 +58,19 @@ def test_clip(lib):
     assert call(ptr=None) == -1 and call(norm=None) == -1
     assert call(count=-1) == -2 and call(most=-1.0) == -2 and call(most=float("nan")) == -2 and call(size=-1) == -2
     assert call(dtype=3) == -3 and call(ptr=P + 2) == -4
+
+
+def test_attention(lib):
+    def fwd(q=P, bias=None, bb=1, bh=1, out=P, stats=P, B=2, H=2, Lq=1, Lk=1):
+        return lib.triposplat_b200_attention_forward(q, P, P, strides(9), bias, bb, bh, out, stats, B, H, Lq, Lk)
+
+    def bwd(dq=P, dbias=None, bias=None, B=2, Lq=1, Lk=1, dout=P):
+        return lib.triposplat_b200_attention_backward(dout, P, P, P, P, P, strides(24), bias, 1, 1, dq, P, P, dbias, B, 2,
+                                                      Lq, Lk)
+
+    assert fwd(q=None) == -1 and fwd(stats=None) == -1 and bwd(dq=None) == -1 and bwd(dbias=P) == -1
+    for bad in (dict(B=0), dict(H=0), dict(Lq=0), dict(Lk=0), dict(B=40000), dict(Lq=64 * 65535 + 1)):
+        assert fwd(**bad) == -2, bad
+    assert bwd(B=0) == -2 and bwd(Lk=0) == -2 and bwd(Lq=4000000, Lk=4000000) == -2
+    assert fwd(bias=P, bb=3) == -3 and fwd(bias=P, bh=3) == -3
+    assert fwd(q=P + 2) == -4 and fwd(out=P + 4) == -4 and fwd(stats=P + 4) == -4 and bwd(dout=P + 1) == -4

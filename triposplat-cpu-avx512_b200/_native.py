@@ -118,6 +118,8 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "triposplat_b200_norm_gate_backward": ([VP] * 17 + [I, I, I64, I, I, I, F], I),
     "triposplat_b200_axis_rope": ([VP] * 6 + [I, I, I64, I, I64, I, I, VP, I, I], I),
     "triposplat_b200_axis_rope_backward": ([VP] * 8 + [I, I, I64, I, I64, I, I, VP, I, I], I),
+    "triposplat_b200_attention_forward": ([VP] * 5 + [I, I, VP, VP] + [I] * 4, I),
+    "triposplat_b200_attention_backward": ([VP] * 8 + [I, I] + [VP] * 4 + [I] * 4, I),
     "triposplat_b200_clip_grad_norm": ([VP] * 4 + [I, F, VP], I),
     "triposplat_repo_phasor_f32_avx512": ([VP, VP, VP, I, VP, VP, I, VP, VP, I, VP, I64, I], I),
 }

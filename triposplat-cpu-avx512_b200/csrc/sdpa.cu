@@ -61,6 +61,7 @@
 
 #include "common.cuh"
 #include "runtime.h"
+#include "sdpa_planes.h"
 
 namespace tsb {
 namespace sdpa {
@@ -112,6 +113,9 @@ struct Params {
   __half* ohi;
   __half* olo;
   float* ors;
+  // nullable: per row (final reference maximum, row sum) for the backward pass; with it a row
+  // without a key is zeros instead of 0 / 0
+  float2* stats;
 };
 
 // 2^s for |s| <= 126 built in the exponent field: x * pow2i(s) is the correctly rounded
@@ -721,7 +725,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const float m = fmaxf(m_run, m0);
         const float f1 = m_run == m ? 1.0f : ex2(m_run - m);  // 0 for a team with no tiles
         const float f0 = m0 == m ? 1.0f : ex2(m0 - m);
-        const float f = vref / (l0 * f0 + l_run * f1);
+        const float l = l0 * f0 + l_run * f1;
+        float f = vref / l;
+        if (p.stats) {
+          if (l == 0.0f) f = 0.0f;
+          p.stats[(int64_t)bh * p.Lq + qrow] = make_float2(m, l * 0x1p-7f);  // the lift of P_LIFT taken out
+        }
         // dimensions 0..31 as team 0's own (o0 f0 + o1 f1), 32..63 as team 1's own
 #pragma unroll
         for (int d = 0; d < D; d += 4) {
@@ -1223,13 +1232,6 @@ static uint64_t now_ns() {
   return (uint64_t)ts.tv_sec * 1000000000ull + ts.tv_nsec;
 }
 
-// Attention inputs in the split format, in the library workspace of the current stream.
-struct SplitPlanesSdpa {
-  __half *qhi, *qlo, *khi, *klo, *vhi, *vlo;
-  float *qinv, *kinv, *vinv;
-  int T, Lkt;
-};
-
 static size_t al256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
 // Q planes of Lq rows per head: [qhi | qlo | qinv]
@@ -1269,15 +1271,21 @@ static void planes_from(uint8_t* q, uint8_t* kv, int64_t BH, int Lq, int Lk, Spl
   sp.vinv = reinterpret_cast<float*>(kv + ko[5]);
 }
 
-static int sdpa_planes(int64_t BH, int Lq, int Lk, cudaStream_t stream, SplitPlanesSdpa& sp) {
+int sdpa_planes_extra(int64_t BH, int Lq, int Lk, size_t extra, cudaStream_t stream, SplitPlanesSdpa& sp,
+                      void** behind) {
   size_t qo[2], ko[6];
   int T, Lkt;
   const size_t qbytes = q_planes_layout(BH, Lq, qo);
   const size_t kvbytes = kv_planes_layout(BH, Lk, ko, T, Lkt);
-  uint8_t* ws = static_cast<uint8_t*>(workspace(qbytes + kvbytes, stream));
+  uint8_t* ws = static_cast<uint8_t*>(workspace(qbytes + kvbytes + extra, stream));
   if (!ws) return kWorkspace;
   planes_from(ws, ws + qbytes, BH, Lq, Lk, sp);
+  if (behind) *behind = ws + qbytes + kvbytes;
   return kOk;
+}
+
+static int sdpa_planes(int64_t BH, int Lq, int Lk, cudaStream_t stream, SplitPlanesSdpa& sp) {
+  return sdpa_planes_extra(BH, Lq, Lk, 0, stream, sp, nullptr);
 }
 
 // Shared-memory opt-in of the fused split kernels, once per device.
@@ -1314,7 +1322,8 @@ static OutSplit out_split_of(void* out_split, int64_t B, int Lq, int H) {
 // The attention kernel on split planes.
 static int sdpa_attend(const SplitPlanesSdpa& sp, const float* bias, int64_t bias_bh_stride,
                        float* out, int64_t BH, int H, int Lq, int Lk, int out_blhd,
-                       cudaStream_t stream, const OutSplit& osplit = OutSplit()) {
+                       cudaStream_t stream, const OutSplit& osplit = OutSplit(),
+                       float2* stats = nullptr) {
   using namespace sdpa;
   CUtensorMap m_qhi, m_qlo, m_khi, m_klo, m_vhi, m_vlo;
   const uint32_t box_rows[3] = {64, 128, 1};
@@ -1362,7 +1371,7 @@ static int sdpa_attend(const SplitPlanesSdpa& sp, const float* bias, int64_t bia
   }
   const int Qt = (Lq + BQ - 1) / BQ;
   Params prm{sp.qinv, sp.kinv, sp.vinv, bias, (long long)bias_bh_stride, out, H, Lq, Lk, sp.T, out_blhd,
-             device_status(), Qt, (int)BH, osplit.hi, osplit.lo, osplit.rs};
+             device_status(), Qt, (int)BH, osplit.hi, osplit.lo, osplit.rs, stats};
   // persistent: one CTA per SM walking the (head, query tile) items
   static std::atomic<int> sm_count[64];
   int dev = 0;
@@ -1381,6 +1390,11 @@ static int sdpa_attend(const SplitPlanesSdpa& sp, const float* bias, int64_t bia
     sdpa_fwd_tc<<<grid, NUM_THREADS, SMEM_BYTES, stream>>>(m_qhi, m_qlo, m_khi, m_klo, m_vhi, m_vlo, prm);
   }
   return launch_status();
+}
+
+int sdpa_attend_stats(const SplitPlanesSdpa& sp, const float* bias, int64_t bias_bh_stride, float* out_blhd,
+                      float2* stats, int64_t BH, int H, int Lq, int Lk, cudaStream_t stream) {
+  return sdpa_attend(sp, bias, bias_bh_stride, out_blhd, BH, H, Lq, Lk, 1, stream, OutSplit(), stats);
 }
 
 // k/v element (bh, j, d) at base + bh*bh_stride + j*j_stride + d*d_stride

@@ -212,6 +212,70 @@ def norm_gate_backward(dz, dh, x, y, stats, *, gate=None, scale=None, shift=None
     return g
 
 
+# --------------------------------------------------------------------------------- attention
+def _attention_args(q, k, v, key_bias):
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("q, k, v must be [B, H, L, 64]")
+    B, H, Lq, D = q.shape
+    Lk = k.shape[2]
+    if D != 64 or min(B, H, Lq, Lk) < 1:
+        raise ValueError(f"unsupported shapes {tuple(q.shape)}, {tuple(k.shape)}: head_dim 64, no empty dimension")
+    _check(q, "q", (B, H, Lq, 64), torch.float32, q.device)
+    _check(k, "k", (B, H, Lk, 64), torch.float32, q.device)
+    _check(v, "v", (B, H, Lk, 64), torch.float32, q.device)
+    bias_dims = (1, 1)
+    if key_bias is not None:
+        shape = tuple(key_bias.shape)
+        if shape not in ((Lk,), (B, Lk), (B, H, Lk)):
+            raise ValueError(f"key_bias must be [Lk], [B, Lk] or [B, H, Lk], got {shape}")
+        key_bias = _param(key_bias, "key_bias", shape, q.device)
+        bias_dims = ((1, 1), (B, 1), (B, H))[len(shape) - 1]
+    return key_bias, bias_dims, (B, H, Lq, Lk)
+
+
+def attention_forward(q, k, v, *, key_bias=None):
+    """softmax(q k^T / 8 + key_bias) v on q [B, H, Lq, 64] and k, v [B, H, Lk, 64] (float32), key_bias
+    [Lk], [B, Lk] or [B, H, Lk].  A key with a bias of -inf does not exist; a query without keys
+    gives zeros.  Returns (out, stats): out [B, H, Lq, 64] in token-major storage
+    ([B, Lq, H, 64], what the out-projection reads), stats [B, H, Lq, 2] for the backward pass.
+    Heads shared by several queries' heads are passed expanded."""
+    key_bias, bias_dims, (B, H, Lq, Lk) = _attention_args(q, k, v, key_bias)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    out = torch.empty((B, Lq, H, 64), dtype=torch.float32, device=q.device)
+    stats = torch.empty((B, H, Lq, 2), dtype=torch.float32, device=q.device)
+    lib = _lib(q.device)
+    _ok(lib, lib.triposplat_b200_attention_forward(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _i64(*(s for t in (q, k, v) for s in t.stride()[:3])),
+        _ptr(key_bias), *bias_dims, out.data_ptr(), stats.data_ptr(), B, H, Lq, Lk), "attention_forward")
+    return out.transpose(1, 2), stats
+
+
+def attention_backward(dout, q, k, v, out, stats, *, key_bias=None, grads=None, bias_grad=True):
+    """Gradients (dq, dk, dv, dbias) of ``attention_forward`` with the incoming dout [B, H, Lq, 64].
+
+    ``grads`` may name the three tensors to write (e.g. slices of a packed gradient); otherwise they
+    are new, in token-major storage.  dbias has key_bias's shape (None without a bias or with
+    ``bias_grad=False``)."""
+    key_bias, bias_dims, (B, H, Lq, Lk) = _attention_args(q, k, v, key_bias)
+    dev = q.device
+    dout = _rows(_check(dout, "dout", q.shape, torch.float32, dev))
+    out = _rows(_check(out, "out", q.shape, torch.float32, dev))
+    stats = _check(stats, "stats", (B, H, Lq, 2), torch.float32, dev).contiguous()
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    if grads is None:
+        dq, dk, dv = (torch.empty((B, n, H, 64), dtype=torch.float32, device=dev).transpose(1, 2)
+                      for n in (Lq, Lk, Lk))
+    else:
+        dq, dk, dv = (_out_like(g, like, "grads") for g, like in zip(grads, (q, k, v), strict=True))
+    dbias = torch.empty_like(key_bias) if key_bias is not None and bias_grad else None
+    lib = _lib(dev)
+    _ok(lib, lib.triposplat_b200_attention_backward(
+        dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), stats.data_ptr(),
+        _i64(*(s for t in (dout, q, k, v, out, dq, dk, dv) for s in t.stride()[:3])), _ptr(key_bias), *bias_dims,
+        dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dbias), B, H, Lq, Lk), "attention_backward")
+    return dq, dk, dv, dbias
+
+
 # -------------------------------------------------------------------- gradient norm, clipping
 def clip_grad_norm(grads, max_norm, *, out=None):
     """Scales the gradients (a sequence of contiguous tensors, float32, bfloat16 and float16
