@@ -17,7 +17,10 @@
 //
 // Bound by HBM: every tensor is read or written once.  A row is held in registers (8 or 16
 // elements per thread) by one warp (up to 256 columns) or one block, statistics are taken
-// in two passes over the registers (mean, then centred squares) in fp32.
+// in two passes over the registers (mean, then centred squares) in fp32.  A row group keeps its
+// columns' coefficients (rho gate w_post, (1 + scale) w_pre, shift) in registers over all its rows,
+// and (up to 4096 columns; beyond, registers are short) the next row's loads are in flight while a
+// row is worked on.
 #include <stdint.h>
 
 #include <initializer_list>
@@ -91,19 +94,26 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[NI][VEC], int kind,
   return make_float2(mean, 1.0f / sqrtf(q / (float)C + eps));
 }
 
+// A row's elements of one tensor as they lie in memory, and as numbers (zeros past C).
 template <class T, int VEC, int NI>
-__device__ __forceinline__ void load_row(const T* p, int C, float (&v)[NI][VEC]) {
+struct RawRow {
+  Pack<T, VEC> v[NI];
+  __device__ __forceinline__ void load(const T* p, int C) {
 #pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
-    if (c < C) {
-      load_vec<T, VEC>(p + c, v[i]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[i][e] = 0.0f;
+    for (int i = 0; i < NI; ++i) {
+      const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
+      if (c < C) v[i] = *reinterpret_cast<const Pack<T, VEC>*>(p + c);
     }
   }
-}
+  __device__ __forceinline__ void get(int C, float (&f)[NI][VEC]) const {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[i][e] = c < C ? to_f32(v[i].v[e]) : 0.0f;
+    }
+  }
+};
 
 template <class T, int VEC, int NI>
 __device__ __forceinline__ void store_row(T* p, int C, const float (&v)[NI][VEC]) {
@@ -114,57 +124,59 @@ __device__ __forceinline__ void store_row(T* p, int C, const float (&v)[NI][VEC]
   }
 }
 
-// per-column fp32 parameter (null: `other`)
-template <int VEC>
-__device__ __forceinline__ void load_par(const float* p, int c, float other, float (&v)[VEC]) {
-  if (p == nullptr) {
+// a[c] * (b[c] + add) (null: a = 1, b = 0), zeros past C
+template <int VEC, int NI>
+__device__ __forceinline__ void load_coef(const float* a, const float* b, float add, int C, float (&v)[NI][VEC]) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = other;
-    return;
+  for (int i = 0; i < NI; ++i) {
+    const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      v[i][e] = c < C ? (a ? __ldg(a + c + e) : 1.0f) * ((b ? __ldg(b + c + e) : 0.0f) + add) : 0.0f;
   }
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) v[e] = __ldg(p + c + e);
 }
 
-template <class T, int VEC, int NI>
-__global__ void __launch_bounds__(kMaxThreads) norm_gate_k(const Args a) {
+// Row group g of batch entry blockIdx.y takes the entry's rows g, g + groups, g + 2 groups, ...
+template <class T, int VEC, int NI, int MAXT>
+__global__ void __launch_bounds__(MAXT, 1) norm_gate_k(const Args a) {
   __shared__ float2 sm[2][32];
   int turn = 0;
-  const int64_t rows = (int64_t)a.B * a.L;
-  for (int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; r < rows;
-       r += (int64_t)gridDim.x * blockDim.y) {
-    const int64_t b = r / a.L, l = r - b * a.L;
+  const int64_t b = blockIdx.y, g = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  const T* x = static_cast<const T*>(a.x) + b * a.xb;
+  const T* y = static_cast<const T*>(a.y) + b * a.yb;
+  RawRow<T, VEC, NI> ry, rx;
+  auto fetch = [&](int64_t l) {
+    ry.load(y + l * a.yl, a.C);
+    rx.load(x + l * a.xl, a.C);
+  };
+  constexpr bool kAhead = NI * VEC <= 8;
+  if (kAhead && g < a.L) fetch(g);
+  float gw[NI][VEC], sw[NI][VEC], sh[NI][VEC];
+  load_coef<VEC, NI>(a.wpost, a.gate ? a.gate + b * a.C : nullptr, a.gate ? 0.0f : 1.0f, a.C, gw);
+  load_coef<VEC, NI>(a.wpre, a.scale ? a.scale + b * a.C : nullptr, 1.0f, a.C, sw);
+  load_coef<VEC, NI>(nullptr, a.shift ? a.shift + b * a.C : nullptr, 0.0f, a.C, sh);
+#pragma unroll 1
+  for (int64_t l = g; l < a.L; l += a.groups) {
+    const int64_t r = b * a.L + l;
     float z[NI][VEC], m[NI][VEC];
-    load_row<T, VEC, NI>(static_cast<const T*>(a.y) + b * a.yb + l * a.yl, a.C, m);
-    load_row<T, VEC, NI>(static_cast<const T*>(a.x) + b * a.xb + l * a.xl, a.C, z);
+    if (!kAhead) fetch(l);
+    ry.get(a.C, m);
+    rx.get(a.C, z);
+    if (kAhead && l + a.groups < a.L) fetch(l + a.groups);
     float2 sp = make_float2(0.0f, 1.0f), sn = make_float2(0.0f, 1.0f);
     if (a.post != kNone) sp = row_stats<VEC, NI>(m, a.post, a.C, a.eps, sm, turn);
+    const float rs = sp.y * a.rho;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
-      if (c >= a.C) continue;
-      float g[VEC], w[VEC];
-      load_par<VEC>(a.gate ? a.gate + b * a.C : nullptr, c, 1.0f, g);
-      load_par<VEC>(a.wpost, c, 1.0f, w);
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        z[i][e] = fmaf((m[i][e] - sp.x) * sp.y * w[e], g[e] * a.rho, z[i][e]);
-    }
+      for (int e = 0; e < VEC; ++e) z[i][e] = fmaf((m[i][e] - sp.x) * rs, gw[i][e], z[i][e]);
     store_row<T, VEC, NI>(static_cast<T*>(a.out0) + r * a.C, a.C, z);
     if (a.pre != kNone) {
       sn = row_stats<VEC, NI>(z, a.pre, a.C, a.eps, sm, turn);
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
-        if (c >= a.C) continue;
-        float s[VEC], t[VEC], w[VEC];
-        load_par<VEC>(a.scale ? a.scale + b * a.C : nullptr, c, 0.0f, s);
-        load_par<VEC>(a.shift ? a.shift + b * a.C : nullptr, c, 0.0f, t);
-        load_par<VEC>(a.wpre, c, 1.0f, w);
+      for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          z[i][e] = fmaf((z[i][e] - sn.x) * sn.y * w[e], 1.0f + s[e], t[e]);
-      }
+        for (int e = 0; e < VEC; ++e) z[i][e] = fmaf((z[i][e] - sn.x) * sn.y, sw[i][e], sh[i][e]);
       store_row<T, VEC, NI>(static_cast<T*>(a.out1) + r * a.C, a.C, z);
     }
     if (threadIdx.x == 0)
@@ -172,106 +184,112 @@ __global__ void __launch_bounds__(kMaxThreads) norm_gate_k(const Args a) {
   }
 }
 
-// Row group g of batch entry blockIdx.y takes the entry's rows [g * chunk, (g + 1) * chunk).
-template <class T, int VEC, int NI>
-__global__ void __launch_bounds__(kMaxThreads) norm_gate_bwd_k(const Args a) {
+template <class T, int VEC, int NI, int MAXT>
+__global__ void __launch_bounds__(MAXT, 1) norm_gate_bwd_k(const Args a) {
   __shared__ float2 sm[2][32];
   int turn = 0;
-  const int b = blockIdx.y, g = blockIdx.x * blockDim.y + threadIdx.y;
-  const int64_t chunk = (a.L + a.groups - 1) / a.groups;
-  const int64_t l1 = min(a.L, (g + 1) * chunk);
+  const int64_t b = blockIdx.y, g = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const float inv_c = 1.0f / (float)a.C;
+  const T* x = static_cast<const T*>(a.x) + b * a.xb;
+  const T* y = static_cast<const T*>(a.y) + b * a.yb;
+  const bool has_h = a.dh != nullptr, has_z = a.dz != nullptr;
+  const T* dh = has_h ? static_cast<const T*>(a.dh) + b * a.hb : nullptr;
+  const T* dz = has_z ? static_cast<const T*>(a.dz) + b * a.zb : nullptr;
+  RawRow<T, VEC, NI> ry, rx, rh, rz;
+  float4 st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
+  auto fetch = [&](int64_t l) {
+    ry.load(y + l * a.yl, a.C);
+    rx.load(x + l * a.xl, a.C);
+    if (has_h) rh.load(dh + l * a.hl, a.C);
+    if (has_z) rz.load(dz + l * a.zl, a.C);
+    st = __ldg(reinterpret_cast<const float4*>(a.stats + 4 * (b * a.L + l)));
+  };
+  constexpr bool kAhead = NI * VEC <= 8;
+  if (kAhead && g < a.L) fetch(g);
+  float gw[NI][VEC], sw[NI][VEC];
+  load_coef<VEC, NI>(a.wpost, a.gate ? a.gate + b * a.C : nullptr, a.gate ? 0.0f : 1.0f, a.C, gw);
+  load_coef<VEC, NI>(a.wpre, a.scale ? a.scale + b * a.C : nullptr, 1.0f, a.C, sw);
   float a0[NI][VEC], a1[NI][VEC], a2[NI][VEC];
 #pragma unroll
   for (int i = 0; i < NI; ++i)
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) a0[i][e] = a1[i][e] = a2[i][e] = 0.0f;
-  for (int64_t l = g * chunk; l < l1; ++l) {
+    for (int e = 0; e < VEC; ++e) {
+      a0[i][e] = a1[i][e] = a2[i][e] = 0.0f;
+      gw[i][e] *= a.rho;
+    }
+#pragma unroll 1
+  for (int64_t l = g; l < a.L; l += a.groups) {
     const int64_t r = b * a.L + l;
-    float n[NI][VEC], m[NI][VEC], d[NI][VEC];
-    load_row<T, VEC, NI>(static_cast<const T*>(a.y) + b * a.yb + l * a.yl, a.C, m);
-    load_row<T, VEC, NI>(static_cast<const T*>(a.x) + b * a.xb + l * a.xl, a.C, n);
-    const float4 st = __ldg(reinterpret_cast<const float4*>(a.stats + 4 * r));
+    float n[NI][VEC], m[NI][VEC], d[NI][VEC], dzv[NI][VEC];
+    if (!kAhead) fetch(l);
+    ry.get(a.C, m);
+    rx.get(a.C, n);
+    const float4 s4 = st;
+    if (has_h) rh.get(a.C, d);
+    if (has_z) rz.get(a.C, dzv);
+    if (kAhead && l + a.groups < a.L) fetch(l + a.groups);
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
-      if (c >= a.C) continue;
-      float gt[VEC], w[VEC];
-      load_par<VEC>(a.gate ? a.gate + (int64_t)b * a.C : nullptr, c, 1.0f, gt);
-      load_par<VEC>(a.wpost, c, 1.0f, w);
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        m[i][e] = (m[i][e] - st.x) * st.y;
-        n[i][e] = (fmaf(m[i][e] * w[e], gt[e] * a.rho, n[i][e]) - st.z) * st.w;
+        m[i][e] = (m[i][e] - s4.x) * s4.y;
+        n[i][e] = (fmaf(m[i][e], gw[i][e], n[i][e]) - s4.z) * s4.w;
       }
-    }
-    if (a.pre != kNone && a.dh != nullptr) {
-      load_row<T, VEC, NI>(static_cast<const T*>(a.dh) + b * a.hb + l * a.hl, a.C, d);
+    if (has_h) {
+      // columns past C hold d = 0 (and a coefficient of 0), whatever n is there
       float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
-        if (c >= a.C) continue;
-        float sc[VEC], w[VEC];
-        load_par<VEC>(a.scale ? a.scale + (int64_t)b * a.C : nullptr, c, 0.0f, sc);
-        load_par<VEC>(a.wpre, c, 1.0f, w);
+      for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           a0[i][e] += d[i][e];
           a1[i][e] = fmaf(d[i][e], n[i][e], a1[i][e]);
-          d[i][e] *= (1.0f + sc[e]) * w[e];
+          d[i][e] *= sw[i][e];
           s.x += d[i][e];
           s.y = fmaf(d[i][e], n[i][e], s.y);
         }
-      }
       s = row_sum(s, sm, turn);
       const float mean = a.pre == kLayer ? s.x * inv_c : 0.0f, dot = s.y * inv_c;
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) d[i][e] = st.w * (d[i][e] - mean - n[i][e] * dot);
+        for (int e = 0; e < VEC; ++e) d[i][e] = s4.w * (d[i][e] - mean - n[i][e] * dot);
     } else {
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) d[i][e] = 0.0f;
     }
-    if (a.dz != nullptr) {
-      load_row<T, VEC, NI>(static_cast<const T*>(a.dz) + b * a.zb + l * a.zl, a.C, n);
+    if (has_z) {
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) d[i][e] += n[i][e];
+        for (int e = 0; e < VEC; ++e) d[i][e] += dzv[i][e];
     }
     store_row<T, VEC, NI>(static_cast<T*>(a.out0) + r * a.C, a.C, d);
+    // gw is 0 past C: those columns stay out of the sums, and a2 there is never stored
     float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
-      if (c >= a.C) continue;
-      float gt[VEC], w[VEC];
-      load_par<VEC>(a.gate ? a.gate + (int64_t)b * a.C : nullptr, c, 1.0f, gt);
-      load_par<VEC>(a.wpost, c, 1.0f, w);
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         a2[i][e] = fmaf(d[i][e], m[i][e], a2[i][e]);
-        d[i][e] *= gt[e] * a.rho * w[e];
+        d[i][e] *= gw[i][e];
         s.x += d[i][e];
         s.y = fmaf(d[i][e], m[i][e], s.y);
       }
-    }
     if (a.post != kNone) {
       s = row_sum(s, sm, turn);
       const float mean = a.post == kLayer ? s.x * inv_c : 0.0f, dot = s.y * inv_c;
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) d[i][e] = st.y * (d[i][e] - mean - m[i][e] * dot);
+        for (int e = 0; e < VEC; ++e) d[i][e] = s4.y * (d[i][e] - mean - m[i][e] * dot);
     }
     store_row<T, VEC, NI>(static_cast<T*>(a.out1) + r * a.C, a.C, d);
   }
   if (a.part == nullptr || g >= a.groups) return;
-  float* p = a.part + ((int64_t)b * a.groups + g) * 3 * a.C;
+  float* p = a.part + (b * a.groups + g) * 3 * a.C;
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
@@ -292,45 +310,41 @@ struct ReduceArgs {
   float rho;
 };
 
-// 32 columns per block, 32 threads per column; partial rows added in a fixed order.
+// 32 columns of one of the three sums (blockIdx.y) per block, 32 threads per column; partial rows
+// added in a fixed order.
 __global__ void __launch_bounds__(1024) norm_gate_reduce_k(const ReduceArgs a) {
-  __shared__ float sm[3][32][33];
-  const int c = blockIdx.x * 32 + threadIdx.x, y = threadIdx.y;
-  float wp = 0.0f, wq = 0.0f;
+  __shared__ float sm[32][33];
+  const int c = blockIdx.x * 32 + threadIdx.x, y = threadIdx.y, q = blockIdx.y;
+  float dw = 0.0f;
   for (int b = 0; b < a.B; ++b) {
-    float s[3] = {0.0f, 0.0f, 0.0f};
+    float s = 0.0f;
     if (c < a.C) {
-      const float* p = a.part + (int64_t)b * a.groups * 3 * a.C + c;
-#pragma unroll 4
-      for (int g = y; g < a.groups; g += 32) {
-#pragma unroll
-        for (int q = 0; q < 3; ++q) s[q] += p[((int64_t)g * 3 + q) * a.C];
-      }
+      const float* p = a.part + ((int64_t)b * a.groups * 3 + q) * a.C + c;
+#pragma unroll 8
+      for (int g = y; g < a.groups; g += 32) s += p[(int64_t)g * 3 * a.C];
     }
-#pragma unroll
-    for (int q = 0; q < 3; ++q) sm[q][threadIdx.x][y] = s[q];
-    __syncthreads();
-    if (y < 3) {  // warp y adds quantity y, one column per lane
-      float t = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 32; ++j) t += sm[y][threadIdx.x][j];
-      sm[y][threadIdx.x][32] = t;
-    }
+    sm[threadIdx.x][y] = s;
     __syncthreads();
     if (y == 0 && c < a.C) {
-      const float s0 = sm[0][threadIdx.x][32], s1 = sm[1][threadIdx.x][32], s2 = sm[2][threadIdx.x][32];
+      s = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) s += sm[threadIdx.x][j];
       const int64_t bc = (int64_t)b * a.C + c;
-      if (a.dshift) a.dshift[bc] = s0;
-      if (a.dscale) a.dscale[bc] = s1 * (a.wpre ? a.wpre[c] : 1.0f);
-      if (a.dgate) a.dgate[bc] = s2 * a.rho * (a.wpost ? a.wpost[c] : 1.0f);
-      wp = fmaf(1.0f + (a.scale ? a.scale[bc] : 0.0f), s1, wp);
-      wq = fmaf(a.rho * (a.gate ? a.gate[bc] : 1.0f), s2, wq);
+      if (q == 0) {
+        if (a.dshift) a.dshift[bc] = s;
+      } else if (q == 1) {
+        if (a.dscale) a.dscale[bc] = s * (a.wpre ? a.wpre[c] : 1.0f);
+        dw = fmaf(1.0f + (a.scale ? a.scale[bc] : 0.0f), s, dw);
+      } else {
+        if (a.dgate) a.dgate[bc] = s * a.rho * (a.wpost ? a.wpost[c] : 1.0f);
+        dw = fmaf(a.rho * (a.gate ? a.gate[bc] : 1.0f), s, dw);
+      }
     }
     __syncthreads();
   }
   if (y == 0 && c < a.C) {
-    if (a.dwpre) a.dwpre[c] = wp;
-    if (a.dwpost) a.dwpost[c] = wq;
+    if (q == 1 && a.dwpre) a.dwpre[c] = dw;
+    if (q == 2 && a.dwpost) a.dwpost[c] = dw;
   }
 }
 
@@ -360,15 +374,25 @@ static Shape shape_of(int C) {
   return s;
 }
 
+// Row groups per batch entry so that about `threads` threads per SM run, one row per group at least.
+static dim3 grid_of(Args& a, const Shape& s, int threads) {
+  const int64_t per_sm = threads / (int)s.block.x > 0 ? threads / (int)s.block.x : 1;
+  const int64_t want = (sm_count() * per_sm + a.B - 1) / a.B;
+  a.groups = (int)(want < a.L ? want : a.L);
+  return dim3((a.groups + s.block.y - 1) / s.block.y, a.B);
+}
+
 template <class T, int VEC>
-static void launch_fwd(const Args& a, const Shape& s, unsigned grid, cudaStream_t st) {
-  if (s.wide) norm_gate_k<T, VEC, 16 / VEC><<<grid, s.block, 0, st>>>(a);
-  else norm_gate_k<T, VEC, 8 / VEC><<<grid, s.block, 0, st>>>(a);
+static void launch_fwd(const Args& a, const Shape& s, dim3 grid, cudaStream_t st) {
+  if (s.wide) norm_gate_k<T, VEC, 16 / VEC, kMaxThreads><<<grid, s.block, 0, st>>>(a);
+  else if (s.block.x > 256) norm_gate_k<T, VEC, 8 / VEC, kMaxThreads><<<grid, s.block, 0, st>>>(a);
+  else norm_gate_k<T, VEC, 8 / VEC, 256><<<grid, s.block, 0, st>>>(a);
 }
 template <class T, int VEC>
 static void launch_bwd(const Args& a, const Shape& s, dim3 grid, cudaStream_t st) {
-  if (s.wide) norm_gate_bwd_k<T, VEC, 16 / VEC><<<grid, s.block, 0, st>>>(a);
-  else norm_gate_bwd_k<T, VEC, 8 / VEC><<<grid, s.block, 0, st>>>(a);
+  if (s.wide) norm_gate_bwd_k<T, VEC, 16 / VEC, kMaxThreads><<<grid, s.block, 0, st>>>(a);
+  else if (s.block.x > 256) norm_gate_bwd_k<T, VEC, 8 / VEC, kMaxThreads><<<grid, s.block, 0, st>>>(a);
+  else norm_gate_bwd_k<T, VEC, 8 / VEC, 256><<<grid, s.block, 0, st>>>(a);
 }
 
 // whether a tensor's pointer is not a multiple of its element's size
@@ -416,9 +440,7 @@ int triposplat_b200_norm_gate(const void* x, const void* y, const int64_t* strid
                         static_cast<const void*>(pre_weight), static_cast<const void*>(post_weight)})
     if (p && !is_device_pointer(p)) return kNotDevicePointer;
   const ng::Shape s = ng::shape_of(C);
-  const int64_t blocks = ((int64_t)B * L + s.block.y - 1) / s.block.y;
-  const int64_t cap = (int64_t)sm_count() * (2048 / (s.block.x * s.block.y)) * 4;
-  const unsigned grid = (unsigned)(blocks < cap ? blocks : cap);
+  const dim3 grid = ng::grid_of(a, s, 768);
   const bool vec = ng::vec_ok(a, dtype_size(dtype));
   cudaStream_t stream = current_stream();
   LaunchScope scope(kKElementwise, stream);
@@ -459,15 +481,12 @@ int triposplat_b200_norm_gate_backward(const void* dz, const void* dh, const voi
     if (p && !is_device_pointer(p)) return kNotDevicePointer;
   const ng::Shape s = ng::shape_of(C);
   cudaStream_t stream = current_stream();
-  // row groups per batch entry: about 512 threads per SM in flight, one row per group at least
-  const int64_t want = ((int64_t)sm_count() * (512 / s.block.x > 0 ? 512 / s.block.x : 1) + B - 1) / B;
-  a.groups = (int)(want < L ? want : L);
+  const dim3 grid = ng::grid_of(a, s, 512);
   const bool sums = dgate || dscale || dshift || dpre_weight || dpost_weight;
   if (sums) {
     a.part = static_cast<float*>(workspace((size_t)B * a.groups * 3 * C * sizeof(float), stream));
     if (!a.part) return kWorkspace;
   }
-  const dim3 grid((a.groups + s.block.y - 1) / s.block.y, B);
   const bool vec = ng::vec_ok(a, dtype_size(dtype));
   {
     LaunchScope scope(kKElementwise, stream);
@@ -481,7 +500,7 @@ int triposplat_b200_norm_gate_backward(const void* dz, const void* dh, const voi
     const ng::ReduceArgs ra{a.part, gate, scale, pre_weight, post_weight, dgate, dscale, dshift, dpre_weight,
                             dpost_weight, B, C, a.groups, residual_scale};
     LaunchScope scope(kKElementwise, stream);
-    ng::norm_gate_reduce_k<<<(C + 31) / 32, dim3(32, 32), 0, stream>>>(ra);
+    ng::norm_gate_reduce_k<<<dim3((C + 31) / 32, 3), dim3(32, 32), 0, stream>>>(ra);
   }
   return launch_status();
 }
