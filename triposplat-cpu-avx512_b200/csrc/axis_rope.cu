@@ -11,12 +11,12 @@
 // their accuracy; a pair and token costs one, all heads share it), sine and cosine in fp32.
 //
 // Bound by HBM: x is read and y written once.  A head's vector belongs to a group of 1 to 32
-// lanes, VEC pairs (two 16-byte accesses) each; the groups of a block take different heads of
-// one token (adjacent in memory) and, with few heads, several tokens.  A block walks tiles of a few
-// tokens: it issues the tile's loads, then its threads put the tokens' cosines and sines into
-// shared memory (two buffers, one barrier per tile), then each group turns its vectors.  A group
-// keeps its head: gamma stays in registers, and so does its part of dgamma, over all tiles of
-// the block; a second kernel adds the blocks' partial rows in a fixed order (no atomics).
+// lanes, four pairs (two accesses of 16 bytes, or 8 of a 16-bit type) each; the groups of a block
+// take different heads of one token (adjacent in memory) and, with few heads, several tokens.  A block
+// walks chunks of tokens: its threads put the chunk's cosines and sines into shared memory once,
+// then each group walks its head's vectors with the next step's loads in flight.  gamma stays in
+// registers, and so does a group's part of dgamma, over all chunks of the block; a second kernel
+// adds the blocks' partial rows in a fixed order (no atomics).
 #include <stdint.h>
 
 #include <initializer_list>
@@ -30,7 +30,7 @@ namespace rope {
 
 constexpr int kMaxAxes = 4;
 constexpr int kMaxDim = 256;
-constexpr int kThreads = 256;
+constexpr int kThreads = 384;  // most per block
 
 enum PosType : int { kInt32 = 0, kInt64 = 1, kFloat = 2 };
 
@@ -48,7 +48,8 @@ struct Args {
   float sq;                      // sqrt(D)
   int B, lanes;                  // lanes per vector (a power of two)
   int heads, token_groups;       // heads and token groups of a block
-  int64_t tiles;                 // tiles per batch entry
+  int steps;                     // steps of U * token_groups tokens in a chunk
+  int64_t chunks;                // chunks per batch entry
 };
 
 __device__ __forceinline__ double position(const Args& a, int64_t i) {
@@ -70,7 +71,8 @@ __device__ __forceinline__ float2 turn_of(double pos, float f) {
 }
 
 // VEC pairs of a head, as two runs of VEC elements.  Interleaved, the runs follow each other and
-// pair i is (2i, 2i + 1) of both together; in halves, pair i is element i of each run.
+// pair i is (2i, 2i + 1) of both together; in halves, pair i is element i of each run.  A single
+// pair is the same either way and uses the second form.
 template <class T, int VEC>
 struct Slot {
   Pack<T, VEC> a, b;
@@ -108,16 +110,17 @@ struct Slot {
   }
 };
 
-// tokens that a group has in flight at once
+// tokens of one step of a group
 template <bool BWD, int K>
-__host__ __device__ constexpr int tokens_at_once() { return K > 1 ? 1 : (BWD ? 2 : 4); }
+__host__ __device__ constexpr int tokens_at_once() { return K > 1 || BWD ? 1 : 2; }
 
 // K slots per lane, `lanes` apart.
-template <class T, int VEC, int K, bool HALVES, bool BWD>
-__global__ void __launch_bounds__(kThreads) axis_rope_k(const Args a) {
+template <class T, int VEC, int K, bool HALVES, bool BWD, bool NORM>
+__global__ void __launch_bounds__(kThreads, K > 1 ? 1 : 2) axis_rope_k(const Args a) {
   constexpr int U = tokens_at_once<BWD, K>();
-  extern __shared__ float2 table[];  // [2][tile tokens][D / 2]
-  const int half = a.D / 2, tile_tokens = a.token_groups * U;
+  // [chunk tokens][VEC][D / 2 / VEC]: the lanes of a vector read neighbouring entries
+  extern __shared__ float2 cs[];
+  const int half = a.D / 2, step_tokens = a.token_groups * U, chunk_tokens = step_tokens * a.steps;
   const int lane = threadIdx.x & (a.lanes - 1), group = threadIdx.x / a.lanes;
   const int tg = group / a.heads, h = blockIdx.y * a.heads + group - tg * a.heads;
   const bool active = tg < a.token_groups && h < a.H;
@@ -128,49 +131,51 @@ __global__ void __launch_bounds__(kThreads) axis_rope_k(const Args a) {
   for (int k = 0; k < K; ++k) {
     p0[k] = (lane + k * a.lanes) * VEC;
     live[k] = active && p0[k] < half;
-    const bool apart = HALVES && p0[k] < a.P;
+    const bool apart = a.halves && p0[k] < a.P;
     e0[k] = apart ? p0[k] : 2 * p0[k];
     e1[k] = apart ? a.P + p0[k] : e0[k] + VEC;
-    Slot<float, VEC> gs;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) gs.a.v[i] = gs.b.v[i] = 1.0f;
-    if (a.gamma && live[k]) {
-      const float* gp = a.gamma + (int64_t)h * a.D;
+    if (NORM) {
+      Slot<float, VEC> gs;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        gs.a.v[i] = __ldg(gp + e0[k] + i);
-        gs.b.v[i] = __ldg(gp + e1[k] + i);
+        gs.a.v[i] = live[k] ? __ldg(a.gamma + (int64_t)h * a.D + e0[k] + i) : 0.0f;
+        gs.b.v[i] = live[k] ? __ldg(a.gamma + (int64_t)h * a.D + e1[k] + i) : 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        g[k][i] = gs.template pair<HALVES>(i);
+        acc[k][i] = make_float2(0.0f, 0.0f);
       }
     }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      g[k][i] = gs.template pair<HALVES>(i);
-      acc[k][i] = make_float2(0.0f, 0.0f);
-    }
   }
-  int turn = 0;
-  const int64_t all = a.tiles * a.B;
+  const int slots = half / VEC;
+  const int64_t all = a.chunks * a.B;
 #pragma unroll 1
-  for (int64_t tile = blockIdx.x; tile < all; tile += gridDim.x) {
-    const int64_t b = tile / a.tiles, l0 = (tile - b * a.tiles) * tile_tokens;
+  for (int64_t chunk = blockIdx.x; chunk < all; chunk += gridDim.x) {
+    const int64_t b = chunk / a.chunks, l0 = (chunk - b * a.chunks) * chunk_tokens;
+    const int tokens = (int)min((int64_t)chunk_tokens, a.L - l0);
+    const T* x = static_cast<const T*>(a.x) + h * a.xh + b * a.xb + (l0 + tg) * a.xl;
+    const T* dy = static_cast<const T*>(a.dy) + h * a.dh + b * a.db + (l0 + tg) * a.dl;
+    T* y = static_cast<T*>(a.y) + h * a.yh + b * a.yb + (l0 + tg) * a.yl;
+    const int64_t dxl = a.token_groups * a.xl, ddl = a.token_groups * a.dl, dyl = a.token_groups * a.yl;
     Slot<T, VEC> xs[U][K], ds[U][K];
-    // the tile's loads first: they fly while the table is made
+    // the next step's loads (nothing past the chunk's end)
+    auto fetch = [&](int t) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t l = l0 + u * a.token_groups + tg;
+      for (int u = 0; u < U; ++u, t += a.token_groups, x += dxl, dy += ddl) {
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (live[k] && l < a.L) {
-          if (!BWD || a.gamma) xs[u][k].load(static_cast<const T*>(a.x) + b * a.xb + l * a.xl + h * a.xh, e0[k], e1[k]);
-          if (BWD) ds[u][k].load(static_cast<const T*>(a.dy) + b * a.db + l * a.dl + h * a.dh, e0[k], e1[k]);
-        }
-    }
-    float2* cs = table + turn * tile_tokens * half;
-    turn ^= 1;
-    for (int i = threadIdx.x; i < tile_tokens * half; i += kThreads) {
-      const int t = i / half, p = i - t * half;
+        for (int k = 0; k < K; ++k)
+          if (live[k] && t < tokens) {
+            if (!BWD || NORM) xs[u][k].load(x, e0[k], e1[k]);
+            if (BWD) ds[u][k].load(dy, e0[k], e1[k]);
+          }
+      }
+    };
+    fetch(tg);  // in flight while the table is made
+    for (int i = threadIdx.x; i < tokens * half; i += blockDim.x) {
+      const int t = i / half, q = i - t * half, p = q % slots * VEC + q / slots;
       float2 w = make_float2(1.0f, 0.0f);
-      if (p < a.P && l0 + t < a.L) {
+      if (p < a.P) {
         int axis = 0;
         while (p >= a.ends[axis]) ++axis;
         w = turn_of(position(a, b * a.pos_batch + (l0 + t) * a.axes + axis), a.inv_freq[p]);
@@ -178,78 +183,83 @@ __global__ void __launch_bounds__(kThreads) axis_rope_k(const Args a) {
       cs[i] = w;
     }
     __syncthreads();
-    float2 r[U][K][VEC];
-    float ss[U], dot[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      ss[u] = dot[u] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          r[u][k][i] = make_float2(0.0f, 0.0f);
-          if (!live[k]) continue;
-          if (!BWD || a.gamma) {
-            const float2 w = cs[(u * a.token_groups + tg) * half + p0[k] + i];
-            const float2 v = xs[u][k].template pair<HALVES>(i);
-            r[u][k][i] = make_float2(v.x * w.x - v.y * w.y, v.x * w.y + v.y * w.x);
-            ss[u] = fmaf(r[u][k][i].x, r[u][k][i].x, fmaf(r[u][k][i].y, r[u][k][i].y, ss[u]));
-            if (BWD) {
-              const float2 d = ds[u][k].template pair<HALVES>(i);
-              dot[u] = fmaf(d.x * g[k][i].x, r[u][k][i].x, fmaf(d.y * g[k][i].y, r[u][k][i].y, dot[u]));
-            }
-          }
-        }
-    }
-    float f[U], back[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) f[u] = 1.0f, back[u] = 0.0f;
-    if (a.gamma) {
 #pragma unroll 1
-      for (int o = a.lanes / 2; o > 0; o >>= 1)
+    for (int t0 = 0; t0 < tokens; t0 += step_tokens) {
+      Slot<T, VEC> xc[U][K], dc[U][K];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          ss[u] += __shfl_xor_sync(0xffffffffu, ss[u], o);
-          if (BWD) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], o);
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (!BWD || NORM) xc[u][k] = xs[u][k];
+          if (BWD) dc[u][k] = ds[u][k];
         }
+      fetch(t0 + step_tokens + tg);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const float n = sqrtf(ss[u]);
-        f[u] = a.sq / fmaxf(n, 1.0e-12f);
-        if (BWD) back[u] = n > 1.0e-12f ? dot[u] / (n * n) : 0.0f;
-      }
-    }
+      for (int u = 0; u < U; ++u, y += dyl) {
+        const int t = t0 + u * a.token_groups + tg;
+        const bool here = t < tokens;
+        const float2* w = cs + (here ? t : 0) * half + lane;
+        float2 r[K][VEC];
+        float ss = 0.0f, dot = 0.0f;
+        if (!BWD || NORM) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t l = l0 + u * a.token_groups + tg;
+          for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (!live[k] || l >= a.L) continue;
-        Slot<T, VEC> o;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          float2 v = r[u][k][i];
-          if (BWD) {
-            const float2 w = cs[(u * a.token_groups + tg) * half + p0[k] + i];
-            const float2 d = ds[u][k].template pair<HALVES>(i);
-            float2 e = d;
-            if (a.gamma) {
-              acc[k][i].x = fmaf(d.x, v.x * f[u], acc[k][i].x);
-              acc[k][i].y = fmaf(d.y, v.y * f[u], acc[k][i].y);
-              e.x = f[u] * fmaf(-v.x, back[u], d.x * g[k][i].x);
-              e.y = f[u] * fmaf(-v.y, back[u], d.y * g[k][i].y);
+            for (int i = 0; i < VEC; ++i) {
+              r[k][i] = make_float2(0.0f, 0.0f);
+              if (!live[k] || !here) continue;
+              const float2 c = w[i * slots + k * a.lanes], v = xc[u][k].template pair<HALVES>(i);
+              r[k][i] = make_float2(v.x * c.x - v.y * c.y, v.x * c.y + v.y * c.x);
+              if (NORM) {
+                ss = fmaf(r[k][i].x, r[k][i].x, fmaf(r[k][i].y, r[k][i].y, ss));
+                if (BWD) {
+                  const float2 d = dc[u][k].template pair<HALVES>(i);
+                  dot = fmaf(d.x * g[k][i].x, r[k][i].x, fmaf(d.y * g[k][i].y, r[k][i].y, dot));
+                }
+              }
             }
-            v = make_float2(e.x * w.x + e.y * w.y, e.y * w.x - e.x * w.y);
-          } else {
-            v = make_float2(v.x * f[u] * g[k][i].x, v.y * f[u] * g[k][i].y);
-          }
-          o.template put<HALVES>(i, v);
         }
-        o.store(static_cast<T*>(a.y) + b * a.yb + l * a.yl + h * a.yh, e0[k], e1[k]);
+        float f = 1.0f, back = 0.0f;
+        if (NORM) {
+          for (int o = a.lanes / 2; o > 0; o >>= 1) {
+            ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (BWD) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+          }
+          const float n = sqrtf(ss);
+          f = a.sq / fmaxf(n, 1.0e-12f);
+          if (BWD) back = n > 1.0e-12f ? dot / (n * n) : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (!live[k] || !here) continue;
+          Slot<T, VEC> o;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            float2 v;
+            if (BWD) {
+              const float2 d = dc[u][k].template pair<HALVES>(i), c = w[i * slots + k * a.lanes];
+              float2 e = d;
+              if (NORM) {
+                const float2 q = r[k][i];
+                acc[k][i].x = fmaf(d.x, q.x * f, acc[k][i].x);
+                acc[k][i].y = fmaf(d.y, q.y * f, acc[k][i].y);
+                e.x = f * fmaf(-q.x, back, d.x * g[k][i].x);
+                e.y = f * fmaf(-q.y, back, d.y * g[k][i].y);
+              }
+              v = make_float2(e.x * c.x + e.y * c.y, e.y * c.x - e.x * c.y);
+            } else {
+              v = r[k][i];
+              if (NORM) v = make_float2(v.x * f * g[k][i].x, v.y * f * g[k][i].y);
+            }
+            o.template put<HALVES>(i, v);
+          }
+          o.store(y, e0[k], e1[k]);
+        }
       }
     }
+    __syncthreads();  // the table is free for the next chunk
   }
-  if (BWD && a.part) {
+  if (BWD && NORM && a.part) {
     float* q = a.part + (((int64_t)blockIdx.x * a.token_groups + tg) * a.H + h) * a.D;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -314,76 +324,69 @@ static bool misaligned(int dtype, std::initializer_list<const void*> ps) {
   return false;
 }
 
-// How a call's vectors are cut: VEC pairs per lane where every run of VEC elements lies on its own
-// boundary (16 bytes for 4 of fp32 or 8 of a 16-bit type, 8 bytes for 4 of a 16-bit type), single pairs
-// otherwise (odd widths, sliced views).
+// How a call's vectors are cut: four pairs per lane where every run of four elements lies on its own
+// boundary, single pairs otherwise (odd widths, sliced views).
 struct Plan {
-  int vec, k, u;
-  unsigned grid_x, grid_y;
+  bool wide;
+  int k, u;
+  unsigned grid_x, grid_y, threads;
+  size_t smem;
 };
 
 static Plan plan_of(Args& a, int dtype, bool bwd) {
   const int half = a.D / 2;
-  auto fits = [&](int vec) {
-    const uintptr_t bytes = (uintptr_t)vec * dtype_size(dtype) - 1;
-    if (half % vec || (a.halves && a.P % vec)) return false;
-    if ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.y)) & bytes)
-      return false;
-    for (int64_t s : {a.xb, a.xl, a.xh, a.db, a.dl, a.dh, a.yb, a.yl, a.yh})
-      if (s % vec) return false;
-    return true;
-  };
+  const uintptr_t low = 4 * dtype_size(dtype) - 1;
   Plan p;
-  p.vec = dtype != kF32 && fits(8) ? 8 : (fits(4) ? 4 : 1);
-  const int slots = half / p.vec;
+  p.wide = half % 4 == 0 && !(a.halves && a.P % 4) &&
+           !((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.y)) & low);
+  for (int64_t s : {a.xb, a.xl, a.xh, a.db, a.dl, a.dh, a.yb, a.yl, a.yh})
+    if (s % 4) p.wide = false;
+  const int slots = p.wide ? half / 4 : half;
   a.lanes = 1;
   while (a.lanes < slots && a.lanes < 32) a.lanes *= 2;
   p.k = slots > a.lanes ? 4 : 1;
-  p.u = p.k > 1 ? tokens_at_once<false, 4>() : (bwd ? tokens_at_once<true, 1>() : tokens_at_once<false, 1>());
+  p.u = p.k > 1 || bwd ? tokens_at_once<true, 4>() : tokens_at_once<false, 1>();
   const int groups = kThreads / a.lanes;
   a.heads = a.H < groups ? a.H : groups;
   p.grid_y = (unsigned)((a.H + a.heads - 1) / a.heads);
   a.heads = (int)((a.H + p.grid_y - 1) / p.grid_y);  // even shares
-  a.token_groups = groups / a.heads;
   // no more tokens at a time than there are, and a table of at most 32 KB
-  const int64_t need = (a.L + p.u - 1) / p.u;
-  const int room = 32768 / (int)(2 * p.u * half * sizeof(float2));
-  if (a.token_groups > need) a.token_groups = (int)need;
-  if (a.token_groups > room) a.token_groups = room > 0 ? room : 1;
-  const int64_t tokens = (int64_t)a.token_groups * p.u;
-  a.tiles = (a.L + tokens - 1) / tokens;
-  const int64_t all = a.tiles * a.B;
-  const int64_t cap = ((int64_t)sm_count() * (bwd ? 2 : 4) + p.grid_y - 1) / p.grid_y;
-  p.grid_x = (unsigned)(all < cap ? all : cap);
+  const int room = 32768 / (int)(half * sizeof(float2));
+  a.token_groups = groups / a.heads;
+  if (a.token_groups > (a.L + p.u - 1) / p.u) a.token_groups = (int)((a.L + p.u - 1) / p.u);
+  if (a.token_groups > room / p.u) a.token_groups = room / p.u;
+  const int step = a.token_groups * p.u;
+  p.threads = (a.heads * a.token_groups * a.lanes + 31) / 32 * 32;
+  // one chunk per block of a full GPU (some 768 threads per SM), within the table's room
+  const int per_sm = 768 / (int)p.threads > 16 ? 16 : 768 / (int)p.threads;
+  const int64_t blocks = ((int64_t)sm_count() * per_sm + p.grid_y - 1) / p.grid_y;
+  const int64_t share = (a.L * a.B + blocks - 1) / blocks;
+  int64_t steps = (share + step - 1) / step;
+  if (steps > room / step) steps = room / step;
+  a.steps = (int)steps;
+  a.chunks = (a.L + steps * step - 1) / (steps * step);
+  const int64_t all = a.chunks * a.B;
+  p.grid_x = (unsigned)(all < blocks ? all : blocks);
+  p.smem = (size_t)a.steps * step * half * sizeof(float2);
   return p;
 }
 
-template <class T, int VEC, int K, bool BWD>
-static void start(const Args& a, const Plan& p, cudaStream_t stream) {
-  const size_t smem = (size_t)2 * a.token_groups * p.u * (a.D / 2) * sizeof(float2);
+template <class T, bool BWD, bool NORM>
+static void start(const Args& a, const Plan& p, cudaStream_t st) {
   const dim3 grid(p.grid_x, p.grid_y);
-  if (a.halves) axis_rope_k<T, VEC, K, true, BWD><<<grid, kThreads, smem, stream>>>(a);
-  else axis_rope_k<T, VEC, K, false, BWD><<<grid, kThreads, smem, stream>>>(a);
+  if (p.wide && a.halves) axis_rope_k<T, 4, 1, true, BWD, NORM><<<grid, p.threads, p.smem, st>>>(a);
+  else if (p.wide) axis_rope_k<T, 4, 1, false, BWD, NORM><<<grid, p.threads, p.smem, st>>>(a);
+  else if (p.k == 1) axis_rope_k<T, 1, 1, true, BWD, NORM><<<grid, p.threads, p.smem, st>>>(a);
+  else axis_rope_k<T, 1, 4, true, BWD, NORM><<<grid, p.threads, p.smem, st>>>(a);
 }
 
 template <bool BWD>
-static void launch(const Args& a, const Plan& p, int dtype, cudaStream_t stream) {
-  LaunchScope scope(kKElementwise, stream);
-  if (dtype == kF32) {
-    if (p.vec == 4) start<float, 4, 1, BWD>(a, p, stream);
-    else if (p.k == 1) start<float, 1, 1, BWD>(a, p, stream);
-    else start<float, 1, 4, BWD>(a, p, stream);
-  } else if (dtype == kBF16) {
-    if (p.vec == 8) start<__nv_bfloat16, 8, 1, BWD>(a, p, stream);
-    else if (p.vec == 4) start<__nv_bfloat16, 4, 1, BWD>(a, p, stream);
-    else if (p.k == 1) start<__nv_bfloat16, 1, 1, BWD>(a, p, stream);
-    else start<__nv_bfloat16, 1, 4, BWD>(a, p, stream);
-  } else {
-    if (p.vec == 8) start<__half, 8, 1, BWD>(a, p, stream);
-    else if (p.vec == 4) start<__half, 4, 1, BWD>(a, p, stream);
-    else if (p.k == 1) start<__half, 1, 1, BWD>(a, p, stream);
-    else start<__half, 1, 4, BWD>(a, p, stream);
-  }
+static void launch(const Args& a, const Plan& p, int dtype, cudaStream_t st) {
+  LaunchScope scope(kKElementwise, st);
+  if (dtype == kF32) a.gamma ? start<float, BWD, true>(a, p, st) : start<float, BWD, false>(a, p, st);
+  else if (dtype == kBF16)
+    a.gamma ? start<__nv_bfloat16, BWD, true>(a, p, st) : start<__nv_bfloat16, BWD, false>(a, p, st);
+  else a.gamma ? start<__half, BWD, true>(a, p, st) : start<__half, BWD, false>(a, p, st);
 }
 
 }  // namespace rope
