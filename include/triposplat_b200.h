@@ -478,7 +478,8 @@ int triposplat_b200_axis_rope_backward(const void* dy, const void* x, const void
 /* Exact attention O = softmax(Q K^T / 8 + key_bias) V for training, head_dim 64, fp32 tensors of
  * any strides with a contiguous last dimension.  strides: batch, head, row of q, k, v; key_bias
  * [bias_batches, bias_heads, Lk] contiguous (1 or B, 1 or H) or null; out_blhd [B, Lq, H, 64];
- * stats [B, H, Lq, 2] for the backward pass.  A key whose bias is -inf does not exist (its K and
+ * stats [B, H, Lq + 1, 2] for the backward pass (a row's reference maximum in log2 units and
+ * its sum; last, the largest bias and whether the scores count beside it).  A key whose bias is -inf does not exist (its K and
  * V may hold anything); a row without keys is zeros.  The scores' accuracy is that of
  * triposplat_sdpa_f32_avx512_exact_q8t512. */
 int triposplat_b200_attention_forward(const float* q, const float* k, const float* v,

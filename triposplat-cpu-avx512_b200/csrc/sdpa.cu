@@ -116,6 +116,7 @@ struct Params {
   // nullable: per row (final reference maximum, row sum) for the backward pass; with it a row
   // without a key is zeros instead of 0 / 0
   float2* stats;
+  int64_t stats_ld;  // rows of stats per (b, h)
 };
 
 // 2^s for |s| <= 126 built in the exponent field: x * pow2i(s) is the correctly rounded
@@ -729,7 +730,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         float f = vref / l;
         if (p.stats) {
           if (l == 0.0f) f = 0.0f;
-          p.stats[(int64_t)bh * p.Lq + qrow] = make_float2(m, l * 0x1p-7f);  // the lift of P_LIFT taken out
+          p.stats[bh * p.stats_ld + qrow] = make_float2(m, l * 0x1p-7f);  // the lift of P_LIFT taken out
         }
         // dimensions 0..31 as team 0's own (o0 f0 + o1 f1), 32..63 as team 1's own
 #pragma unroll
@@ -1323,7 +1324,7 @@ static OutSplit out_split_of(void* out_split, int64_t B, int Lq, int H) {
 static int sdpa_attend(const SplitPlanesSdpa& sp, const float* bias, int64_t bias_bh_stride,
                        float* out, int64_t BH, int H, int Lq, int Lk, int out_blhd,
                        cudaStream_t stream, const OutSplit& osplit = OutSplit(),
-                       float2* stats = nullptr) {
+                       float2* stats = nullptr, int64_t stats_ld = 0) {
   using namespace sdpa;
   CUtensorMap m_qhi, m_qlo, m_khi, m_klo, m_vhi, m_vlo;
   const uint32_t box_rows[3] = {64, 128, 1};
@@ -1371,7 +1372,7 @@ static int sdpa_attend(const SplitPlanesSdpa& sp, const float* bias, int64_t bia
   }
   const int Qt = (Lq + BQ - 1) / BQ;
   Params prm{sp.qinv, sp.kinv, sp.vinv, bias, (long long)bias_bh_stride, out, H, Lq, Lk, sp.T, out_blhd,
-             device_status(), Qt, (int)BH, osplit.hi, osplit.lo, osplit.rs, stats};
+             device_status(), Qt, (int)BH, osplit.hi, osplit.lo, osplit.rs, stats, stats_ld};
   // persistent: one CTA per SM walking the (head, query tile) items
   static std::atomic<int> sm_count[64];
   int dev = 0;
@@ -1393,8 +1394,8 @@ static int sdpa_attend(const SplitPlanesSdpa& sp, const float* bias, int64_t bia
 }
 
 int sdpa_attend_stats(const SplitPlanesSdpa& sp, const float* bias, int64_t bias_bh_stride, float* out_blhd,
-                      float2* stats, int64_t BH, int H, int Lq, int Lk, cudaStream_t stream) {
-  return sdpa_attend(sp, bias, bias_bh_stride, out_blhd, BH, H, Lq, Lk, 1, stream, OutSplit(), stats);
+                      float2* stats, int64_t stats_ld, int64_t BH, int H, int Lq, int Lk, cudaStream_t stream) {
+  return sdpa_attend(sp, bias, bias_bh_stride, out_blhd, BH, H, Lq, Lk, 1, stream, OutSplit(), stats, stats_ld);
 }
 
 // k/v element (bh, j, d) at base + bh*bh_stride + j*j_stride + d*d_stride

@@ -20,26 +20,32 @@
 // Two passes, each the owner of its outputs, instead of one with atomics on dQ: the results are
 // the same bits on every run.  The keys' pass holds 128 keys and walks the queries
 // (S^T, dP^T, dV, dK: four products), the queries' pass holds 128 queries and walks the keys (S, dP,
-// dQ: three).  Both are one kernel: F1, F2 are the held operands (K, V or Q, g), G1, G2 the walked
-// ones (Q, g or K, V):
+// dQ: three).  Both are one kernel and one launch: F1, F2 are the held operands (K, V or Q, g), G1, G2
+// the walked ones (Q, g or K, V):
 //   X = F1 G1^T ;  Y = F2 G2^T ;  e = 2^(c X + column + row) ;  ds = e (a Y - delta) ;
 //   acc1 += ds G1   (dK or dQ) ;  acc2 += e G2   (dV, keys' pass only).
 //
 // Split precision as in sdpa.cu: every operand is an fp16 pair hi + lo after an exact power-of-two
-// scale (one per 64-row tile; for e and ds a power of two from the bound 2^8 on e, and for ds from
-// the tiles' largest row norms, |g . v - delta| <= |g| |v| + |delta|), each product is three
-// tensor-core passes (hi.hi, hi.lo, lo.hi), and a walked tile's products go into a fresh
-// accumulator in tensor memory that is added to fp32 registers: the tensor core's own fp32
-// accumulation truncates, and one accumulator over thousands of rows would drift.
+// scale (one per 128-row tile; 2^7 for e <= 2^8, and for ds a power of two from the tiles' largest
+// norms, |g . v - delta| <= |g| |v| + |delta|), each product is three tensor-core passes (hi.hi, hi.lo,
+// lo.hi), and the products of two walked tiles (24 steps) go into a fresh accumulator in tensor
+// memory that is added to fp32 registers: the tensor core's own fp32 accumulation truncates, and one
+// accumulator over thousands of rows would drift.
 //
-// CTA: 384 threads, one per SM, persistent over (head, held tile).  Warp 0 loads walked tiles
-// (64 rows: 32 KB of planes and the tile's vectors, kStages deep), warp 1 issues all MMAs, two
-// warpgroups compute.  The held operands live in tensor memory as the A side of X and Y (128
-// columns), so that shared memory feeds the tensor core only the walked side.  X and Y have
-// two buffers of 64 columns each: the tensor core forms X, Y of the next tile while the
+// CTA: 384 threads, one per SM, persistent over work items (pass, head, held tile, share of the walk).
+// Warp 0 loads walked tiles (64 rows: 32 KB of planes and the tile's vectors, kStages deep), warp 1
+// issues all MMAs, two warpgroups compute: thread = held row = tensor-memory lane, warpgroup = 32
+// walked rows.  The held operands live in tensor memory as the A side of X and Y (128 columns), so
+// that shared memory feeds the tensor core only the walked side: measured, an MMA of 128 x 64 x 16
+// takes its 32 cycles with A in tensor memory and 48 with both operands in shared memory.  X and Y
+// have two buffers of 64 columns each: the tensor core forms X, Y of the next tile while the
 // warpgroups turn the current ones, in place, into the fp16 pairs of e and ds, the A side of the
 // accumulating products.  G1, G2 are read from the same shared tile both ways: K-major for X
 // and Y (the 64 head dimensions contracted), MN-major for the accumulators (rows contracted).
+//
+// Few held tiles (a handful of queries or keys): a walk longer than an SM's share of the whole
+// work is cut, each share writes partial sums, and a last kernel adds them in their order.
+//
 #include <stdint.h>
 
 #include <atomic>
@@ -54,7 +60,7 @@ namespace sdpab {
 
 constexpr int D = 64;
 constexpr int HELD = 128;               // rows of a held tile
-constexpr int WALK = 64;                // rows of a walked tile, and of a scale tile
+constexpr int WALK = 64;                // rows of a walked tile (two share their scales and accumulators)
 constexpr int kThreads = 384;
 constexpr int kStages = 4;
 constexpr int PLANE = WALK * D * 2;     // 8 KB: one 64 x 64 fp16 tile
@@ -137,19 +143,44 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
       : "memory");
 }
 
-// Shared-memory descriptor of a 64-column fp16 tile (128-byte rows, 128-byte swizzle) read
-// MN-major: the 64 columns are the operand's N, rows its K; groups of 8 rows are 1024 bytes apart.
-__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_addr) {
-  uint64_t d = 0;
-  d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);
-  d |= (uint64_t)(1024u >> 4) << 16;  // next 64 columns (N = 64: not used)
-  d |= (uint64_t)(1024u >> 4) << 32;  // next 8 rows
-  d |= (uint64_t)1u << 46;
-  d |= (uint64_t)2u << 61;
-  return d;
+// Shared-memory descriptors of a 64-column fp16 tile (128-byte rows, 128-byte swizzle) as two words:
+// the low one is the start address (in 16-byte units) under a constant, the high one is constant.
+// K-major (columns contracted): 8-row groups 1024 bytes apart, 16 columns on is 32 bytes.
+// MN-major (rows contracted, the columns are the operand's N): the same groups, 16 rows on is 2048
+// bytes; the distance to the next 64 columns is not used at N = 64.
+constexpr uint32_t kDescHi = (1024u >> 4) | 1u << 14 | 2u << 29;
+constexpr uint32_t kDescLo = (1024u >> 4) << 16;
+__device__ __forceinline__ uint32_t desc_lo(uint32_t smem_addr) { return kDescLo | ((smem_addr >> 4) & 0x3FFFu); }
+
+// D(tmem) (+)= A(tmem) B(smem): one of a product's steps of 16 contracted elements.  The issuing
+// thread has 32 cycles of tensor-core time per call, so its operands are one addition each.
+template <bool ADD>
+__device__ __forceinline__ void mma_step(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "n"(kDescHi), "r"(idesc), "n"(ADD ? 1 : 0)
+      : "memory");
 }
 
-// One scale tile (64 rows) of the two tensors of a side.
+// D = A B (FRESH) or D += A B over 64 contracted elements in three passes.  A: hi and lo pairs A_STEP columns per
+// 16 elements apart, lo A_LO columns behind hi; B: tiles hi and lo (PLANE apart), B_STEP 16-byte units
+// per 16 elements.
+template <int A_STEP, int A_LO, int B_STEP, bool FRESH>
+__device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc) {
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk) {
+    const uint32_t ah = a + kk * A_STEP, bh = b_lo + kk * B_STEP;
+    if (FRESH && kk == 0) mma_step<false>(d, ah, bh, idesc);
+    else mma_step<true>(d, ah, bh, idesc);
+    mma_step<true>(d, ah, bh + (PLANE >> 4), idesc);
+    mma_step<true>(d, ah + A_LO, bh, idesc);
+  }
+}
+
+// One scale tile (128 rows) of the two tensors of a side.
 struct TileScale {
   float inv1, inv2;   // inverse pre-scales of (Q, g) or (K, V)
   float norm, delta;  // queries: largest |g_i|, |delta_i|; keys: largest |v_j|, 0
@@ -158,346 +189,418 @@ struct TileScale {
 // The two sides' planes, all [BH, rows padded to 128, 64] fp16, rows past the end zero.
 struct Side {
   __half *hi1, *lo1, *hi2, *lo2;
-  float *col;         // queries: -m_i (-inf past the end and for rows without a key); keys: bias in log2 units
+  float *col;         // queries: 7 - m_i (-inf past the end and for rows without a key); keys: bias in log2 units
   float *delta;       // queries: -delta_i; keys: unused
-  TileScale* scale;   // [BH, padded / 64]
+  TileScale* scale;   // [BH, padded / 128]
   int L, Lt;          // rows, padded rows
 };
 
-struct Params {
+// One pass: what it holds and walks, how its walk is cut, where its gradients go.
+struct Pass {
   Side held, walk;
-  const float* head;  // [BH]: 0 where the bias leaves the scores no weight, 1 otherwise
-  float *out1, *out2; // dK (or dQ), dV
-  float* db;          // nullable: [2, BH, Lt of the keys] sums of ds over each warpgroup's queries
+  float *out1, *out2;  // dK (or dQ), dV; with cuts, partial sums [cuts, BH, held.Lt, 64] instead
   int64_t s1b, s1h, s1l, s2b, s2h, s2l;  // element strides of out1, out2
-  int H, BH, T, Ft, vec_out;  // T walked tiles, Ft held tiles per head
+  int T, Ft;           // walked tiles, held tiles per head
+  int cuts, span;      // shares of the walk, walked tiles per share (even unless there is one share)
+  int ragged;          // the last walked tile ends before its 64 rows
+  int vec_out;         // 16-byte stores
+};
+
+struct Params {
+  Pass keys, queries;
+  const float2* head;  // [BH] head_stride apart: .y = 0 where the bias leaves the scores no weight, 1 otherwise
+  int64_t head_stride;
+  float* db;           // nullable: [cuts, 2, BH, Lt of the keys] sums of ds over each warpgroup's queries
+  int H, BH;
+  int key_items, items;
   int* status;
 };
 
-template <bool KEYS>
-__global__ void __launch_bounds__(kThreads, 1)
-    sdpa_bwd_tc(const __grid_constant__ CUtensorMap tm1h, const __grid_constant__ CUtensorMap tm1l,
-                const __grid_constant__ CUtensorMap tm2h, const __grid_constant__ CUtensorMap tm2l,
-                const Params p) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* tiles = smem;                                     // [kStages] G1 hi, lo, G2 hi, lo
-  uint8_t* vecs = tiles + kStages * STAGE;                   // [kStages] columns, deltas, scales
-  uint64_t* bars = reinterpret_cast<uint64_t*>(vecs + kStages * VEC_STAGE);
-  uint64_t* full = bars;               // [kStages] walked tile loaded
-  uint64_t* empty = full + kStages;    // [kStages] both products of the tile retired
-  uint64_t* xy_full = empty + kStages; // [2] X, Y formed
-  uint64_t* ed_full = xy_full + 2;     // [2] e, ds written over them (8 warps)
-  uint64_t* acc_full = ed_full + 2;    // [2] accumulators of a tile formed
-  uint64_t* acc_free = acc_full + 2;   // [2] ... and folded into registers (8 warps)
-  uint64_t* held_full = acc_free + 2;  // the item's held operands are in tensor memory (8 warps)
-  uint64_t* all_done = held_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+struct Maps {
+  CUtensorMap q1h, q1l, q2h, q2l, k1h, k1l, k2h, k2l;
+};
 
-  const uint32_t warp = warp_id(), lane = lane_id();
-  const int T = p.T;
-  const int items = p.Ft * p.BH;
-  const int my_items = (int)blockIdx.x < items ? (items - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
-  auto item_of = [&](int i, int& bh, int& f0) {
-    const int j = blockIdx.x + i * gridDim.x;
-    bh = j / p.Ft;
-    f0 = (j - bh * p.Ft) * HELD;
-  };
+// Work item j: keys' items first; shares of a walk next to each other, then held tiles, then heads.
+struct Item {
+  bool keys;
+  int bh, f0, t0, n, cut;  // head, first held row, walked tiles [t0, t0 + n)
+};
+__device__ __forceinline__ Item item_of(const Params& p, int j) {
+  Item it;
+  it.keys = j < p.key_items;
+  const Pass& s = it.keys ? p.keys : p.queries;
+  if (!it.keys) j -= p.key_items;
+  it.cut = j % s.cuts;
+  j /= s.cuts;
+  it.bh = j / s.Ft;
+  it.f0 = (j - it.bh * s.Ft) * HELD;
+  it.t0 = it.cut * s.span;
+  it.n = min(s.span, s.T - it.t0);
+  return it;
+}
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&xy_full[i], 1);
-      mbar_init(&ed_full[i], 8);
-      mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_free[i], 8);
+// A wait of a whole warp: one lane polls.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status, int code, volatile int* abort_flag) {
+  int ok = 1;
+  if (lane_id() == 0) ok = mbar_wait(bar, parity, status, code, abort_flag);
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
+// Of one walked tile, the 32 columns of this thread's row that its warpgroup has: X and Y in, e
+// (KEYS) and ds out as fp16 pairs over them.  The exponent's offset is a column's (COL) or the row's
+// (ROW) or both; the column's and the row's delta come in the units of a * Y.
+template <bool KEYS, bool COL, bool ROW>
+__device__ __forceinline__ void tile_math(uint32_t x0, const uint32_t (&xv)[32], const uint32_t (&yv)[32],
+                                          const float4* col, const float4* del, float c, float a, float up, float row,
+                                          float row_delta, uint64_t& dsum) {
+  // up: ds is formed times 2^kk, e is lifted by 2^7; the queries' pass has both in a and row_delta
+  const uint64_t c2 = f2pack(c, c), a2 = f2pack(a, a), up2 = f2pack(up, up);
+  const uint64_t row2 = f2pack(row, row), rd2 = f2pack(row_delta, row_delta);
+#pragma unroll
+  for (int ch = 0; ch < 2; ++ch) {  // 16 walked rows: 8 columns of hi pairs, 8 of lo pairs
+    uint32_t pe[16], pd[16];
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+      const int q = ch * 16 + j;
+      const float4 cv = COL ? col[q / 4] : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 dv = KEYS ? del[q / 4] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = q + 2 * h;
+        uint64_t off = row2;
+        if (COL) {
+          off = h == 0 ? f2pack(cv.x, cv.y) : f2pack(cv.z, cv.w);
+          if (ROW) off = f2add(off, row2);
+        }
+        float e0, e1;
+        f2unpack(f2fma(f2pack(__uint_as_float(xv[k]), __uint_as_float(xv[k + 1])), c2, off), e0, e1);
+        const uint64_t e = f2pack(ex2(e0), ex2(e1));
+        const uint64_t nd = KEYS ? (h == 0 ? f2pack(dv.x, dv.y) : f2pack(dv.z, dv.w)) : rd2;
+        const uint64_t y = f2fma(f2pack(__uint_as_float(yv[k]), __uint_as_float(yv[k + 1])), a2, nd);
+        const uint64_t ds = f2mul(KEYS ? f2mul(e, up2) : e, y);
+        if (KEYS) split2(e, pe[j / 2 + h], pe[8 + j / 2 + h]);
+        if (KEYS && ROW) dsum = f2add(dsum, ds);
+        split2(ds, pd[j / 2 + h], pd[8 + j / 2 + h]);
+      }
     }
-    mbar_init(held_full, 8);
-    mbar_init(all_done, 1);
-    *abort_flag = 0;
+    if (KEYS) tmem_st16(x0 + ch * 16, pe);
+    tmem_st16(x0 + 64 + ch * 16, pd);
+  }
+}
+
+// Barriers and shared memory of a CTA, and the counts that its roles keep in step: walked tiles (G)
+// and pairs of them (P) so far, over all items.
+struct Shared {
+  uint8_t *tiles, *vecs;  // [kStages] G1 hi, lo, G2 hi, lo; [kStages] columns, deltas, scales
+  uint64_t* full;         // [kStages] walked tile loaded
+  uint64_t* empty;        // [kStages] both products of the tile retired
+  uint64_t* xy_full;      // [2] X, Y formed
+  uint64_t* ed_full;      // [2] e, ds written over them (8 warps)
+  uint64_t* acc_full;     // [2] accumulators of a pair formed
+  uint64_t* acc_free;     // [2] ... and folded into registers (8 warps)
+  uint64_t* held_full;    // the item's held operands are in tensor memory (8 warps)
+  uint64_t* all_done;
+  uint32_t* tmem_slot;
+  volatile int* abort_flag;
+};
+
+__device__ __forceinline__ Shared carve(uint8_t* raw) {
+  Shared s;
+  s.tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  s.vecs = s.tiles + kStages * STAGE;
+  s.full = reinterpret_cast<uint64_t*>(s.vecs + kStages * VEC_STAGE);
+  s.empty = s.full + kStages;
+  s.xy_full = s.empty + kStages;
+  s.ed_full = s.xy_full + 2;
+  s.acc_full = s.ed_full + 2;
+  s.acc_free = s.acc_full + 2;
+  s.held_full = s.acc_free + 2;
+  s.all_done = s.held_full + 1;
+  s.tmem_slot = reinterpret_cast<uint32_t*>(s.all_done + 1);
+  s.abort_flag = reinterpret_cast<volatile int*>(s.tmem_slot + 1);
+  return s;
+}
+
+// Warp 0, one thread: an item's walked tiles.
+template <bool KEYS>
+__device__ __forceinline__ bool load_item(const Params& p, const Pass& ps, const Item& it, const CUtensorMap* m1h,
+                                          const CUtensorMap* m1l, const CUtensorMap* m2h, const CUtensorMap* m2l,
+                                          const Shared& sh, int& G) {
+  for (int t = it.t0; t < it.t0 + it.n; ++t, ++G) {
+    const int st = G % kStages;
+    if (G >= kStages &&
+        !mbar_wait(&sh.empty[st], ((G / kStages) & 1) ^ 1, p.status, kDevTimeoutProducer, sh.abort_flag))
+      return false;
+    uint8_t* d = sh.tiles + st * STAGE;
+    uint8_t* v = sh.vecs + st * VEC_STAGE;
+    const int64_t row = (int64_t)it.bh * ps.walk.Lt + t * WALK;
+    mbar_arrive_expect_tx(&sh.full[st], STAGE + WALK * 4 * (KEYS ? 2 : 1) + 16);
+    tma_load_3d(d, m1h, &sh.full[st], 0, t * WALK, it.bh);
+    tma_load_3d(d + PLANE, m1l, &sh.full[st], 0, t * WALK, it.bh);
+    tma_load_3d(d + 2 * PLANE, m2h, &sh.full[st], 0, t * WALK, it.bh);
+    tma_load_3d(d + 3 * PLANE, m2l, &sh.full[st], 0, t * WALK, it.bh);
+    bulk_load(v, ps.walk.col + row, WALK * 4, &sh.full[st]);
+    if (KEYS) bulk_load(v + WALK * 4, ps.walk.delta + row, WALK * 4, &sh.full[st]);
+    bulk_load(v + 2 * WALK * 4, ps.walk.scale + row / HELD, 16, &sh.full[st]);
+  }
+  return true;
+}
+
+// Warp 1, one thread: an item's MMAs.  X, Y of tile t + 1 are issued ahead of tile t's accumulating
+// products, so the tensor core has them to do while e, ds of tile t are formed.  Their buffer's last
+// readers, the products of tile t - 1, come before them in the same order.
+template <bool KEYS>
+__device__ __forceinline__ bool mma_item(const Params& p, int n, const Shared& sh, uint32_t tmem, int& G, int& P) {
+  constexpr uint32_t idesc_xy = idesc_f16_f32(HELD, WALK);
+  constexpr uint32_t idesc_acc = idesc_f16_f32(HELD, D) | (1u << 16);  // B MN-major
+  auto form_xy = [&](int g_) -> bool {
+    const int st = g_ % kStages;
+    if (!mbar_wait(&sh.full[st], (g_ / kStages) & 1, p.status, kDevTimeoutMma, sh.abort_flag)) return false;
+    tc_fence_after();
+    const uint32_t g = desc_lo(smem_u32(sh.tiles + st * STAGE));
+    const uint32_t x = tmem + XY_COL + (g_ & 1) * 128;
+    product<8, 32, 32 / 16, true>(x, tmem + F_COL, g, idesc_xy);                                // F1 G1^T
+    product<8, 32, 32 / 16, true>(x + 64, tmem + F_COL + 64, g + (2 * PLANE >> 4), idesc_xy);  // F2 G2^T
+    mma_commit(&sh.xy_full[g_ & 1]);
+    return true;
+  };
+  if (!form_xy(G)) return false;
+  for (int t = 0; t < n; ++t, ++G) {
+    const int st = G % kStages;
+    if (t + 1 < n && !form_xy(G + 1)) return false;
+    // accumulators of pair P: the keys' pass has one buffer, the queries' two
+    const int prev = KEYS ? P - 1 : P - 2;
+    if (!mbar_wait(&sh.ed_full[G & 1], (G >> 1) & 1, p.status, kDevTimeoutMma, sh.abort_flag)) return false;
+    if (!(t & 1) && prev >= 0 &&
+        !mbar_wait(&sh.acc_free[prev & 1], (prev >> 1) & 1, p.status, kDevTimeoutMma, sh.abort_flag))
+      return false;
+    tc_fence_after();
+    const uint32_t g = desc_lo(smem_u32(sh.tiles + st * STAGE));
+    const uint32_t x = tmem + XY_COL + (G & 1) * 128;
+    const uint32_t acc1 = tmem + ACC_COL + (KEYS ? 0 : (P & 1) * 64);
+    if (t & 1) {
+      if (KEYS) product<16, 8, 2048 / 16, false>(acc1 + 64, x, g + (2 * PLANE >> 4), idesc_acc);  // e G2
+      product<16, 8, 2048 / 16, false>(acc1, x + 64, g, idesc_acc);                              // ds G1
+    } else {
+      if (KEYS) product<16, 8, 2048 / 16, true>(acc1 + 64, x, g + (2 * PLANE >> 4), idesc_acc);
+      product<16, 8, 2048 / 16, true>(acc1, x + 64, g, idesc_acc);
+    }
+    mma_commit(&sh.empty[st]);
+    if ((t & 1) || t + 1 == n) {
+      mma_commit(&sh.acc_full[P & 1]);
+      ++P;
+    }
+  }
+  return true;
+}
+
+// The two compute warpgroups: an item's e, ds, folds and gradients.
+template <bool KEYS, bool BIAS>
+__device__ __forceinline__ bool compute_item(const Params& p, const Pass& ps, const Item& it, const Shared& sh,
+                                             uint32_t tmem, int& G, int& P) {
+  const uint32_t warp = warp_id(), lane = lane_id(), sub = warp & 3;
+  const int w = (warp - 4) >> 2;  // warpgroup w has walked rows 32w..32w+31
+  const int r = sub * 32 + lane;  // held row == tensor-memory lane
+  const uint32_t trow = tmem + ((sub * 32) << 16);
+  constexpr int NACC = KEYS ? 64 : 32;  // keys: w = 0 keeps dV, w = 1 dK; queries: half of dQ each
+  const int64_t frow = (int64_t)it.bh * ps.held.Lt + it.f0 + r;
+  {
+    // held operands into tensor memory: this warpgroup's pair of planes
+    const __half* hi = w == 0 ? ps.held.hi1 : ps.held.hi2;
+    const __half* lo = w == 0 ? ps.held.lo1 : ps.held.lo2;
+#pragma unroll
+    for (int pl = 0; pl < 2; ++pl) {
+      const uint4* src = reinterpret_cast<const uint4*>((pl == 0 ? hi : lo) + frow * D);
+      uint32_t v[32];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint4 u = __ldg(src + k);
+        v[4 * k] = u.x; v[4 * k + 1] = u.y; v[4 * k + 2] = u.z; v[4 * k + 3] = u.w;
+      }
+      tmem_st32(trow + F_COL + w * 64 + pl * 32, v);
+    }
+    tmem_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(sh.held_full);
+  }
+  const TileScale fs = ps.held.scale[frow / HELD];
+  const float c0 = 0.125f * LOG2E * p.head[it.bh * p.head_stride].y * fs.inv1;
+  // row constants: queries' pass 7 - m_i and -delta_i, keys' pass b_j
+  const float row = ps.held.col[frow], row_delta = KEYS ? 0.0f : ps.held.delta[frow];
+  uint64_t acc[NACC / 2];
+#pragma unroll
+  for (int k = 0; k < NACC / 2; ++k) acc[k] = 0ull;
+  float db = 0.0f, fold_scale = 0.0f;
+  // adds the accumulators of the next pair to the registers
+  auto fold = [&]() -> bool {
+    if (!warp_wait(&sh.acc_full[P & 1], (P >> 1) & 1, p.status, kDevTimeoutConsumer, sh.abort_flag)) return false;
+    tc_fence_after();
+    const uint32_t src = trow + ACC_COL + (KEYS ? (w == 0 ? 64 : 0) : (P & 1) * 64 + w * 32);
+    const uint64_t s2 = f2pack(fold_scale, fold_scale);
+    uint32_t v[NACC / 32][32];
+#pragma unroll
+    for (int c = 0; c < NACC / 32; ++c) tmem_ld32(src + c * 32, v[c]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int c = 0; c < NACC / 32; ++c) reg_fence(v[c]);
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.acc_free[P & 1]);
+    ++P;
+#pragma unroll
+    for (int c = 0; c < NACC / 32; ++c)
+#pragma unroll
+      for (int k = 0; k < 32; k += 2)
+        acc[c * 16 + k / 2] = f2fma(f2pack(__uint_as_float(v[c][k]), __uint_as_float(v[c][k + 1])), s2, acc[c * 16 + k / 2]);
+    return true;
+  };
+  for (int t = 0; t < it.n; ++t, ++G) {
+    const int st = G % kStages;
+    // the tile's vectors (their copy's completion seen by this warp) and its X, Y
+    if (!warp_wait(&sh.full[st], (G / kStages) & 1, p.status, kDevTimeoutConsumer, sh.abort_flag) ||
+        !warp_wait(&sh.xy_full[G & 1], (G >> 1) & 1, p.status, kDevTimeoutConsumer, sh.abort_flag))
+      return false;
+    tc_fence_after();
+    const uint32_t x0 = trow + XY_COL + (G & 1) * 128 + w * 32;
+    uint32_t xv[32], yv[32];
+    tmem_ld32(x0, xv);
+    tmem_ld32(x0 + 64, yv);
+    const uint8_t* v = sh.vecs + st * VEC_STAGE;
+    const float4* col = reinterpret_cast<const float4*>(v) + w * 8;
+    const float4* del = reinterpret_cast<const float4*>(v + WALK * 4) + w * 8;
+    const TileScale ws = *reinterpret_cast<const TileScale*>(v + 2 * WALK * 4);
+    const float c = c0 * ws.inv1, a = fs.inv2 * ws.inv2;
+    // ds is formed as ds * 2^kk with |ds| 2^kk <= 2^15: e <= 2^8, |Y - delta| <= bound < 2^(ilogb + 1)
+    const float bound = fs.norm * ws.norm + (KEYS ? ws.delta : fs.delta);
+    int kk = 6 - ((__float_as_int(bound) >> 23) - 127);
+    kk = kk > 100 ? 100 : (kk < -100 ? -100 : kk);
+    const float up = pow2i(kk) * 0x1p-7f, down = pow2i(-kk);
+    uint64_t dsum = 0ull;
+    tmem_wait_ld();
+    reg_fence(xv);
+    reg_fence(yv);
+    if (KEYS)
+      tile_math<true, true, BIAS>(x0, xv, yv, col, del, c, a, up, row, 0.0f, dsum);
+    else if (BIAS || (ps.ragged && it.t0 + t + 1 == ps.T))
+      tile_math<false, true, true>(x0, xv, yv, col, del, c, a * up, 1.0f, row, row_delta * up, dsum);
+    else
+      tile_math<false, false, true>(x0, xv, yv, col, del, c, a * up, 1.0f, row, row_delta * up, dsum);
+    tmem_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.ed_full[G & 1]);
+    if (t >= 2 && !(t & 1) && !fold()) return false;
+    // scales of the pair that this tile is in (both of its tiles have the same)
+    fold_scale = KEYS && w == 0 ? ws.inv2 * 0x1p-7f : ws.inv1 * down;
+    if (KEYS && BIAS) {
+      float d0, d1;
+      f2unpack(dsum, d0, d1);
+      db = fmaf(d0 + d1, down, db);
+    }
+  }
+  if (!fold()) return false;
+  // ---- the held rows' gradients ----
+  const bool first = !KEYS || w == 1;  // out1 (dK, dQ) or out2 (dV)
+  float* dst = first ? ps.out1 : ps.out2;
+  bool vec = true;
+  if (ps.cuts > 1) {
+    dst += (((int64_t)it.cut * p.BH + it.bh) * ps.held.Lt + it.f0 + r) * D;
+  } else {
+    const int b = it.bh / p.H, h = it.bh - b * p.H;
+    dst += first ? b * ps.s1b + h * ps.s1h + (it.f0 + r) * ps.s1l : b * ps.s2b + h * ps.s2h + (it.f0 + r) * ps.s2l;
+    vec = ps.vec_out;
+  }
+  if (!KEYS) dst += w * 32;
+  if (it.f0 + r < ps.held.L) {
+    const float s = first ? 0.125f : 1.0f;
+    if (vec) {
+#pragma unroll
+      for (int k = 0; k < NACC; k += 4) {
+        float4 o;
+        f2unpack(acc[k / 2], o.x, o.y);
+        f2unpack(acc[k / 2 + 1], o.z, o.w);
+        *reinterpret_cast<float4*>(dst + k) = make_float4(o.x * s, o.y * s, o.z * s, o.w * s);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < NACC; k += 2) {
+        float o0, o1;
+        f2unpack(acc[k / 2], o0, o1);
+        dst[k] = o0 * s;
+        dst[k + 1] = o1 * s;
+      }
+    }
+  }
+  if (KEYS && BIAS && p.db) p.db[(int64_t)(it.cut * 2 + w) * p.BH * ps.held.Lt + frow] = db;
+  return true;
+}
+
+// BIAS: the call has a key bias (without one, the keys' pass has no row offset and the queries' pass
+// needs column offsets only for the tile past the last key).
+template <bool BIAS>
+__global__ void __launch_bounds__(kThreads, 1) sdpa_bwd_tc(const __grid_constant__ Maps m, const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  const Shared sh = carve(smem_raw);
+  const uint32_t warp = warp_id();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.xy_full[i], 1);
+      mbar_init(&sh.ed_full[i], 8);
+      mbar_init(&sh.acc_full[i], 1);
+      mbar_init(&sh.acc_free[i], 8);
+    }
+    mbar_init(sh.held_full, 8);
+    mbar_init(sh.all_done, 1);
+    *sh.abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&tm1h); tma_prefetch_desc(&tm1l);
-    tma_prefetch_desc(&tm2h); tma_prefetch_desc(&tm2l);
-  }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_alloc(sh.tmem_slot, TMEM_COLS);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-
+  const uint32_t tmem = *sh.tmem_slot;
+  int G = 0, P = 0;
+  bool ok = true;
   if (warp < 4) {
     setmaxnreg_dec<REGS_CONTROL>();
     if (warp == 0) {
-      // ---------------- walked tiles ----------------
       if (elect_one()) {
-        int issued[kStages];
-        for (int s = 0; s < kStages; ++s) issued[s] = -1;
-        bool ok = true;
-        for (int i = 0; i < my_items && ok; ++i) {
-          int bh, f0;
-          item_of(i, bh, f0);
-          for (int t = 0; t < T; ++t) {
-            const int G = i * T + t, st = G % kStages;
-            if (G >= kStages &&
-                !mbar_wait(&empty[st], ((G / kStages) & 1) ^ 1, p.status, kDevTimeoutProducer, abort_flag)) {
-              ok = false;
-              break;
-            }
-            uint8_t* d = tiles + st * STAGE;
-            uint8_t* v = vecs + st * VEC_STAGE;
-            const int64_t row = (int64_t)bh * p.walk.Lt + t * WALK;
-            mbar_arrive_expect_tx(&full[st], STAGE + WALK * 4 * (KEYS ? 2 : 1) + 16);
-            tma_load_3d(d, &tm1h, &full[st], 0, t * WALK, bh);
-            tma_load_3d(d + PLANE, &tm1l, &full[st], 0, t * WALK, bh);
-            tma_load_3d(d + 2 * PLANE, &tm2h, &full[st], 0, t * WALK, bh);
-            tma_load_3d(d + 3 * PLANE, &tm2l, &full[st], 0, t * WALK, bh);
-            bulk_load(v, p.walk.col + row, WALK * 4, &full[st]);
-            if (KEYS) bulk_load(v + WALK * 4, p.walk.delta + row, WALK * 4, &full[st]);
-            bulk_load(v + 2 * WALK * 4, p.walk.scale + row / WALK, 16, &full[st]);
-            issued[st] = G;
-          }
+        for (int j = blockIdx.x; j < p.items && ok; j += gridDim.x) {
+          const Item it = item_of(p, j);
+          ok = it.keys ? load_item<true>(p, p.keys, it, &m.q1h, &m.q1l, &m.q2h, &m.q2l, sh, G)
+                       : load_item<false>(p, p.queries, it, &m.k1h, &m.k1l, &m.k2h, &m.k2l, sh, G);
         }
-        if (*abort_flag)  // never leave the CTA while a bulk copy may still write its shared memory
-          for (int s = 0; s < kStages; ++s)
-            if (issued[s] >= 0) mbar_wait(&full[s], (issued[s] / kStages) & 1, p.status, kDevTimeoutProducer, nullptr);
+        if (*sh.abort_flag)  // never leave the CTA while a bulk copy may still write its shared memory
+          for (int g = G < kStages ? 0 : G - kStages; g < G; ++g)
+            mbar_wait(&sh.full[g % kStages], (g / kStages) & 1, p.status, kDevTimeoutProducer, nullptr);
       }
     } else if (warp == 1) {
-      // ---------------- all MMAs, in one thread's order ----------------
-      // X, Y of tile t + 1 are issued ahead of tile t's accumulating products, so the tensor core
-      // has them to do while e, ds of tile t are formed.  Their buffer's last readers, the
-      // products of tile t - 1, come before them in the same order.
       if (elect_one()) {
-        constexpr uint32_t idesc_xy = idesc_f16_f32(HELD, WALK);
-        constexpr uint32_t idesc_acc = idesc_f16_f32(HELD, D) | (1u << 16);  // B MN-major
-        bool ok = true;
-        auto form_xy = [&](int G) -> bool {
-          const int st = G % kStages;
-          if (!mbar_wait(&full[st], (G / kStages) & 1, p.status, kDevTimeoutMma, abort_flag)) return false;
+        int i = 0;
+        for (int j = blockIdx.x; j < p.items && ok; j += gridDim.x, ++i) {
+          const Item it = item_of(p, j);
+          ok = mbar_wait(sh.held_full, i & 1, p.status, kDevTimeoutMma, sh.abort_flag);
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t g = smem_u32(tiles + st * STAGE);
-          const uint32_t x = tmem + XY_COL + (G & 1) * 128;
-#pragma unroll 1
-          for (int o = 0; o < 2; ++o) {  // X from F1, G1, then Y from F2, G2
-            const uint32_t f = tmem + F_COL + o * 64, gh = g + o * 2 * PLANE, d = x + o * 64;
-#pragma unroll 1
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint64_t b_h = sw128_kmajor_desc(gh + kk * 32), b_l = sw128_kmajor_desc(gh + PLANE + kk * 32);
-              mma_f16_ts(d, f + kk * 8, b_h, idesc_xy, kk != 0);
-              mma_f16_ts(d, f + kk * 8, b_l, idesc_xy, 1);
-              mma_f16_ts(d, f + 32 + kk * 8, b_h, idesc_xy, 1);
-            }
-          }
-          mma_commit(&xy_full[G & 1]);
-          return true;
-        };
-        for (int i = 0; i < my_items && ok; ++i) {
-          ok = mbar_wait(held_full, i & 1, p.status, kDevTimeoutMma, abort_flag);
-          if (ok) {
-            tc_fence_after();
-            ok = form_xy(i * T);
-          }
-          for (int t = 0; t < T && ok; ++t) {
-            const int G = i * T + t, st = G % kStages;
-            if (t + 1 < T) ok = form_xy(G + 1);
-            // the keys' pass has one buffer of accumulators, the queries' pass two
-            const int prev = KEYS ? G - 1 : G - 2;
-            ok = ok && mbar_wait(&ed_full[G & 1], (G >> 1) & 1, p.status, kDevTimeoutMma, abort_flag) &&
-                 (prev < 0 || mbar_wait(&acc_free[prev & 1], (prev >> 1) & 1, p.status, kDevTimeoutMma, abort_flag));
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t g = smem_u32(tiles + st * STAGE);
-            const uint32_t x = tmem + XY_COL + (G & 1) * 128;
-#pragma unroll 1
-            for (int o = KEYS ? 0 : 1; o < 2; ++o) {  // acc2 from e and G2, then acc1 from ds and G1
-              const uint32_t a = x + o * 64, gh = g + (1 - o) * 2 * PLANE;
-              const uint32_t d = tmem + ACC_COL + (KEYS ? (1 - o) * 64 : (G & 1) * 64);
-#pragma unroll 1
-              for (int kk = 0; kk < WALK / 16; ++kk) {
-                const uint64_t b_h = sw128_mnmajor_desc(gh + kk * 2048), b_l = sw128_mnmajor_desc(gh + PLANE + kk * 2048);
-                mma_f16_ts(d, a + kk * 16, b_h, idesc_acc, kk != 0);
-                mma_f16_ts(d, a + kk * 16, b_l, idesc_acc, 1);
-                mma_f16_ts(d, a + kk * 16 + 8, b_h, idesc_acc, 1);
-              }
-            }
-            mma_commit(&empty[st]);
-            mma_commit(&acc_full[G & 1]);
-          }
+          ok = it.keys ? mma_item<true>(p, it.n, sh, tmem, G, P) : mma_item<false>(p, it.n, sh, tmem, G, P);
         }
-        mma_commit(all_done);
-        mbar_wait(all_done, 0, p.status, kDevTimeoutMma, nullptr);
+        mma_commit(sh.all_done);
+        mbar_wait(sh.all_done, 0, p.status, kDevTimeoutMma, nullptr);
       }
     }
   } else {
     setmaxnreg_inc<REGS_COMPUTE>();
-    // ---------------- e, ds and the folds: warpgroup w has walked rows 32w..32w+31 ----------------
-    const int w = (warp - 4) >> 2;
-    const uint32_t sub = warp & 3;
-    const int r = sub * 32 + lane;  // held row == tensor-memory lane
-    const uint32_t trow = tmem + ((sub * 32) << 16);
-    constexpr int NACC = KEYS ? 64 : 32;  // keys: w = 0 keeps dV, w = 1 dK; queries: half of dQ each
-    bool ok = true;
-    for (int i = 0; i < my_items && ok; ++i) {
-      int bh, f0;
-      item_of(i, bh, f0);
-      const int64_t frow = (int64_t)bh * p.held.Lt + f0 + r;
-      {
-        // held operands into tensor memory: this warpgroup's pair of planes
-        const __half* hi = w == 0 ? p.held.hi1 : p.held.hi2;
-        const __half* lo = w == 0 ? p.held.lo1 : p.held.lo2;
-#pragma unroll
-        for (int pl = 0; pl < 2; ++pl) {
-          const uint4* src = reinterpret_cast<const uint4*>((pl == 0 ? hi : lo) + frow * D);
-          uint32_t v[32];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint4 u = __ldg(src + k);
-            v[4 * k] = u.x; v[4 * k + 1] = u.y; v[4 * k + 2] = u.z; v[4 * k + 3] = u.w;
-          }
-          tmem_st32(trow + F_COL + w * 64 + pl * 32, v);
-        }
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(held_full);
-      }
-      const TileScale fs = p.held.scale[frow / WALK];
-      const float head = p.head[bh];
-      // row constants: queries' pass -m_i and -delta_i, keys' pass b_j
-      const float row = p.held.col[frow] + E_LIFT;
-      const float row_delta = KEYS ? 0.0f : p.held.delta[frow];
-      const uint64_t row2 = f2pack(row, row);
-      float acc[NACC];
-#pragma unroll
-      for (int k = 0; k < NACC; ++k) acc[k] = 0.0f;
-      float db = 0.0f, fold_scale = 0.0f;
-      // adds the accumulators of tile G to the registers
-      auto fold = [&](int G) -> bool {
-        if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[G & 1], (G >> 1) & 1, p.status, kDevTimeoutConsumer, abort_flag)))
-          return false;
-        tc_fence_after();
-        const uint32_t src = trow + ACC_COL + (KEYS ? (w == 0 ? 64 : 0) : (G & 1) * 64 + w * 32);
-        const uint64_t s2 = f2pack(fold_scale, fold_scale);
-#pragma unroll
-        for (int c = 0; c < NACC / 32; ++c) {
-          uint32_t v[32];
-          tmem_ld32(src + c * 32, v);
-          tmem_wait_ld();
-          reg_fence(v);
-#pragma unroll
-          for (int k = 0; k < 32; k += 2)
-            f2unpack(f2fma(f2pack(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), s2,
-                           f2pack(acc[c * 32 + k], acc[c * 32 + k + 1])),
-                     acc[c * 32 + k], acc[c * 32 + k + 1]);
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_free[G & 1]);
-        return true;
-      };
-      for (int t = 0; t < T; ++t) {
-        const int G = i * T + t, st = G % kStages;
-        // the tile's vectors (their copy's completion seen by this thread) and its X, Y
-        ok = mbar_wait(&full[st], (G / kStages) & 1, p.status, kDevTimeoutConsumer, abort_flag) &&
-             mbar_wait(&xy_full[G & 1], (G >> 1) & 1, p.status, kDevTimeoutConsumer, abort_flag);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        tc_fence_after();
-        const uint8_t* v = vecs + st * VEC_STAGE;
-        const float4* col = reinterpret_cast<const float4*>(v) + w * 8;
-        const float4* del = reinterpret_cast<const float4*>(v + WALK * 4) + w * 8;
-        const TileScale ws = *reinterpret_cast<const TileScale*>(v + 2 * WALK * 4);
-        const float c = 0.125f * LOG2E * head * fs.inv1 * ws.inv1;
-        // ds is formed as ds * 2^kk with |ds| 2^kk <= 2^15: e <= 2^8, |Y - delta| <= bound < 2^(ilogb + 1)
-        const float bound = fs.norm * ws.norm + (KEYS ? ws.delta : fs.delta);
-        int kk = 6 - ((__float_as_int(bound) >> 23) - 127);
-        kk = kk > 100 ? 100 : (kk < -100 ? -100 : kk);
-        const float up = pow2i(kk);
-        const float a = fs.inv2 * ws.inv2;
-        const uint64_t c2 = f2pack(c, c), a2 = f2pack(a, a);
-        const uint64_t b2 = f2pack(up * 0x1p-7f, up * 0x1p-7f);  // takes the lift of e back
-        const uint64_t rd2 = f2pack(row_delta, row_delta);
-        const uint32_t x0 = trow + XY_COL + (G & 1) * 128 + w * 32;
-        uint32_t xv[32], yv[32];
-        tmem_ld32(x0, xv);
-        tmem_ld32(x0 + 64, yv);
-        tmem_wait_ld();
-        reg_fence(xv);
-        reg_fence(yv);
-        uint64_t dsum = 0ull;
-#pragma unroll
-        for (int ch = 0; ch < 2; ++ch) {  // 16 walked rows: 8 columns of hi pairs, 8 of lo pairs
-          uint32_t pe[16], pd[16];
-#pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            const int q = ch * 16 + j;
-            const float4 cv = col[q / 4];
-            const float4 dv = KEYS ? del[q / 4] : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int k = q + 2 * h;
-              const uint64_t off = f2add(h == 0 ? f2pack(cv.x, cv.y) : f2pack(cv.z, cv.w), row2);
-              float e0, e1;
-              f2unpack(f2fma(f2pack(__uint_as_float(xv[k]), __uint_as_float(xv[k + 1])), c2, off), e0, e1);
-              e0 = ex2(e0);
-              e1 = ex2(e1);
-              const uint64_t e = f2pack(e0, e1);
-              const uint64_t nd = KEYS ? (h == 0 ? f2pack(dv.x, dv.y) : f2pack(dv.z, dv.w)) : rd2;
-              const uint64_t y = f2fma(f2pack(__uint_as_float(yv[k]), __uint_as_float(yv[k + 1])), a2, nd);
-              const uint64_t ds = f2mul(f2mul(e, b2), y);
-              if (KEYS) {
-                split2(e, pe[j / 2 + h], pe[8 + j / 2 + h]);
-                dsum = f2add(dsum, ds);
-              }
-              split2(ds, pd[j / 2 + h], pd[8 + j / 2 + h]);
-            }
-          }
-          if (KEYS) tmem_st16(x0 + ch * 16, pe);
-          tmem_st16(x0 + 64 + ch * 16, pd);
-        }
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ed_full[G & 1]);
-        if (t > 0 && !fold(G - 1)) { ok = false; break; }
-        const float down = pow2i(-kk);
-        if (KEYS) {
-          fold_scale = w == 0 ? ws.inv2 * 0x1p-7f : ws.inv1 * down;
-          float d0, d1;
-          f2unpack(dsum, d0, d1);
-          db = fmaf(d0 + d1, down, db);
-        } else {
-          fold_scale = ws.inv1 * down;
-        }
-      }
-      if (ok && T > 0) ok = fold(i * T + T - 1);
-      if (!ok) break;
-      // ---- the held rows' gradients ----
-      const int b = bh / p.H, h = bh - b * p.H;
-      if (f0 + r < p.held.L) {
-        const bool first = !KEYS || w == 1;  // out1 (dK, dQ) or out2 (dV)
-        float* dst = first ? p.out1 + b * p.s1b + h * p.s1h + (int64_t)(f0 + r) * p.s1l + (KEYS ? 0 : w * 32)
-                           : p.out2 + b * p.s2b + h * p.s2h + (int64_t)(f0 + r) * p.s2l;
-        const float s = first ? 0.125f : 1.0f;
-        if (p.vec_out) {
-#pragma unroll
-          for (int k = 0; k < NACC; k += 4)
-            *reinterpret_cast<float4*>(dst + k) =
-                make_float4(acc[k] * s, acc[k + 1] * s, acc[k + 2] * s, acc[k + 3] * s);
-        } else {
-#pragma unroll
-          for (int k = 0; k < NACC; ++k) dst[k] = acc[k] * s;
-        }
-      }
-      if (KEYS && p.db) p.db[(int64_t)w * p.BH * p.held.Lt + frow] = db;
+    for (int j = blockIdx.x; j < p.items && ok; j += gridDim.x) {
+      const Item it = item_of(p, j);
+      ok = it.keys ? compute_item<true, BIAS>(p, p.keys, it, sh, tmem, G, P)
+                   : compute_item<false, BIAS>(p, p.queries, it, sh, tmem, G, P);
     }
   }
-
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -511,37 +614,38 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Preparation
 // ---------------------------------------------------------------------------
 
-// One block per (b, h): the key bias relative to its largest finite value, times `unit`, clamped to
-// -1e6 (2^-1e6 is zero next to the largest), -inf kept; zeros without a bias; -inf past Lk.  head[bh]
-// = 0 where the largest is beyond 2^60 in magnitude.
-__global__ void __launch_bounds__(256) bias_rows_k(const float* __restrict__ bias, int bias_b, int bias_h, int H,
-                                                   int Lk, int Lt, float unit, float* __restrict__ out,
-                                                   float* __restrict__ head) {
+// The key bias of the softmax: relative to the row's largest, clamped to -1e6 (2^-1e6 is zero next to
+// the largest), -inf kept.
+__device__ __forceinline__ float relative_bias(float v, float mx) {
+  const float d = v - mx;  // NaN for NaN and for +inf
+  return v == -INFINITY ? v : (d < -1.0e6f ? -1.0e6f : d);
+}
+
+// Which bias row (b, h) reads: [bias_b, bias_h, Lk] with 1 for a shared dimension.
+struct Bias {
+  const float* p;
+  int b, h, L;
+  __device__ __forceinline__ const float* row(int ib, int ih) const {
+    return p + ((int64_t)(b == 1 ? 0 : ib) * h + (h == 1 ? 0 : ih)) * L;
+  }
+};
+
+// One block per (b, h): the row's largest bias, where it leaves the scores weight (head = 0 beyond
+// 2^60 in magnitude), both behind the statistics for the backward pass, and the relative bias.
+__global__ void __launch_bounds__(256) bias_rows_k(Bias bias, int H, float* __restrict__ out, float2* head, int64_t head_stride) {
   __shared__ float sm[8];
   const int bh = blockIdx.x, b = bh / H, h = bh - b * H;
-  const float* src = bias ? bias + ((int64_t)(bias_b == 1 ? 0 : b) * bias_h + (bias_h == 1 ? 0 : h)) * Lk : nullptr;
+  const float* src = bias.row(b, h);
   float mx = -INFINITY;
-  if (src)
-    for (int j = threadIdx.x; j < Lk; j += 256) mx = fmaxf(mx, src[j]);
+  for (int j = threadIdx.x; j < bias.L; j += 256) mx = fmaxf(mx, src[j]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = mx;
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < 8; ++k) mx = fmaxf(mx, sm[k]);
-  if (threadIdx.x == 0) head[bh] = mx > -INFINITY && fabsf(mx) > 0x1p60f ? 0.0f : 1.0f;
-  for (int j = threadIdx.x; j < Lt; j += 256) {
-    float v = j < Lk ? 0.0f : -INFINITY;
-    if (src && j < Lk) {
-      v = src[j];
-      if (v != -INFINITY) {
-        v -= mx;
-        if (v < -1.0e6f) v = -1.0e6f;
-        v *= unit;
-      }
-    }
-    out[(int64_t)bh * Lt + j] = v;
-  }
+  if (threadIdx.x == 0) head[bh * head_stride] = make_float2(mx, mx > -INFINITY && fabsf(mx) > 0x1p60f ? 0.0f : 1.0f);
+  for (int j = threadIdx.x; j < bias.L; j += 256) out[(int64_t)bh * bias.L + j] = relative_bias(src[j], mx);
 }
 
 struct Rows {
@@ -607,108 +711,135 @@ __device__ __forceinline__ float4 block_max4(float4 v, float4* sm) {
   return v;
 }
 
-// One block per (b h, 64-row tile), four threads per row: the planes, vectors and scales of one side.
-// Queries (KEYS = false): Q and g = dO / l, -m, -delta.  Keys: K and V, rows with a bias of -inf as zeros.
-template <bool KEYS>
-__global__ void __launch_bounds__(256) bwd_split_k(Rows t1, Rows t2, Rows o, const float2* __restrict__ stats,
-                                                   int H, int vec, Side s) {
+// The planes, vectors and scales of both sides of the backward pass.  One block per (b h, 128-row
+// tile), the keys' tiles first; a thread has a quarter of rows j and j + 64.  Keys: K and V, rows with
+// a bias of -inf as zeros, the relative bias in log2 units (-inf past the end).  Queries: Q and
+// g = dO / l, 7 - m, -delta.
+__global__ void __launch_bounds__(256) bwd_split_k(Rows q, Rows dout, Rows out, Rows k, Rows v, Bias bias,
+                                                   const float2* __restrict__ stats, int64_t stats_ld, int H, int vec,
+                                                   Side qs, Side ks) {
   __shared__ float4 sm[8];
-  const int bh = blockIdx.x, b = bh / H, h = bh - b * H;
-  const int row = blockIdx.y * WALK + (threadIdx.x >> 2), c0 = (threadIdx.x & 3) * 16;
-  const int64_t prow = (int64_t)bh * s.Lt + row;
-  float x[16], y[16];
+  const int bh = blockIdx.x, b = bh / H, h = bh - b * H, c0 = (threadIdx.x & 3) * 16;
+  const int key_tiles = ks.Lt / HELD;
+  const bool keys = (int)blockIdx.y < key_tiles;
+  const Side& s = keys ? ks : qs;
+  const int row0 = (keys ? blockIdx.y : blockIdx.y - key_tiles) * HELD + (threadIdx.x >> 2);
+  float x[2][16], y[2][16], sq[2] = {0.0f, 0.0f}, delta[2] = {0.0f, 0.0f}, col[2] = {-INFINITY, -INFINITY};
+  if (keys) {
+    const float mx = bias.p ? stats[bh * stats_ld + stats_ld - 1].x : 0.0f;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) x[k] = y[k] = 0.0f;
-  float delta = 0.0f;
-  if (row < s.L) {
-    if (KEYS) {
-      if (s.col[prow] != -INFINITY) {
-        load16(t1.at(b, h, row) + c0, vec, x);
-        load16(t2.at(b, h, row) + c0, vec, y);
+    for (int u = 0; u < 2; ++u) {
+      const int row = row0 + 64 * u;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[u][e] = y[u][e] = 0.0f;
+      if (row < s.L) col[u] = bias.p ? relative_bias(bias.row(b, h)[row], mx) * LOG2E : 0.0f;
+      if (col[u] != -INFINITY) {
+        load16(k.at(b, h, row) + c0, vec, x[u]);
+        load16(v.at(b, h, row) + c0, vec, y[u]);
       }
-    } else {
-      const float2 ml = stats[(int64_t)bh * s.L + row];
-      load16(t1.at(b, h, row) + c0, vec, x);
-      if (ml.y != 0.0f) {
-        float ov[16];
-        load16(t2.at(b, h, row) + c0, vec, y);
-        load16(o.at(b, h, row) + c0, vec, ov);
-        const float inv = 1.0f / ml.y;
+    }
+  } else {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          y[k] *= inv;
-          delta = fmaf(y[k], ov[k], delta);
-        }
+    for (int u = 0; u < 2; ++u) {
+      const int row = row0 + 64 * u;
+      float ov[16];
+      float2 ml = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[u][e] = y[u][e] = ov[e] = 0.0f;
+      if (row < s.L) {
+        load16(q.at(b, h, row) + c0, vec, x[u]);
+        load16(dout.at(b, h, row) + c0, vec, y[u]);
+        load16(out.at(b, h, row) + c0, vec, ov);
+        ml = stats[bh * stats_ld + row];
+      }
+      const bool any = ml.y != 0.0f;  // a row without a key gives nothing, whatever dO holds
+      const float inv = any ? 1.0f / ml.y : 0.0f;
+      if (any) col[u] = E_LIFT - ml.x;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        y[u][e] = any ? y[u][e] * inv : 0.0f;
+        delta[u] = fmaf(y[u][e], ov[e], delta[u]);
       }
     }
   }
-  float sq = 0.0f;
+  float4 mx = make_float4(fmaxf(absmax16(x[0]), absmax16(x[1])), fmaxf(absmax16(y[0]), absmax16(y[1])), 0.0f, 0.0f);
 #pragma unroll
-  for (int k = 0; k < 16; ++k) sq = fmaf(y[k], y[k], sq);
+  for (int u = 0; u < 2; ++u) {
 #pragma unroll
-  for (int i = 1; i < 4; i <<= 1) {
-    sq += __shfl_xor_sync(0xffffffffu, sq, i);
-    delta += __shfl_xor_sync(0xffffffffu, delta, i);
+    for (int e = 0; e < 16; ++e) sq[u] = fmaf(y[u][e], y[u][e], sq[u]);
+#pragma unroll
+    for (int i = 1; i < 4; i <<= 1) {
+      sq[u] += __shfl_xor_sync(0xffffffffu, sq[u], i);
+      delta[u] += __shfl_xor_sync(0xffffffffu, delta[u], i);
+    }
+    mx.z = fmaxf(mx.z, sqrtf(sq[u]));
+    mx.w = fmaxf(mx.w, fabsf(delta[u]));
   }
-  if (!KEYS && (threadIdx.x & 3) == 0) {
-    const float2 ml = row < s.L ? stats[(int64_t)bh * s.L + row] : make_float2(0.0f, 0.0f);
-    s.col[prow] = ml.y != 0.0f ? -ml.x : -INFINITY;
-    s.delta[prow] = -delta;
-  }
-  const float4 mx = block_max4(make_float4(absmax16(x), absmax16(y), sqrtf(sq), fabsf(delta)), sm);
+  mx = block_max4(mx, sm);
   const int s1 = scale_shift(mx.x), s2 = scale_shift(mx.y);
-  if (threadIdx.x == 0)
-    s.scale[prow / WALK] = {pow2i(-s1), pow2i(-s2), mx.z * 1.0001f, KEYS ? 0.0f : mx.w * 1.0001f};
-  store_split16(x, pow2i(s1), s.hi1 + prow * D + c0, s.lo1 + prow * D + c0);
-  store_split16(y, pow2i(s2), s.hi2 + prow * D + c0, s.lo2 + prow * D + c0);
+  const int64_t prow0 = (int64_t)bh * s.Lt + row0;
+  if (threadIdx.x == 0)  // the norms a little up: they bound what is formed from rounded values
+    s.scale[prow0 / HELD] = {pow2i(-s1), pow2i(-s2), mx.z * 1.0001f, mx.w * 1.0001f};
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int64_t prow = prow0 + 64 * u;
+    if ((threadIdx.x & 3) == 0) {
+      s.col[prow] = col[u];
+      if (!keys) s.delta[prow] = -delta[u];
+    }
+    store_split16(x[u], pow2i(s1), s.hi1 + prow * D + c0, s.lo1 + prow * D + c0);
+    store_split16(y[u], pow2i(s2), s.hi2 + prow * D + c0, s.lo2 + prow * D + c0);
+  }
 }
 
-// The forward kernel's planes (sdpa_planes.h) from strided tensors.  Queries: one scale per row,
-// four threads per row, 64 rows per block.
-__global__ void __launch_bounds__(256) fwd_split_q_k(Rows q, const float* __restrict__ head, int H, int Lq, int vec,
-                                                     __half* __restrict__ hi, __half* __restrict__ lo,
-                                                     float* __restrict__ qinv) {
-  const int bh = blockIdx.x, b = bh / H, h = bh - b * H;
-  const int row = blockIdx.y * WALK + (threadIdx.x >> 2), c0 = (threadIdx.x & 3) * 16;
-  float x[16];
-#pragma unroll
-  for (int k = 0; k < 16; ++k) x[k] = 0.0f;
-  if (row < Lq) load16(q.at(b, h, row) + c0, vec, x);
-  float mx = absmax16(x);
-#pragma unroll
-  for (int i = 1; i < 4; i <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
-  if (row >= Lq) return;
-  const int s = scale_shift(mx);
-  const int64_t prow = (int64_t)bh * Lq + row;
-  store_split16(x, pow2i(s), hi + prow * D + c0, lo + prow * D + c0);
-  if ((threadIdx.x & 3) == 0) qinv[prow] = pow2i(-s) * head[bh];
-}
-
-// Keys: one block per 128-key tile (one scale each for K and V), eight warps of 16 keys; V goes
-// through shared memory to its transposed planes.
+// The forward kernel's planes (sdpa_planes.h) from strided tensors.  One block per (b h, 128-row tile),
+// the keys' tiles first, threads as above.  Keys: one scale each for K and V of a tile, V through
+// shared memory to its transposed planes.  Queries: one scale per row.
 constexpr int KT = 128;
-__global__ void __launch_bounds__(256) fwd_split_kv_k(Rows kr, Rows vr, const float* __restrict__ bias, int H, int Lk,
-                                                      int Lkt, int vec, __half* __restrict__ khi,
-                                                      __half* __restrict__ klo, __half* __restrict__ vhi,
-                                                      __half* __restrict__ vlo, float* __restrict__ kinv,
-                                                      float* __restrict__ vinv) {
+__global__ void __launch_bounds__(256) fwd_split_k(Rows q, Rows k, Rows v, Bias bias, float2* head, int64_t head_stride,
+                                                   int H, int Lq, int Lk, int vec, SplitPlanesSdpa sp) {
   __shared__ float vt[KT][D + 1];
   __shared__ float4 sm[8];
-  const int bh = blockIdx.x, b = bh / H, h = bh - b * H, tile = blockIdx.y;
+  const int bh = blockIdx.x, b = bh / H, h = bh - b * H, c0 = (threadIdx.x & 3) * 16;
   float x[2][16];
+  if ((int)blockIdx.y >= sp.T) {
+    const int row0 = (blockIdx.y - sp.T) * KT + (threadIdx.x >> 2);
+    float weight = 1.0f;
+    if (bias.p) weight = head[bh * head_stride].y;
+    else if (row0 == 0 && threadIdx.x == 0) head[bh * head_stride] = make_float2(0.0f, 1.0f);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[u][e] = 0.0f;
+      if (row0 + 64 * u < Lq) load16(q.at(b, h, row0 + 64 * u) + c0, vec, x[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float mx = absmax16(x[u]);
+#pragma unroll
+      for (int i = 1; i < 4; i <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
+      if (row0 + 64 * u >= Lq) continue;
+      const int s = scale_shift(mx);
+      const int64_t prow = (int64_t)bh * Lq + row0 + 64 * u;
+      store_split16(x[u], pow2i(s), sp.qhi + prow * D + c0, sp.qlo + prow * D + c0);
+      if ((threadIdx.x & 3) == 0) sp.qinv[prow] = pow2i(-s) * weight;
+    }
+    return;
+  }
+  const int tile = blockIdx.y, row0 = tile * KT + (threadIdx.x >> 2);
   float kmx = 0.0f, vmx = 0.0f;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const int j = u * 64 + (threadIdx.x >> 2), row = tile * KT + j, c0 = (threadIdx.x & 3) * 16;
+    const int j = u * 64 + (threadIdx.x >> 2), row = row0 + u * 64;
     float y[16];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) x[u][k] = y[k] = 0.0f;
-    if (row < Lk && !(bias && bias[(int64_t)bh * Lk + row] == -INFINITY)) {
-      load16(kr.at(b, h, row) + c0, vec, x[u]);
-      load16(vr.at(b, h, row) + c0, vec, y);
+    for (int e = 0; e < 16; ++e) x[u][e] = y[e] = 0.0f;
+    if (row < Lk && !(bias.p && bias.row(b, h)[row] == -INFINITY)) {
+      load16(k.at(b, h, row) + c0, vec, x[u]);
+      load16(v.at(b, h, row) + c0, vec, y);
     }
 #pragma unroll
-    for (int k = 0; k < 16; ++k) vt[j][c0 + k] = y[k];
+    for (int e = 0; e < 16; ++e) vt[j][c0 + e] = y[e];
     kmx = fmaxf(kmx, absmax16(x[u]));
     vmx = fmaxf(vmx, absmax16(y));
   }
@@ -720,27 +851,42 @@ __global__ void __launch_bounds__(256) fwd_split_kv_k(Rows kr, Rows vr, const fl
   const int sv = mx.y == 0.0f ? 60 : max(-60, min(60, scale_shift(mx.y)));
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const int64_t prow = (int64_t)bh * Lkt + tile * KT + u * 64 + (threadIdx.x >> 2);
-    const int c0 = (threadIdx.x & 3) * 16;
-    store_split16(x[u], pow2i(sk), khi + prow * D + c0, klo + prow * D + c0);
+    const int64_t prow = (int64_t)bh * sp.Lkt + row0 + u * 64;
+    store_split16(x[u], pow2i(sk), sp.khi + prow * D + c0, sp.klo + prow * D + c0);
   }
   for (int e = threadIdx.x; e < D * (KT / 16); e += 256) {
     const int d = e % D, jb = e / D * 16;
-    float v[16];
+    float y[16];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) v[k] = vt[jb + k][d];
-    const int64_t off = ((int64_t)bh * D + d) * Lkt + tile * KT + jb;
-    store_split16(v, pow2i(sv), vhi + off, vlo + off);
+    for (int i = 0; i < 16; ++i) y[i] = vt[jb + i][d];
+    const int64_t off = ((int64_t)bh * D + d) * sp.Lkt + tile * KT + jb;
+    store_split16(y, pow2i(sv), sp.vhi + off, sp.vlo + off);
   }
   if (threadIdx.x == 0) {
-    kinv[(int64_t)bh * (Lkt / KT) + tile] = pow2i(-sk);
-    vinv[(int64_t)bh * (Lkt / KT) + tile] = pow2i(-sv);
+    sp.kinv[(int64_t)bh * sp.T + tile] = pow2i(-sk);
+    sp.vinv[(int64_t)bh * sp.T + tile] = pow2i(-sv);
   }
 }
 
-// db [bias_b, bias_h, Lk]: part [2, B, H, Lt] added over the halves and the batch entries and heads
+// Gradients of a pass whose walk was cut: its shares' partial sums [cuts, BH, Lt, 64] added in their
+// order, a thread per element.
+__global__ void __launch_bounds__(256) join_k(const float* __restrict__ part, int cuts, int H, int BH, int L, int Lt,
+                                              float* __restrict__ out, int64_t sb, int64_t sh, int64_t sl) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)BH * L * D) return;
+  const int d = (int)(i % D);
+  const int64_t row = i / D % L;
+  const int bh = (int)(i / D / L), b = bh / H, h = bh - b * H;
+  const float* src = part + ((int64_t)bh * Lt + row) * D + d;
+  float s = 0.0f;
+#pragma unroll 4
+  for (int c = 0; c < cuts; ++c) s += src[(int64_t)c * BH * Lt * D];
+  out[b * sb + h * sh + row * sl + d] = s;
+}
+
+// db [bias_b, bias_h, Lk]: part [parts, B, H, Lt] added over the parts and the batch entries and heads
 // that share a row, in their order.
-__global__ void __launch_bounds__(256) bias_grad_k(const float* __restrict__ part, int B, int H, int bias_b,
+__global__ void __launch_bounds__(256) bias_grad_k(const float* __restrict__ part, int parts, int B, int H, int bias_b,
                                                    int bias_h, int Lk, int Lt, float* __restrict__ db) {
   const int j = blockIdx.x * 256 + threadIdx.x, row = blockIdx.y;
   if (j >= Lk) return;
@@ -748,10 +894,11 @@ __global__ void __launch_bounds__(256) bias_grad_k(const float* __restrict__ par
   const int b0 = bias_b == 1 ? 0 : rb, b1 = bias_b == 1 ? B : rb + 1;
   const int h0 = bias_h == 1 ? 0 : rh, h1 = bias_h == 1 ? H : rh + 1;
   float s = 0.0f;
-  for (int b = b0; b < b1; ++b)
-    for (int h = h0; h < h1; ++h) {
-      const int64_t i = ((int64_t)b * H + h) * Lt + j;
-      s += part[i] + part[i + (int64_t)B * H * Lt];
+  for (int g = 0; g < parts; ++g)
+    for (int b = b0; b < b1; ++b) {
+      const float* p = part + ((int64_t)g * B + b) * H * Lt + j;
+#pragma unroll 8
+      for (int h = h0; h < h1; ++h) s += p[(int64_t)h * Lt];
     }
   db[(int64_t)row * Lk + j] = s;
 }
@@ -778,7 +925,7 @@ static size_t side_layout(uint8_t* base, int64_t BH, int L, bool delta, Side& s)
   s.lo2 = reinterpret_cast<__half*>(take(rows * D * 2));
   s.col = reinterpret_cast<float*>(take(rows * 4));
   s.delta = reinterpret_cast<float*>(take(delta ? rows * 4 : 0));
-  s.scale = reinterpret_cast<TileScale*>(take(rows / WALK * sizeof(TileScale)));
+  s.scale = reinterpret_cast<TileScale*>(take(rows / HELD * sizeof(TileScale)));
   return at;
 }
 
@@ -792,36 +939,42 @@ static bool plane_map(CUtensorMap* m, const __half* base, int64_t BH, int Lt) {
 
 // Shared-memory opt-in and the register check of the split budgets, once per device: with fewer
 // registers compiled in, setmaxnreg.inc would wait for ever.
-template <bool KEYS>
+template <bool BIAS>
 static int ensure_kernel() {
   static std::atomic<uint64_t> done{0};
   int dev = 0;
   cudaGetDevice(&dev);
   if (done.load(std::memory_order_acquire) >> (dev & 63) & 1) return kOk;
   cudaFuncAttributes fa{};
-  if (cudaFuncGetAttributes(&fa, sdpa_bwd_tc<KEYS>) != cudaSuccess || fa.numRegs < (int)REGS_LAUNCH) {
+  if (cudaFuncGetAttributes(&fa, sdpa_bwd_tc<BIAS>) != cudaSuccess || fa.numRegs < (int)REGS_LAUNCH) {
     set_last_error("sdpa_bwd_tc was compiled with fewer registers than its warpgroup budget needs");
     return kLaunchFailed;
   }
-  if (cudaFuncSetAttribute(sdpa_bwd_tc<KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess)
+  if (cudaFuncSetAttribute(sdpa_bwd_tc<BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess)
     return launch_status();
   done.fetch_or(1ull << (dev & 63), std::memory_order_acq_rel);
   return kOk;
 }
 
-template <bool KEYS>
-static int launch_bwd(const Params& p, int64_t BH, cudaStream_t stream) {
-  int st = ensure_kernel<KEYS>();
-  if (st != kOk) return st;
-  CUtensorMap m1h, m1l, m2h, m2l;
-  if (!plane_map(&m1h, p.walk.hi1, BH, p.walk.Lt) || !plane_map(&m1l, p.walk.lo1, BH, p.walk.Lt) ||
-      !plane_map(&m2h, p.walk.hi2, BH, p.walk.Lt) || !plane_map(&m2l, p.walk.lo2, BH, p.walk.Lt))
-    return kLaunchFailed;
-  const int64_t items = (int64_t)p.Ft * BH;
-  const int sms = sm_count();
-  LaunchScope scope(kKSdpaAttn, stream);
-  sdpa_bwd_tc<KEYS><<<(unsigned)(items < sms ? items : sms), kThreads, SMEM_BYTES, stream>>>(m1h, m1l, m2h, m2l, p);
-  return launch_status();
+// Cuts a pass's walk where one item would be longer than an SM's share of both passes.  Costs in
+// products of a 64-row tile (keys' pass 4, queries' pass 3), an item's start as much as 4 tiles.
+static void cut_walks(Pass& keys, Pass& queries, int64_t BH) {
+  const int64_t sms = sm_count();
+  int64_t total = 0;
+  for (int q = 0; q < 2; ++q) {
+    const Pass& s = q ? queries : keys;
+    total += BH * s.Ft * (s.T + 4) * (q ? 3 : 4);
+  }
+  const int64_t share = (total + sms - 1) / sms;
+  for (int q = 0; q < 2; ++q) {
+    Pass& s = q ? queries : keys;
+    s.cuts = 1;
+    s.span = s.T;
+    const int64_t fair = share / (q ? 3 : 4) - 4;  // tiles
+    if (s.T <= fair || s.T < 8) continue;
+    s.span = (int)(fair < 4 ? 4 : (fair + 1) / 2 * 2);
+    s.cuts = (s.T + s.span - 1) / s.span;
+  }
 }
 
 // sizes a launch can hold: items * tiles counted in ints, grid rows in 16 bits
@@ -873,30 +1026,23 @@ int triposplat_b200_attention_forward(const float* q, const float* k, const floa
   const int64_t BH = (int64_t)B * H;
   SplitPlanesSdpa sp;
   void* behind = nullptr;
-  const size_t bias_bytes = al256((size_t)BH * Lk * 4);
-  st = sdpa_planes_extra(BH, Lq, Lk, bias_bytes + al256((size_t)BH * 4), stream, sp, &behind);
+  st = sdpa_planes_extra(BH, Lq, Lk, key_bias ? al256((size_t)BH * Lk * 4) : 0, stream, sp, &behind);
   if (st != kOk) return st;
-  float* bias = static_cast<float*>(behind);
-  float* head = reinterpret_cast<float*>(static_cast<uint8_t*>(behind) + bias_bytes);
-  const int vec = rows16({q, k, v}, strides, 3);
-  {
+  float* relative = key_bias ? static_cast<float*>(behind) : nullptr;
+  float2* rows = reinterpret_cast<float2*>(stats);
+  const Bias bias{key_bias, bias_batches, bias_heads, Lk};
+  if (key_bias) {
     LaunchScope scope(kKSdpaSplit, stream);
-    bias_rows_k<<<(unsigned)BH, 256, 0, stream>>>(key_bias, bias_batches, bias_heads, H, Lk, Lk, 1.0f, bias, head);
+    bias_rows_k<<<(unsigned)BH, 256, 0, stream>>>(bias, H, relative, rows + Lq, Lq + 1);
   }
   {
     LaunchScope scope(kKSdpaSplit, stream);
-    fwd_split_q_k<<<dim3((unsigned)BH, (Lq + WALK - 1) / WALK), 256, 0, stream>>>(rows_of(q, strides), head, H, Lq, vec,
-                                                                             sp.qhi, sp.qlo, sp.qinv);
-  }
-  {
-    LaunchScope scope(kKSdpaSplit, stream);
-    fwd_split_kv_k<<<dim3((unsigned)BH, sp.T), 256, 0, stream>>>(rows_of(k, strides + 3), rows_of(v, strides + 6),
-                                                                 key_bias ? bias : nullptr, H, Lk, sp.Lkt, vec, sp.khi,
-                                                                 sp.klo, sp.vhi, sp.vlo, sp.kinv, sp.vinv);
+    fwd_split_k<<<dim3((unsigned)BH, sp.T + (Lq + KT - 1) / KT), 256, 0, stream>>>(
+        rows_of(q, strides), rows_of(k, strides + 3), rows_of(v, strides + 6), bias, rows + Lq, Lq + 1, H, Lq, Lk,
+        rows16({q, k, v}, strides, 3), sp);
   }
   if ((st = launch_status()) != kOk) return st;
-  return sdpa_attend_stats(sp, key_bias ? bias : nullptr, Lk, out_blhd, reinterpret_cast<float2*>(stats), BH, H, Lq, Lk,
-                           stream);
+  return sdpa_attend_stats(sp, relative, Lk, out_blhd, rows, Lq + 1, BH, H, Lq, Lk, stream);
 }
 
 int triposplat_b200_attention_backward(const float* dout, const float* q, const float* k, const float* v,
@@ -915,61 +1061,83 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
   for (const float* p : {dout, q, k, v, out, stats, key_bias, static_cast<const float*>(dq), static_cast<const float*>(dk),
                          static_cast<const float*>(dv), static_cast<const float*>(dbias)})
     if (p && !is_device_pointer(p)) return kNotDevicePointer;
+  st = key_bias ? ensure_kernel<true>() : ensure_kernel<false>();
+  if (st != kOk) return st;
   cudaStream_t stream = current_stream();
   const int64_t BH = (int64_t)B * H;
+  Params p{};
   Side qs{}, ks{};
   const size_t qbytes = side_layout(nullptr, BH, Lq, true, qs), kbytes = side_layout(nullptr, BH, Lk, false, ks);
-  const size_t head_bytes = al256((size_t)BH * 4), db_bytes = dbias ? al256((size_t)2 * BH * ks.Lt * 4) : 0;
-  uint8_t* ws = static_cast<uint8_t*>(workspace(qbytes + kbytes + head_bytes + db_bytes, stream));
+  p.keys.T = (Lq + WALK - 1) / WALK;
+  p.keys.Ft = (Lk + HELD - 1) / HELD;
+  p.keys.ragged = Lq % WALK != 0;
+  p.queries.T = (Lk + WALK - 1) / WALK;
+  p.queries.Ft = (Lq + HELD - 1) / HELD;
+  p.queries.ragged = Lk % WALK != 0;
+  cut_walks(p.keys, p.queries, BH);
+  const size_t kpart = p.keys.cuts > 1 ? al256((size_t)p.keys.cuts * BH * ks.Lt * D * 4) : 0;
+  const size_t qpart = p.queries.cuts > 1 ? al256((size_t)p.queries.cuts * BH * qs.Lt * D * 4) : 0;
+  const size_t db_bytes = dbias ? al256((size_t)2 * p.keys.cuts * BH * ks.Lt * 4) : 0;
+  uint8_t* ws = static_cast<uint8_t*>(workspace(qbytes + kbytes + 2 * kpart + qpart + db_bytes, stream));
   if (!ws) return kWorkspace;
   side_layout(ws, BH, Lq, true, qs);
   side_layout(ws + qbytes, BH, Lk, false, ks);
-  float* head = reinterpret_cast<float*>(ws + qbytes + kbytes);
-  float* part = dbias ? reinterpret_cast<float*>(ws + qbytes + kbytes + head_bytes) : nullptr;
-  const int vec = rows16({dout, q, k, v, out}, strides, 5);
-  {
-    LaunchScope scope(kKSdpaSplit, stream);
-    bias_rows_k<<<(unsigned)BH, 256, 0, stream>>>(key_bias, bias_batches, bias_heads, H, Lk, ks.Lt, LOG2E, ks.col, head);
-  }
-  {
-    LaunchScope scope(kKSdpaSplit, stream);
-    bwd_split_k<true><<<dim3((unsigned)BH, ks.Lt / WALK), 256, 0, stream>>>(
-        rows_of(k, strides + 6), rows_of(v, strides + 9), Rows{}, nullptr, H, vec, ks);
-  }
-  {
-    LaunchScope scope(kKSdpaSplit, stream);
-    bwd_split_k<false><<<dim3((unsigned)BH, qs.Lt / WALK), 256, 0, stream>>>(
-        rows_of(q, strides + 3), rows_of(dout, strides), rows_of(out, strides + 12),
-        reinterpret_cast<const float2*>(stats), H, vec, qs);
-  }
-  if ((st = launch_status()) != kOk) return st;
+  uint8_t* at = ws + qbytes + kbytes;
   const int64_t* go = strides + 15;  // dq, dk, dv
-  Params p{};
-  p.head = head;
+  const int vec_out = rows16({dq, dk, dv}, go, 3);
+  p.keys.held = ks;
+  p.keys.walk = qs;
+  p.keys.out1 = kpart ? reinterpret_cast<float*>(at) : dk;
+  p.keys.out2 = kpart ? reinterpret_cast<float*>(at + kpart) : dv;
+  p.keys.s1b = go[3]; p.keys.s1h = go[4]; p.keys.s1l = go[5];
+  p.keys.s2b = go[6]; p.keys.s2h = go[7]; p.keys.s2l = go[8];
+  p.keys.vec_out = vec_out;
+  p.queries.held = qs;
+  p.queries.walk = ks;
+  p.queries.out1 = qpart ? reinterpret_cast<float*>(at + 2 * kpart) : dq;
+  p.queries.s1b = go[0]; p.queries.s1h = go[1]; p.queries.s1l = go[2];
+  p.queries.vec_out = vec_out;
+  p.db = dbias ? reinterpret_cast<float*>(at + 2 * kpart + qpart) : nullptr;
+  p.head = reinterpret_cast<const float2*>(stats) + Lq;
+  p.head_stride = Lq + 1;
   p.H = H;
   p.BH = (int)BH;
-  p.vec_out = rows16({dq, dk, dv}, go, 3);
+  p.key_items = (int)(BH * p.keys.Ft * p.keys.cuts);
+  p.items = p.key_items + (int)(BH * p.queries.Ft * p.queries.cuts);
   p.status = device_status();
-  p.held = ks;
-  p.walk = qs;
-  p.T = (Lq + WALK - 1) / WALK;
-  p.Ft = (Lk + HELD - 1) / HELD;
-  p.out1 = dk; p.s1b = go[3]; p.s1h = go[4]; p.s1l = go[5];
-  p.out2 = dv; p.s2b = go[6]; p.s2h = go[7]; p.s2l = go[8];
-  p.db = part;
-  if ((st = launch_bwd<true>(p, BH, stream)) != kOk) return st;
-  p.held = qs;
-  p.walk = ks;
-  p.T = (Lk + WALK - 1) / WALK;
-  p.Ft = (Lq + HELD - 1) / HELD;
-  p.out1 = dq; p.s1b = go[0]; p.s1h = go[1]; p.s1l = go[2];
-  p.out2 = nullptr;
-  p.db = nullptr;
-  if ((st = launch_bwd<false>(p, BH, stream)) != kOk) return st;
+  Maps m;
+  if (!plane_map(&m.q1h, qs.hi1, BH, qs.Lt) || !plane_map(&m.q1l, qs.lo1, BH, qs.Lt) ||
+      !plane_map(&m.q2h, qs.hi2, BH, qs.Lt) || !plane_map(&m.q2l, qs.lo2, BH, qs.Lt) ||
+      !plane_map(&m.k1h, ks.hi1, BH, ks.Lt) || !plane_map(&m.k1l, ks.lo1, BH, ks.Lt) ||
+      !plane_map(&m.k2h, ks.hi2, BH, ks.Lt) || !plane_map(&m.k2l, ks.lo2, BH, ks.Lt))
+    return kLaunchFailed;
+  {
+    LaunchScope scope(kKSdpaSplit, stream);
+    bwd_split_k<<<dim3((unsigned)BH, (ks.Lt + qs.Lt) / HELD), 256, 0, stream>>>(
+        rows_of(q, strides + 3), rows_of(dout, strides), rows_of(out, strides + 12), rows_of(k, strides + 6),
+        rows_of(v, strides + 9), Bias{key_bias, bias_batches, bias_heads, Lk}, reinterpret_cast<const float2*>(stats),
+        Lq + 1, H, rows16({dout, q, k, v, out}, strides, 5), qs, ks);
+  }
+  {
+    LaunchScope scope(kKSdpaAttn, stream);
+    const unsigned grid = (unsigned)(p.items < sm_count() ? p.items : sm_count());
+    if (key_bias) sdpa_bwd_tc<true><<<grid, kThreads, SMEM_BYTES, stream>>>(m, p);
+    else sdpa_bwd_tc<false><<<grid, kThreads, SMEM_BYTES, stream>>>(m, p);
+  }
+  auto join = [&](const Pass& s, const float* part, float* dst, const int64_t* g) {
+    LaunchScope scope(kKSdpaSplit, stream);
+    join_k<<<(unsigned)((BH * s.held.L * D + 255) / 256), 256, 0, stream>>>(part, s.cuts, H, (int)BH, s.held.L, s.held.Lt,
+                                                                          dst, g[0], g[1], g[2]);
+  };
+  if (qpart) join(p.queries, p.queries.out1, dq, go);
+  if (kpart) {
+    join(p.keys, p.keys.out1, dk, go + 3);
+    join(p.keys, p.keys.out2, dv, go + 6);
+  }
   if (dbias) {
     LaunchScope scope(kKSdpaSplit, stream);
-    bias_grad_k<<<dim3((Lk + 255) / 256, bias_batches * bias_heads), 256, 0, stream>>>(part, B, H, bias_batches,
-                                                                                     bias_heads, Lk, ks.Lt, dbias);
+    bias_grad_k<<<dim3((Lk + 255) / 256, bias_batches * bias_heads), 256, 0, stream>>>(
+        p.db, 2 * p.keys.cuts, B, H, bias_batches, bias_heads, Lk, ks.Lt, dbias);
   }
   return launch_status();
 }

@@ -237,12 +237,12 @@ def attention_forward(q, k, v, *, key_bias=None):
     """softmax(q k^T / 8 + key_bias) v on q [B, H, Lq, 64] and k, v [B, H, Lk, 64] (float32), key_bias
     [Lk], [B, Lk] or [B, H, Lk].  A key with a bias of -inf does not exist; a query without keys
     gives zeros.  Returns (out, stats): out [B, H, Lq, 64] in token-major storage
-    ([B, Lq, H, 64], what the out-projection reads), stats [B, H, Lq, 2] for the backward pass.
+    ([B, Lq, H, 64], what the out-projection reads), stats [B, H, Lq + 1, 2] for the backward pass.
     Heads shared by several queries' heads are passed expanded."""
     key_bias, bias_dims, (B, H, Lq, Lk) = _attention_args(q, k, v, key_bias)
     q, k, v = _rows(q), _rows(k), _rows(v)
     out = torch.empty((B, Lq, H, 64), dtype=torch.float32, device=q.device)
-    stats = torch.empty((B, H, Lq, 2), dtype=torch.float32, device=q.device)
+    stats = torch.empty((B, H, Lq + 1, 2), dtype=torch.float32, device=q.device)
     lib = _lib(q.device)
     _ok(lib, lib.triposplat_b200_attention_forward(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), _i64(*(s for t in (q, k, v) for s in t.stride()[:3])),
@@ -260,7 +260,7 @@ def attention_backward(dout, q, k, v, out, stats, *, key_bias=None, grads=None, 
     dev = q.device
     dout = _rows(_check(dout, "dout", q.shape, torch.float32, dev))
     out = _rows(_check(out, "out", q.shape, torch.float32, dev))
-    stats = _check(stats, "stats", (B, H, Lq, 2), torch.float32, dev).contiguous()
+    stats = _check(stats, "stats", (B, H, Lq + 1, 2), torch.float32, dev).contiguous()
     q, k, v = _rows(q), _rows(k), _rows(v)
     if grads is None:
         dq, dk, dv = (torch.empty((B, n, H, 64), dtype=torch.float32, device=dev).transpose(1, 2)
