@@ -10,7 +10,7 @@ transposed heads); outputs are contiguous unless said otherwise.
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
@@ -22,12 +22,20 @@ _LAYOUTS = {"interleaved": 0, "halves": 1}
 _KINDS = {None: 0, "layer": 1, "rms": 2}
 
 
+_loaded = None
+
+
 def _lib(device):
-    if device.type != "cuda" or (device.index is not None and device.index != torch.cuda.current_device()):
+    """The library, with PyTorch's current stream set for its next launches."""
+    global _loaded
+    if device.type != "cuda":
+        raise ValueError(f"expected CUDA tensors, got {device}")
+    if device.index is not None and device.index != torch.cuda.current_device():
         raise ValueError(f"expected tensors on the current CUDA device, got {device}")
-    lib = _native.load()
-    _native.use_current_stream(lib)
-    return lib
+    if _loaded is None:
+        _loaded = _native.load()
+    _native.use_current_stream(_loaded)
+    return _loaded
 
 
 def _ok(lib, status, name):
@@ -37,13 +45,13 @@ def _ok(lib, status, name):
 
 def _check(t, name, shape, dtype, device):
     """`t` as a tensor of this shape, type and device (no conversion)."""
+    if t.dtype is dtype and t.shape == shape and t.device == device:
+        return t
     if t.device != device:
         raise ValueError(f"{name} must be on {device}, got {t.device}")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.shape != shape:
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    return t
+    raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
 def _param(t, name, shape, device):
@@ -60,8 +68,21 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _i64(*values):
-    return (ctypes.c_int64 * len(values))(*values)
+# Host arrays of the C interface, as bytes: a small call spends most of its time in Python, and
+# packing takes a third of what filling a ctypes array does.
+_I64 = [struct.Struct(f"{n}q") for n in range(33)]
+
+
+def _i64(values):
+    return _I64[len(values)].pack(*values)
+
+
+def _strides(n, *tensors):
+    """The first n strides of each tensor (zeros for None)."""
+    values = []
+    for t in tensors:
+        values += (0,) * n if t is None else t.stride()[:n]
+    return _i64(values)
 
 
 # ------------------------------------------------------------------------ rotary positions
@@ -86,14 +107,14 @@ def _rope_args(x, positions, inv_freq, axis_pairs, gamma, layout):
     gamma = _param(gamma, "gamma", (H, D), x.device)
     positions = positions.contiguous()
     how = (_DTYPES[x.dtype], _POSITIONS[positions.dtype], L * len(pairs) if positions.dim() == 3 else 0,
-           B, L, H, D, (ctypes.c_int * len(pairs))(*pairs), len(pairs), _LAYOUTS[layout])
+           B, L, H, D, struct.pack(f"{len(pairs)}i", *pairs), len(pairs), _LAYOUTS[layout])
     return positions, inv_freq, gamma, how
 
 
 def _out_like(out, x, name):
     """An output of x's shape and type: `out` if given (unit last stride), a new one otherwise."""
     if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        return x.new_empty(x.shape)
     _check(out, name, x.shape, x.dtype, x.device)
     if out.stride(-1) != 1 and out.shape[-1] != 1:
         raise ValueError(f"{name} needs a contiguous last dimension")
@@ -115,7 +136,7 @@ def axis_rope(x, positions, inv_freq, *, axis_pairs, gamma=None, layout="interle
     lib = _lib(x.device)
     _ok(lib, lib.triposplat_b200_axis_rope(
         x.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), _ptr(gamma), y.data_ptr(),
-        _i64(*x.stride()[:3], *y.stride()[:3]), *how), "axis_rope")
+        _strides(3, x, y), *how), "axis_rope")
     return y
 
 
@@ -129,12 +150,11 @@ def axis_rope_backward(dy, x, positions, inv_freq, *, axis_pairs, gamma=None, la
         x = _rows(_check(x, "x", dy.shape, dy.dtype, dy.device))
     dx = _out_like(out, dy, "out")
     dgamma = None if gamma is None else torch.empty_like(gamma)
-    xs = x.stride()[:3] if gamma is not None else (0, 0, 0)
     lib = _lib(dy.device)
     _ok(lib, lib.triposplat_b200_axis_rope_backward(
         dy.data_ptr(), x.data_ptr() if gamma is not None else None, positions.data_ptr(),
         inv_freq.data_ptr(), _ptr(gamma), dx.data_ptr(), _ptr(dgamma),
-        _i64(*dy.stride()[:3], *xs, *dx.stride()[:3]), *how), "axis_rope_backward")
+        _strides(3, dy, x if gamma is not None else None, dx), *how), "axis_rope_backward")
     return dx, dgamma
 
 
@@ -172,12 +192,12 @@ def norm_gate(x, y, *, gate=None, scale=None, shift=None, pre="layer", pre_weigh
     gate, scale, shift, wpre, wpost = _norm_args(x, y, gate, scale, shift, pre, pre_weight, post, post_weight)
     x, y = _rows(x), _rows(y)
     B, L, C = x.shape
-    z = torch.empty((B, L, C), dtype=x.dtype, device=x.device)
-    h = torch.empty_like(z) if pre is not None else None
-    stats = torch.empty((B, L, 4), dtype=torch.float32, device=x.device)
+    z = x.new_empty((B, L, C))
+    h = x.new_empty((B, L, C)) if pre is not None else None
+    stats = x.new_empty((B, L, 4), dtype=torch.float32)
     lib = _lib(x.device)
     _ok(lib, lib.triposplat_b200_norm_gate(
-        x.data_ptr(), y.data_ptr(), _i64(*x.stride()[:2], *y.stride()[:2]), _ptr(gate), _ptr(scale), _ptr(shift),
+        x.data_ptr(), y.data_ptr(), _strides(2, x, y), _ptr(gate), _ptr(scale), _ptr(shift),
         _ptr(wpre), _ptr(wpost), z.data_ptr(), _ptr(h), stats.data_ptr(), _DTYPES[x.dtype], B, L, C, _KINDS[pre],
         _KINDS[post], float(residual_scale), float(eps)), "norm_gate")
     return z, h, stats
@@ -197,15 +217,13 @@ def norm_gate_backward(dz, dh, x, y, stats, *, gate=None, scale=None, shift=None
     x, y = _rows(x), _rows(y)
     B, L, C = x.shape
     stats = _check(stats, "stats", (B, L, 4), torch.float32, x.device).contiguous()
-    dx = torch.empty((B, L, C), dtype=x.dtype, device=x.device)
-    g = {"x": dx, "y": torch.empty_like(dx)}
+    g = {"x": x.new_empty((B, L, C)), "y": x.new_empty((B, L, C))}
     for name, t in (("gate", gate), ("scale", scale), ("shift", shift), ("pre_weight", wpre),
                     ("post_weight", wpost)):
         g[name] = None if t is None else torch.empty_like(t)
-    strides = _i64(*(s for t in (x, y, dz, dh) for s in ((0, 0) if t is None else t.stride()[:2])))
     lib = _lib(x.device)
     _ok(lib, lib.triposplat_b200_norm_gate_backward(
-        _ptr(dz), _ptr(dh), x.data_ptr(), y.data_ptr(), strides, stats.data_ptr(), _ptr(gate), _ptr(scale),
+        _ptr(dz), _ptr(dh), x.data_ptr(), y.data_ptr(), _strides(2, x, y, dz, dh), stats.data_ptr(), _ptr(gate), _ptr(scale),
         _ptr(wpre), _ptr(wpost), g["x"].data_ptr(), g["y"].data_ptr(), _ptr(g["gate"]), _ptr(g["scale"]),
         _ptr(g["shift"]), _ptr(g["pre_weight"]), _ptr(g["post_weight"]), _DTYPES[x.dtype], B, L, C, _KINDS[pre],
         _KINDS[post], float(residual_scale)), "norm_gate_backward")
@@ -241,11 +259,11 @@ def attention_forward(q, k, v, *, key_bias=None):
     Heads shared by several queries' heads are passed expanded."""
     key_bias, bias_dims, (B, H, Lq, Lk) = _attention_args(q, k, v, key_bias)
     q, k, v = _rows(q), _rows(k), _rows(v)
-    out = torch.empty((B, Lq, H, 64), dtype=torch.float32, device=q.device)
-    stats = torch.empty((B, H, Lq + 1, 2), dtype=torch.float32, device=q.device)
+    out = q.new_empty((B, Lq, H, 64))
+    stats = q.new_empty((B, H, Lq + 1, 2))
     lib = _lib(q.device)
     _ok(lib, lib.triposplat_b200_attention_forward(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), _i64(*(s for t in (q, k, v) for s in t.stride()[:3])),
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(3, q, k, v),
         _ptr(key_bias), *bias_dims, out.data_ptr(), stats.data_ptr(), B, H, Lq, Lk), "attention_forward")
     return out.transpose(1, 2), stats
 
@@ -263,15 +281,14 @@ def attention_backward(dout, q, k, v, out, stats, *, key_bias=None, grads=None, 
     stats = _check(stats, "stats", (B, H, Lq + 1, 2), torch.float32, dev).contiguous()
     q, k, v = _rows(q), _rows(k), _rows(v)
     if grads is None:
-        dq, dk, dv = (torch.empty((B, n, H, 64), dtype=torch.float32, device=dev).transpose(1, 2)
-                      for n in (Lq, Lk, Lk))
+        dq, dk, dv = (q.new_empty((B, n, H, 64)).transpose(1, 2) for n in (Lq, Lk, Lk))
     else:
         dq, dk, dv = (_out_like(g, like, "grads") for g, like in zip(grads, (q, k, v), strict=True))
     dbias = torch.empty_like(key_bias) if key_bias is not None and bias_grad else None
     lib = _lib(dev)
     _ok(lib, lib.triposplat_b200_attention_backward(
         dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), stats.data_ptr(),
-        _i64(*(s for t in (dout, q, k, v, out, dq, dk, dv) for s in t.stride()[:3])), _ptr(key_bias), *bias_dims,
+        _strides(3, dout, q, k, v, out, dq, dk, dv), _ptr(key_bias), *bias_dims,
         dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dbias), B, H, Lq, Lk), "attention_backward")
     return dq, dk, dv, dbias
 
@@ -301,9 +318,10 @@ def clip_grad_norm(grads, max_norm, *, out=None):
             raise ValueError("gradients and outputs must be contiguous, an output of its gradient's shape")
     norm = torch.empty((), dtype=torch.float32, device=device)
     lib = _lib(device)
-    ptrs = (ctypes.c_void_p * n)(*[g.data_ptr() for g in grads])
-    to = None if out is None else (ctypes.c_void_p * n)(*[o.data_ptr() for o in outs])
+    array = f"{n}q"
+    ptrs = struct.pack(array, *[g.data_ptr() for g in grads])
+    to = None if out is None else struct.pack(array, *[o.data_ptr() for o in outs])
     _ok(lib, lib.triposplat_b200_clip_grad_norm(
-        ptrs, to, _i64(*[g.numel() for g in grads]), (ctypes.c_int * n)(*[_DTYPES[g.dtype] for g in grads]), n,
-        max_norm, norm.data_ptr()), "clip_grad_norm")
+        ptrs, to, struct.pack(array, *[g.numel() for g in grads]),
+        struct.pack(f"{n}i", *[_DTYPES[g.dtype] for g in grads]), n, max_norm, norm.data_ptr()), "clip_grad_norm")
     return norm
