@@ -117,6 +117,10 @@ struct Params {
   // without a key is zeros instead of 0 / 0
   float2* stats;
   int64_t stats_ld;  // rows of stats per (b, h)
+  // a row's keys cut into `cuts` work items of T tiles each (the last may reach past the Tk tiles there
+  // are: those read as zeros and are masked), outputs and statistics cut_out / cut_stats apart
+  int Tk, cuts;
+  int64_t cut_out, cut_stats;
 };
 
 // 2^s for |s| <= 126 built in the exponent field: x * pow2i(s) is the correctly rounded
@@ -366,6 +370,8 @@ __device__ __forceinline__ void softmax_tile(uint32_t srow, uint32_t orow, bool 
   l_run = fmaf((s0 + s1) + (s2 + s3), ex2(-vshift), l_run);  // sum of unshifted p
 }
 
+// CUT: the keys of a row are cut into several work items (Params::cuts).
+template <bool CUT>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     sdpa_fwd_tc(const __grid_constant__ CUtensorMap tm_qhi, const __grid_constant__ CUtensorMap tm_qlo,
                 const __grid_constant__ CUtensorMap tm_khi, const __grid_constant__ CUtensorMap tm_klo,
@@ -406,10 +412,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   // persistent CTAs: work item j = blockIdx.x + i * gridDim.x (query tiles of one head
   // consecutive, so CTAs running together share the head's K / V in L2); every role walks
   // the same items, and stages / barrier phases run on the global tile counter G = i*T + t
-  const int items = p.Qt * p.BH;
+  const int items = CUT ? p.Qt * p.BH * p.cuts : p.Qt * p.BH;
+  const int Tk = CUT ? p.Tk : T;
   const int my_items = (int)blockIdx.x < items ? (items - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
-  auto item_of = [&](int i, int& bh, int& q0) {
-    const int j = blockIdx.x + i * gridDim.x;
+  // head, first query row, first key tile of work item i
+  auto item_of = [&](int i, int& bh, int& q0, int& t0) {
+    int j = blockIdx.x + i * gridDim.x;
+    t0 = 0;
+    if (CUT) {
+      const int c = j % p.cuts;
+      j /= p.cuts;
+      t0 = c * T;
+    }
     bh = j / p.Qt;
     q0 = (j - bh * p.Qt) * BQ;
   };
@@ -458,8 +472,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       int q_issued = -1;
       bool ok = true;
       for (int i = 0; i < my_items && ok; ++i) {
-        int bh, q0;
-        item_of(i, bh, q0);
+        int bh, q0, t0;
+        item_of(i, bh, q0, t0);
         if (is_k) {
           // the item's Q tile, once the previous item's QK MMAs have read the old one
           // (rows past Lq read as zeros)
@@ -478,13 +492,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           uint8_t* d = base + st * STAGE;
           mbar_arrive_expect_tx(&full[st], STAGE);
           if (is_k) {
-            tma_load_3d(d, &tm_khi, &full[st], 0, t * BKV, bh);
-            tma_load_3d(d + PLANE, &tm_klo, &full[st], 0, t * BKV, bh);
+            tma_load_3d(d, &tm_khi, &full[st], 0, (t0 + t) * BKV, bh);
+            tma_load_3d(d + PLANE, &tm_klo, &full[st], 0, (t0 + t) * BKV, bh);
           } else {
-            tma_load_3d(d, &tm_vhi, &full[st], t * BKV, 0, bh);
-            tma_load_3d(d + PLANE / 2, &tm_vhi, &full[st], t * BKV + 64, 0, bh);
-            tma_load_3d(d + PLANE, &tm_vlo, &full[st], t * BKV, 0, bh);
-            tma_load_3d(d + PLANE + PLANE / 2, &tm_vlo, &full[st], t * BKV + 64, 0, bh);
+            tma_load_3d(d, &tm_vhi, &full[st], (t0 + t) * BKV, 0, bh);
+            tma_load_3d(d + PLANE / 2, &tm_vhi, &full[st], (t0 + t) * BKV + 64, 0, bh);
+            tma_load_3d(d + PLANE, &tm_vlo, &full[st], (t0 + t) * BKV, 0, bh);
+            tma_load_3d(d + PLANE + PLANE / 2, &tm_vlo, &full[st], (t0 + t) * BKV + 64, 0, bh);
           }
           issued[st] = G;
         }
@@ -587,21 +601,21 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     constexpr int PF_V = 3;
     float pf_cq = 0.0f, pf_k0 = 0.0f, pf_v[PF_V];
     auto prefetch = [&](int i) {
-      int bh_, q0_;
-      item_of(i, bh_, q0_);
+      int bh_, q0_, t0_;
+      item_of(i, bh_, q0_, t0_);
       const int qr = q0_ + r;
       pf_cq = qr < p.Lq ? p.qinv[(int64_t)bh_ * p.Lq + qr] : 0.0f;
-      pf_k0 = team < T ? p.kinv[(int64_t)bh_ * T + team] : 0.0f;
+      pf_k0 = team < T && (!CUT || t0_ + team < Tk) ? p.kinv[(int64_t)bh_ * Tk + t0_ + team] : 0.0f;
 #pragma unroll
       for (int k = 0; k < PF_V; ++k) {
         const int t = lane + 32 * k;
-        pf_v[k] = t < T ? p.vinv[(int64_t)bh_ * T + t] : 0.0f;
+        pf_v[k] = t < Tk ? p.vinv[(int64_t)bh_ * Tk + t] : 0.0f;
       }
     };
     if (my_items > 0) prefetch(0);
     for (int i = 0; i < my_items && ok; ++i) {
-    int bh, q0;
-    item_of(i, bh, q0);
+    int bh, q0, t0;
+    item_of(i, bh, q0, t0);
     const int qrow = q0 + r;
     const bool row_valid = qrow < p.Lq;
     const float cq = 0.125f * LOG2E * pf_cq;
@@ -611,11 +625,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     float vref = pf_v[0];
 #pragma unroll
     for (int k = 1; k < PF_V; ++k) vref = fmaxf(vref, pf_v[k]);
-    for (int t = lane + 32 * PF_V; t < T; t += 32) vref = fmaxf(vref, p.vinv[(int64_t)bh * T + t]);
+    for (int t = lane + 32 * PF_V; t < Tk; t += 32) vref = fmaxf(vref, p.vinv[(int64_t)bh * Tk + t]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) vref = fmaxf(vref, __shfl_xor_sync(0xffffffffu, vref, o));
     // the team's first tile's K and V scales (tile `team`: lane `team`'s first share)
-    const float k0_cur = pf_k0, v0_cur = __shfl_sync(0xffffffffu, pf_v[0], team);
+    const float k0_cur = pf_k0;
+    float v0_cur = __shfl_sync(0xffffffffu, pf_v[0], team);
+    if (CUT) v0_cur = t0 + team < Tk ? p.vinv[(int64_t)bh * Tk + t0 + team] : vref;
     // the next item's scales are requested after this item's first tile: right here the
     // previous item's output stores still fill the load / store queue
     bool pf_next = i + 1 < my_items;
@@ -627,22 +643,23 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     int n = 0;  // tiles this team has processed in this item
     for (int t = team; t < T; t += 2, ++n) {
       const int G = i * T + t, sb = G % NSB;
-      const bool plain = bias_row == nullptr && (t + 1) * BKV <= p.Lk;  // no bias, no masking
+      const bool plain = bias_row == nullptr && (t0 + t + 1) * BKV <= p.Lk;  // no bias, no masking
       if (!plain) {
         // key bias (+ -inf past Lk) for this tile, staged in a warp-private buffer
         __syncwarp();
 #pragma unroll
         for (int ii = 0; ii < BKV / 32; ++ii) {
           const int jl = ii * 32 + lane;
-          const int j = t * BKV + jl;
+          const int j = (t0 + t) * BKV + jl;
           bt[jl] = j < p.Lk ? (bias_row ? bias_row[j] * LOG2E : 0.0f) : -INFINITY;
         }
         __syncwarp();
       }
-      const float c2 = cq * (n == 0 ? k0_cur : p.kinv[(int64_t)bh * T + t]);
+      const int tk = CUT ? min(t0 + t, Tk - 1) : t;  // tiles past the last one are masked: any scale serves
+      const float c2 = cq * (n == 0 ? k0_cur : p.kinv[(int64_t)bh * Tk + tk]);
       // exponent offset folding this V tile's pre-scale relative to the head reference
       const float vshift =
-          (float)((__float_as_int(n == 0 ? v0_cur : p.vinv[(int64_t)bh * T + t]) >> 23) - vref_exp);
+          (float)((__float_as_int(n == 0 ? v0_cur : p.vinv[(int64_t)bh * Tk + tk]) >> 23) - vref_exp);
       ok = mbar_wait(&s_full[sb], (G / NSB) & 1, p.status, kDevTimeoutConsumer, abort_flag);
       // this team's previous O, P.V(G-2), retired long ago; it is folded in with the scores
       if (ok && n > 0) {
@@ -670,8 +687,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     // the wait for the last P.V; the 8 shares meet in the exchange)
     float vb_part = 0.0f;
     if (p.ohi) {
-      const float* vb = p.vinv + (int64_t)(bh / p.H) * p.H * T;
-      const int cnt = p.H * T;
+      const float* vb = p.vinv + (int64_t)(bh / p.H) * p.H * Tk;
+      const int cnt = p.H * Tk;
 #pragma unroll 4
       for (int e = (warp - 4) * 32 + lane; e < cnt; e += 256) vb_part = fmaxf(vb_part, vb[e]);
     }
@@ -730,7 +747,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         float f = vref / l;
         if (p.stats) {
           if (l == 0.0f) f = 0.0f;
-          p.stats[bh * p.stats_ld + qrow] = make_float2(m, l * 0x1p-7f);  // the lift of P_LIFT taken out
+          p.stats[(CUT ? t0 / T * p.cut_stats : 0) + bh * p.stats_ld + qrow] = make_float2(m, l * 0x1p-7f);  // the lift of P_LIFT taken out
         }
         // dimensions 0..31 as team 0's own (o0 f0 + o1 f1), 32..63 as team 1's own
 #pragma unroll
@@ -781,8 +798,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             *reinterpret_cast<uint2*>(p.olo + off) =
                 make_uint2(*reinterpret_cast<const uint32_t*>(&l01), *reinterpret_cast<const uint32_t*>(&l23));
           } else {
-            float* dst = p.out_blhd ? p.out + (((int64_t)b * p.Lq + qr) * p.H + hh) * D + c
-                                    : p.out + ((int64_t)bh * p.Lq + qr) * D + c;
+            float* base = CUT ? p.out + t0 / T * p.cut_out : p.out;
+            float* dst = p.out_blhd ? base + (((int64_t)b * p.Lq + qr) * p.H + hh) * D + c
+                                    : base + ((int64_t)bh * p.Lq + qr) * D + c;
             *reinterpret_cast<float4*>(dst) = v;
           }
         }
@@ -1324,7 +1342,8 @@ static OutSplit out_split_of(void* out_split, int64_t B, int Lq, int H) {
 static int sdpa_attend(const SplitPlanesSdpa& sp, const float* bias, int64_t bias_bh_stride,
                        float* out, int64_t BH, int H, int Lq, int Lk, int out_blhd,
                        cudaStream_t stream, const OutSplit& osplit = OutSplit(),
-                       float2* stats = nullptr, int64_t stats_ld = 0) {
+                       float2* stats = nullptr, int64_t stats_ld = 0, int cuts = 1, int64_t cut_out = 0,
+                       int64_t cut_stats = 0) {
   using namespace sdpa;
   CUtensorMap m_qhi, m_qlo, m_khi, m_klo, m_vhi, m_vlo;
   const uint32_t box_rows[3] = {64, 128, 1};
@@ -1360,19 +1379,23 @@ static int sdpa_attend(const SplitPlanesSdpa& sp, const float* bias, int64_t bia
       // compiled with REGS_LAUNCH registers per thread; with fewer, an increase would wait
       // for ever, so refuse to launch instead
       cudaFuncAttributes fa{};
-      if (cudaFuncGetAttributes(&fa, sdpa_fwd_tc) != cudaSuccess || fa.numRegs < (int)REGS_LAUNCH) {
-        set_last_error("sdpa_fwd_tc was compiled with fewer registers than its warpgroup budget needs");
-        return kLaunchFailed;
+      for (auto* kernel : {sdpa_fwd_tc<false>, sdpa_fwd_tc<true>}) {
+        if (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess || fa.numRegs < (int)REGS_LAUNCH) {
+          set_last_error("sdpa_fwd_tc was compiled with fewer registers than its warpgroup budget needs");
+          return kLaunchFailed;
+        }
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
       }
-      cudaFuncSetAttribute(sdpa_fwd_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
       cudaFuncSetAttribute(qkv_split_k<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, QKV_SPLIT_SMEM);
       cudaFuncSetAttribute(qkv_split_k<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, QKV_SPLIT_SMEM);
       attr_done.fetch_or(1ull << (dev & 63), std::memory_order_acq_rel);
     }
   }
   const int Qt = (Lq + BQ - 1) / BQ;
-  Params prm{sp.qinv, sp.kinv, sp.vinv, bias, (long long)bias_bh_stride, out, H, Lq, Lk, sp.T, out_blhd,
-             device_status(), Qt, (int)BH, osplit.hi, osplit.lo, osplit.rs, stats, stats_ld};
+  Params prm{sp.qinv, sp.kinv, sp.vinv, bias, (long long)bias_bh_stride, out, H, Lq, Lk,
+             (sp.T + cuts - 1) / cuts, out_blhd,
+             device_status(), Qt, (int)BH, osplit.hi, osplit.lo, osplit.rs, stats, stats_ld, sp.T, cuts,
+             cut_out, cut_stats};
   // persistent: one CTA per SM walking the (head, query tile) items
   static std::atomic<int> sm_count[64];
   int dev = 0;
@@ -1384,18 +1407,21 @@ static int sdpa_attend(const SplitPlanesSdpa& sp, const float* bias, int64_t bia
     sms = n > 0 ? n : 148;
     sm_count[dev & 63].store(sms, std::memory_order_release);
   }
-  const long long items = (long long)Qt * BH;
+  const long long items = (long long)Qt * BH * cuts;
   const dim3 grid((unsigned)(items < sms ? items : sms));
   {
     LaunchScope scope(kKSdpaAttn, stream);
-    sdpa_fwd_tc<<<grid, NUM_THREADS, SMEM_BYTES, stream>>>(m_qhi, m_qlo, m_khi, m_klo, m_vhi, m_vlo, prm);
+    if (cuts > 1) sdpa_fwd_tc<true><<<grid, NUM_THREADS, SMEM_BYTES, stream>>>(m_qhi, m_qlo, m_khi, m_klo, m_vhi, m_vlo, prm);
+    else sdpa_fwd_tc<false><<<grid, NUM_THREADS, SMEM_BYTES, stream>>>(m_qhi, m_qlo, m_khi, m_klo, m_vhi, m_vlo, prm);
   }
   return launch_status();
 }
 
 int sdpa_attend_stats(const SplitPlanesSdpa& sp, const float* bias, int64_t bias_bh_stride, float* out_blhd,
-                      float2* stats, int64_t stats_ld, int64_t BH, int H, int Lq, int Lk, cudaStream_t stream) {
-  return sdpa_attend(sp, bias, bias_bh_stride, out_blhd, BH, H, Lq, Lk, 1, stream, OutSplit(), stats, stats_ld);
+                      float2* stats, int64_t stats_ld, int64_t BH, int H, int Lq, int Lk, int cuts, int64_t cut_out,
+                      int64_t cut_stats, cudaStream_t stream) {
+  return sdpa_attend(sp, bias, bias_bh_stride, out_blhd, BH, H, Lq, Lk, 1, stream, OutSplit(), stats, stats_ld, cuts,
+                     cut_out, cut_stats);
 }
 
 // k/v element (bh, j, d) at base + bh*bh_stride + j*j_stride + d*d_stride

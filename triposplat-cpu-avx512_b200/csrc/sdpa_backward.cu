@@ -631,7 +631,8 @@ struct Bias {
 };
 
 // One block per (b, h): the row's largest bias, where it leaves the scores weight (head = 0 beyond
-// 2^60 in magnitude), both behind the statistics for the backward pass, and the relative bias.
+// 2^60 in magnitude), both behind the statistics for the backward pass, and (out not null) the
+// relative bias.
 __global__ void __launch_bounds__(256) bias_rows_k(Bias bias, int H, float* __restrict__ out, float2* head, int64_t head_stride) {
   __shared__ float sm[8];
   const int bh = blockIdx.x, b = bh / H, h = bh - b * H;
@@ -645,7 +646,8 @@ __global__ void __launch_bounds__(256) bias_rows_k(Bias bias, int H, float* __re
 #pragma unroll
   for (int k = 0; k < 8; ++k) mx = fmaxf(mx, sm[k]);
   if (threadIdx.x == 0) head[bh * head_stride] = make_float2(mx, mx > -INFINITY && fabsf(mx) > 0x1p60f ? 0.0f : 1.0f);
-  for (int j = threadIdx.x; j < bias.L; j += 256) out[(int64_t)bh * bias.L + j] = relative_bias(src[j], mx);
+  if (out)
+    for (int j = threadIdx.x; j < bias.L; j += 256) out[(int64_t)bh * bias.L + j] = relative_bias(src[j], mx);
 }
 
 struct Rows {
@@ -884,6 +886,38 @@ __global__ void __launch_bounds__(256) join_k(const float* __restrict__ part, in
   out[b * sb + h * sh + row * sl + d] = s;
 }
 
+// Shares of the keys joined: partial outputs [cuts, BH or B, Lq, ...] as normalised by their own sums,
+// with their statistics.  A warp per row; the shares in their order.  last: the statistics' last row
+// has no bias kernel to set it.
+__global__ void __launch_bounds__(256) attn_join_k(const float* __restrict__ o, const float2* __restrict__ st, int cuts,
+                                                   int64_t cut_o, int64_t cut_st, int64_t st_ld, int by_head, int BH, int H,
+                                                   int Lq, int last, float* __restrict__ out, float2* __restrict__ stats) {
+  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (i >= (int64_t)BH * Lq) return;
+  const int bh = (int)(i / Lq), row = (int)(i - (int64_t)bh * Lq), b = bh / H, h = bh - b * H;
+  const int64_t dst = (((int64_t)b * Lq + row) * H + h) * D + lane * 2;
+  const float* src = o + (by_head ? i * D + lane * 2 : dst);
+  const float2* s = st + bh * st_ld + row;
+  float m = -INFINITY;
+  for (int c = 0; c < cuts; ++c) m = fmaxf(m, s[c * cut_st].x);
+  float l = 0.0f;
+  float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+  for (int c = 0; c < cuts; ++c) {
+    const float2 ml = s[c * cut_st];
+    const float w = ml.y * (ml.x == m ? 1.0f : ex2(ml.x - m));
+    const float2 x = *reinterpret_cast<const float2*>(src + c * cut_o);
+    l += w;
+    v.x = fmaf(w, x.x, v.x);
+    v.y = fmaf(w, x.y, v.y);
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  *reinterpret_cast<float2*>(out + dst) = make_float2(v.x * inv, v.y * inv);
+  if (lane == 0) stats[(int64_t)bh * (Lq + 1) + row] = make_float2(m, l);
+  if (last && row == 0 && lane == 1) stats[(int64_t)bh * (Lq + 1) + Lq] = make_float2(0.0f, 1.0f);
+}
+
 // db [bias_b, bias_h, Lk]: part [parts, B, H, Lt] added over the parts and the batch entries and heads
 // that share a row, in their order.
 __global__ void __launch_bounds__(256) bias_grad_k(const float* __restrict__ part, int parts, int B, int H, int bias_b,
@@ -1002,6 +1036,8 @@ static bool rows16(std::initializer_list<const void*> ps, const int64_t* strides
   return true;
 }
 
+#include "sdpa_few.cuh"
+
 static Rows rows_of(const void* p, const int64_t* s) { return {static_cast<const float*>(p), s[0], s[1], s[2]}; }
 
 }  // namespace sdpab
@@ -1024,25 +1060,66 @@ int triposplat_b200_attention_forward(const float* q, const float* k, const floa
     if (p && !is_device_pointer(p)) return kNotDevicePointer;
   cudaStream_t stream = current_stream();
   const int64_t BH = (int64_t)B * H;
-  SplitPlanesSdpa sp;
-  void* behind = nullptr;
-  st = sdpa_planes_extra(BH, Lq, Lk, key_bias ? al256((size_t)BH * Lk * 4) : 0, stream, sp, &behind);
-  if (st != kOk) return st;
-  float* relative = key_bias ? static_cast<float*>(behind) : nullptr;
   float2* rows = reinterpret_cast<float2*>(stats);
   const Bias bias{key_bias, bias_batches, bias_heads, Lk};
-  if (key_bias) {
+  const int vec = rows16({q, k, v}, strides, 3);
+  auto bias_rows = [&](float* relative) {
     LaunchScope scope(kKSdpaSplit, stream);
     bias_rows_k<<<(unsigned)BH, 256, 0, stream>>>(bias, H, relative, rows + Lq, Lq + 1);
+  };
+  auto join = [&](const float* o, const float2* part, int cuts, int64_t cut_o, int64_t cut_st, int64_t st_ld, int by_head,
+                  int last) {
+    LaunchScope scope(kKSdpaSplit, stream);
+    attn_join_k<<<(unsigned)((BH * Lq + 7) / 8), 256, 0, stream>>>(o, part, cuts, cut_o, cut_st, st_ld, by_head, (int)BH, H,
+                                                                 Lq, last, out_blhd, rows);
+  };
+  if (Lq <= kFewRows) {
+    FewArgs a{};
+    a.q = rows_of(q, strides); a.k = rows_of(k, strides + 3); a.v = rows_of(v, strides + 6);
+    a.bias = bias;
+    a.head = rows + Lq; a.head_stride = Lq + 1;
+    a.o = out_blhd; a.stats_out = rows;
+    a.H = H; a.BH = (int)BH; a.Lq = Lq; a.Lk = Lk; a.vec = vec;
+    few_shares(a);
+    if (a.shares > 1) {
+      const size_t obytes = al256((size_t)a.shares * BH * Lq * D * 4);
+      uint8_t* ws = static_cast<uint8_t*>(workspace(obytes + (size_t)a.shares * BH * Lq * 8, stream));
+      if (!ws) return kWorkspace;
+      a.o = reinterpret_cast<float*>(ws);
+      a.stats_out = reinterpret_cast<float2*>(ws + obytes);
+    }
+    if (key_bias) bias_rows(nullptr);
+    few_fwd(a, stream);
+    if (a.shares > 1) join(a.o, a.stats_out, a.shares, BH * Lq * D, BH * Lq, Lq, 1, key_bias == nullptr);
+    return launch_status();
   }
+  // few work items: the keys in shares of two tiles or more, so that most SMs have one
+  const int Qt = (Lq + KT - 1) / KT, T = (Lk + KT - 1) / KT;
+  const int64_t fit = sm_count() / (Qt * BH);
+  const int cuts = fit < 2 || T < 4 ? 1 : (int)(fit < T / 2 ? fit : T / 2);
+  const size_t bias_bytes = key_bias ? al256((size_t)BH * Lk * 4) : 0;
+  const size_t part_bytes = cuts > 1 ? al256((size_t)cuts * BH * Lq * D * 4) : 0;
+  SplitPlanesSdpa sp;
+  void* behind = nullptr;
+  st = sdpa_planes_extra(BH, Lq, Lk, bias_bytes + part_bytes + (cuts > 1 ? (size_t)cuts * BH * Lq * 8 : 0), stream, sp,
+                         &behind);
+  if (st != kOk) return st;
+  float* relative = key_bias ? static_cast<float*>(behind) : nullptr;
+  float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(behind) + bias_bytes);
+  float2* part_st = reinterpret_cast<float2*>(static_cast<uint8_t*>(behind) + bias_bytes + part_bytes);
+  if (key_bias) bias_rows(relative);
   {
     LaunchScope scope(kKSdpaSplit, stream);
-    fwd_split_k<<<dim3((unsigned)BH, sp.T + (Lq + KT - 1) / KT), 256, 0, stream>>>(
-        rows_of(q, strides), rows_of(k, strides + 3), rows_of(v, strides + 6), bias, rows + Lq, Lq + 1, H, Lq, Lk,
-        rows16({q, k, v}, strides, 3), sp);
+    fwd_split_k<<<dim3((unsigned)BH, sp.T + Qt), 256, 0, stream>>>(rows_of(q, strides), rows_of(k, strides + 3),
+                                                                rows_of(v, strides + 6), bias, rows + Lq, Lq + 1, H, Lq,
+                                                                Lk, vec, sp);
   }
   if ((st = launch_status()) != kOk) return st;
-  return sdpa_attend_stats(sp, relative, Lk, out_blhd, rows, Lq + 1, BH, H, Lq, Lk, stream);
+  if (cuts == 1) return sdpa_attend_stats(sp, relative, Lk, out_blhd, rows, Lq + 1, BH, H, Lq, Lk, 1, 0, 0, stream);
+  st = sdpa_attend_stats(sp, relative, Lk, part, part_st, Lq, BH, H, Lq, Lk, cuts, BH * Lq * D, BH * Lq, stream);
+  if (st != kOk) return st;
+  join(part, part_st, cuts, BH * Lq * D, BH * Lq, Lq, 0, 0);
+  return launch_status();
 }
 
 int triposplat_b200_attention_backward(const float* dout, const float* q, const float* k, const float* v,
@@ -1061,10 +1138,44 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
   for (const float* p : {dout, q, k, v, out, stats, key_bias, static_cast<const float*>(dq), static_cast<const float*>(dk),
                          static_cast<const float*>(dv), static_cast<const float*>(dbias)})
     if (p && !is_device_pointer(p)) return kNotDevicePointer;
-  st = key_bias ? ensure_kernel<true>() : ensure_kernel<false>();
-  if (st != kOk) return st;
   cudaStream_t stream = current_stream();
   const int64_t BH = (int64_t)B * H;
+  const int64_t* go = strides + 15;  // dq, dk, dv
+  const int vec = rows16({dout, q, k, v, out}, strides, 5), vec_out = rows16({dq, dk, dv}, go, 3);
+  const float2* rows = reinterpret_cast<const float2*>(stats);
+  const Bias bias{key_bias, bias_batches, bias_heads, Lk};
+  auto join = [&](const float* part, int cuts, int L, int Lt, float* dst, const int64_t* g) {
+    LaunchScope scope(kKSdpaSplit, stream);
+    join_k<<<(unsigned)((BH * L * D + 255) / 256), 256, 0, stream>>>(part, cuts, H, (int)BH, L, Lt, dst, g[0], g[1], g[2]);
+  };
+  auto bias_grad = [&](const float* part, int parts, int Lt) {
+    LaunchScope scope(kKSdpaSplit, stream);
+    bias_grad_k<<<dim3((Lk + 255) / 256, bias_batches * bias_heads), 256, 0, stream>>>(part, parts, B, H, bias_batches,
+                                                                                     bias_heads, Lk, Lt, dbias);
+  };
+  if (Lq <= kFewRows) {
+    FewArgs a{};
+    a.dout = rows_of(dout, strides); a.q = rows_of(q, strides + 3); a.k = rows_of(k, strides + 6);
+    a.v = rows_of(v, strides + 9); a.out = rows_of(out, strides + 12);
+    a.bias = bias;
+    a.head = rows + Lq; a.head_stride = Lq + 1;
+    a.stats = rows;
+    a.dk = dk; a.kb = go[3]; a.kh = go[4]; a.kl = go[5];
+    a.dv = dv; a.vb = go[6]; a.vh = go[7]; a.vl = go[8];
+    a.H = H; a.BH = (int)BH; a.Lq = Lq; a.Lk = Lk; a.vec = vec; a.vec_out = vec_out;
+    few_shares(a);
+    const size_t qbytes = al256((size_t)a.shares * BH * Lq * D * 4);
+    uint8_t* ws = static_cast<uint8_t*>(workspace(qbytes + (dbias ? (size_t)BH * Lk * 4 : 0), stream));
+    if (!ws) return kWorkspace;
+    a.dq = reinterpret_cast<float*>(ws);
+    a.db = dbias ? reinterpret_cast<float*>(ws + qbytes) : nullptr;
+    few_bwd(a, stream);
+    join(a.dq, a.shares, Lq, Lq, dq, go);
+    if (dbias) bias_grad(a.db, 1, Lk);
+    return launch_status();
+  }
+  st = key_bias ? ensure_kernel<true>() : ensure_kernel<false>();
+  if (st != kOk) return st;
   Params p{};
   Side qs{}, ks{};
   const size_t qbytes = side_layout(nullptr, BH, Lq, true, qs), kbytes = side_layout(nullptr, BH, Lk, false, ks);
@@ -1083,8 +1194,6 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
   side_layout(ws, BH, Lq, true, qs);
   side_layout(ws + qbytes, BH, Lk, false, ks);
   uint8_t* at = ws + qbytes + kbytes;
-  const int64_t* go = strides + 15;  // dq, dk, dv
-  const int vec_out = rows16({dq, dk, dv}, go, 3);
   p.keys.held = ks;
   p.keys.walk = qs;
   p.keys.out1 = kpart ? reinterpret_cast<float*>(at) : dk;
@@ -1098,7 +1207,7 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
   p.queries.s1b = go[0]; p.queries.s1h = go[1]; p.queries.s1l = go[2];
   p.queries.vec_out = vec_out;
   p.db = dbias ? reinterpret_cast<float*>(at + 2 * kpart + qpart) : nullptr;
-  p.head = reinterpret_cast<const float2*>(stats) + Lq;
+  p.head = rows + Lq;
   p.head_stride = Lq + 1;
   p.H = H;
   p.BH = (int)BH;
@@ -1115,8 +1224,7 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
     LaunchScope scope(kKSdpaSplit, stream);
     bwd_split_k<<<dim3((unsigned)BH, (ks.Lt + qs.Lt) / HELD), 256, 0, stream>>>(
         rows_of(q, strides + 3), rows_of(dout, strides), rows_of(out, strides + 12), rows_of(k, strides + 6),
-        rows_of(v, strides + 9), Bias{key_bias, bias_batches, bias_heads, Lk}, reinterpret_cast<const float2*>(stats),
-        Lq + 1, H, rows16({dout, q, k, v, out}, strides, 5), qs, ks);
+        rows_of(v, strides + 9), bias, rows, Lq + 1, H, vec, qs, ks);
   }
   {
     LaunchScope scope(kKSdpaAttn, stream);
@@ -1124,21 +1232,12 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
     if (key_bias) sdpa_bwd_tc<true><<<grid, kThreads, SMEM_BYTES, stream>>>(m, p);
     else sdpa_bwd_tc<false><<<grid, kThreads, SMEM_BYTES, stream>>>(m, p);
   }
-  auto join = [&](const Pass& s, const float* part, float* dst, const int64_t* g) {
-    LaunchScope scope(kKSdpaSplit, stream);
-    join_k<<<(unsigned)((BH * s.held.L * D + 255) / 256), 256, 0, stream>>>(part, s.cuts, H, (int)BH, s.held.L, s.held.Lt,
-                                                                          dst, g[0], g[1], g[2]);
-  };
-  if (qpart) join(p.queries, p.queries.out1, dq, go);
+  if (qpart) join(p.queries.out1, p.queries.cuts, Lq, qs.Lt, dq, go);
   if (kpart) {
-    join(p.keys, p.keys.out1, dk, go + 3);
-    join(p.keys, p.keys.out2, dv, go + 6);
+    join(p.keys.out1, p.keys.cuts, Lk, ks.Lt, dk, go + 3);
+    join(p.keys.out2, p.keys.cuts, Lk, ks.Lt, dv, go + 6);
   }
-  if (dbias) {
-    LaunchScope scope(kKSdpaSplit, stream);
-    bias_grad_k<<<dim3((Lk + 255) / 256, bias_batches * bias_heads), 256, 0, stream>>>(
-        p.db, 2 * p.keys.cuts, B, H, bias_batches, bias_heads, Lk, ks.Lt, dbias);
-  }
+  if (dbias) bias_grad(p.db, 2 * p.keys.cuts, ks.Lt);
   return launch_status();
 }
 

@@ -1,0 +1,273 @@
+// Attention of up to four query rows per head (a pooled token, a decoded one), forward and backward,
+// in fp32 on the CUDA cores.  With so few rows the work is reading K and V once (and, backward, writing
+// their gradients): the tensor-core path would first write both as fp16 pairs and read those back,
+// and walk them with one held tile per head.
+//
+// Four lanes per key, 16 of its 64 dimensions each; a score is 16 products per lane and two shuffles.
+// A block takes a share of a head's keys, eight warps of eight keys at a time.  Forward: each group
+// of four lanes keeps a softmax of its own (integer reference m in log2 units, raised when a score
+// passes it by more than 8, so that its factor is a power of two; l; 16 output values per row),
+// joined over the warp by shuffles, over the block in shared memory, and over the shares of the keys by
+// a last kernel in their order.  Backward: per key e and ds of every row give its dK, dV at once, dQ is
+// kept in registers and joined the same way.
+//
+// Included by sdpa_backward.cu, whose Rows, Bias and helpers it uses.
+
+constexpr int kFewRows = 4;
+constexpr int kFewThreads = 256;
+
+struct FewArgs {
+  Rows q, k, v, out, dout;
+  Bias bias;               // .p null: none
+  const float2* head;      // [BH] head_stride apart: (largest bias, weight of the scores); only with a bias
+  int64_t head_stride;
+  const float2* stats;     // backward: [BH, Lq + 1]
+  float *o, *dk, *dv;      // forward: [B, Lq, H, 64] or partial [shares, BH, Lq, 64]; backward: with strides
+  float2* stats_out;       // forward: [BH, Lq + 1] or partial [shares, BH, Lq]
+  float* dq;               // partial [shares, BH, Lq, 64]
+  float* db;               // nullable: [BH, Lk]
+  int64_t kb, kh, kl, vb, vh, vl;  // strides of dk, dv
+  int H, BH, Lq, Lk, vec, vec_out, shares, span;
+};
+
+// sum over the lanes of a warp that hold the same dimensions (lane mod 4)
+__device__ __forceinline__ float sum_groups(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// sum over the four lanes of a key
+__device__ __forceinline__ float sum_key(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+
+template <int NQ>
+__global__ void __launch_bounds__(kFewThreads) few_fwd_k(const FewArgs a) {
+  __shared__ float qs[NQ][D];
+  __shared__ float sm_m[kFewThreads / 32][NQ], sm_l[kFewThreads / 32][NQ], sm_o[kFewThreads / 32][NQ][D];
+  const int bh = blockIdx.y, b = bh / a.H, h = bh - b * a.H;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = (lane & 3) * 16;
+  float2 head = make_float2(0.0f, 1.0f);
+  if (a.bias.p) head = a.head[bh * a.head_stride];
+  for (int i = threadIdx.x; i < NQ * D; i += kFewThreads) {
+    const int r = i / D, d = i - r * D;
+    qs[r][d] = r < a.Lq && head.y != 0.0f ? a.q.at(b, h, r)[d] * (0.125f * LOG2E) : 0.0f;
+  }
+  __syncthreads();
+  float m[NQ], l[NQ], o[NQ][16];
+#pragma unroll
+  for (int r = 0; r < NQ; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[r][e] = 0.0f;
+  }
+  const int j1 = min(a.Lk, (int)(blockIdx.x + 1) * a.span);
+#pragma unroll 1
+  for (int jb = blockIdx.x * a.span + warp * 8; jb < j1; jb += kFewThreads / 4) {  // uniform over the warp
+    const int j = jb + (lane >> 2);
+    float off = -INFINITY, kv[16], vv[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) kv[e] = vv[e] = 0.0f;
+    if (j < j1) off = a.bias.p ? relative_bias(a.bias.row(b, h)[j], head.x) * LOG2E : 0.0f;
+    if (off != -INFINITY) {
+      load16(a.k.at(b, h, j) + c0, a.vec, kv);
+      load16(a.v.at(b, h, j) + c0, a.vec, vv);
+    }
+#pragma unroll
+    for (int r = 0; r < NQ; ++r) {
+      float s = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s = fmaf(qs[r][c0 + e], kv[e], s);
+      s = sum_key(s) + off;
+      if (s > m[r] + 8.0f) {  // the same in the key's four lanes
+        const float up = ceilf(s), f = ex2(m[r] - up);  // 0 from -inf
+        m[r] = up;
+        l[r] *= f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[r][e] *= f;
+      }
+      // a missing key gives 0, also while m is -inf; NaN stays
+      const float w = s == -INFINITY ? 0.0f : ex2(s - m[r]);
+      l[r] += w;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[r][e] = fmaf(w, vv[e], o[r][e]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < NQ; ++r) {
+    float top = m[r];
+#pragma unroll
+    for (int i = 4; i < 32; i <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+    const float f = m[r] == top ? 1.0f : ex2(m[r] - top);
+    const float ls = sum_groups(l[r] * f);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float v = sum_groups(o[r][e] * f);
+      if (lane < 4) sm_o[warp][r][c0 + e] = v;
+    }
+    if (lane == 0) {
+      sm_m[warp][r] = top;
+      sm_l[warp][r] = ls;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < NQ * D; i += kFewThreads) {
+    const int r = i / D, d = i - r * D;
+    if (r >= a.Lq) continue;
+    float top = -INFINITY, ls = 0.0f, os = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kFewThreads / 32; ++w) top = fmaxf(top, sm_m[w][r]);
+#pragma unroll
+    for (int w = 0; w < kFewThreads / 32; ++w) {
+      const float f = sm_m[w][r] == top ? 1.0f : ex2(sm_m[w][r] - top);
+      ls = fmaf(sm_l[w][r], f, ls);
+      os = fmaf(sm_o[w][r][d], f, os);
+    }
+    os = ls == 0.0f ? 0.0f : os / ls;
+    if (a.shares > 1) {
+      const int64_t row = ((int64_t)blockIdx.x * a.BH + bh) * a.Lq + r;
+      a.o[row * D + d] = os;
+      if (d == 0) a.stats_out[row] = make_float2(top, ls);
+    } else {
+      a.o[(((int64_t)b * a.Lq + r) * a.H + h) * D + d] = os;
+      if (d == 0) a.stats_out[(int64_t)bh * (a.Lq + 1) + r] = make_float2(top, ls);
+    }
+  }
+  if (!a.bias.p && blockIdx.x == 0 && threadIdx.x == 0 && a.shares == 1)
+    a.stats_out[(int64_t)bh * (a.Lq + 1) + a.Lq] = make_float2(0.0f, 1.0f);
+}
+
+template <int NQ>
+__global__ void __launch_bounds__(kFewThreads) few_bwd_k(const FewArgs a) {
+  __shared__ float qs[NQ][D], gs[NQ][D], sm_m[NQ], sm_d[NQ];
+  __shared__ float sm_q[kFewThreads / 32][NQ][D];
+  const int bh = blockIdx.y, b = bh / a.H, h = bh - b * a.H;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = (lane & 3) * 16;
+  const float2 head = a.bias.p ? a.head[bh * a.head_stride] : make_float2(0.0f, 1.0f);
+  const float c = 0.125f * LOG2E * head.y;
+  if (warp < NQ) {  // a warp per row: q, g = dO / l, delta = g . O, m
+    const int r = warp;
+    float delta = 0.0f, m = INFINITY;
+    float q[2] = {0.0f, 0.0f}, g[2] = {0.0f, 0.0f};
+    if (r < a.Lq) {
+      const float2 ml = a.stats[(int64_t)bh * (a.Lq + 1) + r];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        q[u] = a.q.at(b, h, r)[lane + 32 * u];
+        if (ml.y != 0.0f) {
+          g[u] = a.dout.at(b, h, r)[lane + 32 * u] / ml.y;
+          delta = fmaf(g[u], a.out.at(b, h, r)[lane + 32 * u], delta);
+        }
+      }
+      if (ml.y != 0.0f) m = ml.x;  // else +inf: e = 0 throughout
+    }
+    delta = warp_sum(delta);
+    qs[r][lane] = q[0]; qs[r][lane + 32] = q[1];
+    gs[r][lane] = g[0]; gs[r][lane + 32] = g[1];
+    if (lane == 0) {
+      sm_m[r] = m;
+      sm_d[r] = delta;
+    }
+  }
+  __syncthreads();
+  float dq[NQ][16];
+#pragma unroll
+  for (int r = 0; r < NQ; ++r)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dq[r][e] = 0.0f;
+  const int j1 = min(a.Lk, (int)(blockIdx.x + 1) * a.span);
+#pragma unroll 1
+  for (int jb = blockIdx.x * a.span + warp * 8; jb < j1; jb += kFewThreads / 4) {
+    const int j = jb + (lane >> 2);
+    float off = -INFINITY, kv[16], vv[16], dk[16], dv[16], db = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) kv[e] = vv[e] = dk[e] = dv[e] = 0.0f;
+    if (j < j1) off = a.bias.p ? relative_bias(a.bias.row(b, h)[j], head.x) * LOG2E : 0.0f;
+    if (off != -INFINITY) {
+      load16(a.k.at(b, h, j) + c0, a.vec, kv);
+      load16(a.v.at(b, h, j) + c0, a.vec, vv);
+    }
+#pragma unroll
+    for (int r = 0; r < NQ; ++r) {
+      float s = 0.0f, dp = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s = fmaf(qs[r][c0 + e], kv[e], s);
+        dp = fmaf(gs[r][c0 + e], vv[e], dp);
+      }
+      s = sum_key(s);
+      dp = sum_key(dp);
+      const float w = ex2(fmaf(s, c, off - sm_m[r])), ds = w * (dp - sm_d[r]);
+      db += ds;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        dk[e] = fmaf(ds, qs[r][c0 + e], dk[e]);
+        dv[e] = fmaf(w, gs[r][c0 + e], dv[e]);
+        dq[r][e] = fmaf(ds, kv[e], dq[r][e]);
+      }
+    }
+    if (j < j1) {
+      float* pk = a.dk + b * a.kb + h * a.kh + j * a.kl + c0;
+      float* pv = a.dv + b * a.vb + h * a.vh + j * a.vl + c0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dk[e] *= 0.125f;
+      if (a.vec_out) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          *reinterpret_cast<float4*>(pk + e) = make_float4(dk[e], dk[e + 1], dk[e + 2], dk[e + 3]);
+          *reinterpret_cast<float4*>(pv + e) = make_float4(dv[e], dv[e + 1], dv[e + 2], dv[e + 3]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          pk[e] = dk[e];
+          pv[e] = dv[e];
+        }
+      }
+      if (a.db && (lane & 3) == 0) a.db[(int64_t)bh * a.Lk + j] = db;
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < NQ; ++r)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float v = sum_groups(dq[r][e]);
+      if (lane < 4) sm_q[warp][r][c0 + e] = v;
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < NQ * D; i += kFewThreads) {
+    const int r = i / D, d = i - r * D;
+    if (r >= a.Lq) continue;
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kFewThreads / 32; ++w) s += sm_q[w][r][d];
+    a.dq[(((int64_t)blockIdx.x * a.BH + bh) * a.Lq + r) * D + d] = s * 0.125f;
+  }
+}
+
+// Keys per block so that the GPU has some four blocks per SM, a multiple of the 64 that a block takes
+// at a time.
+static void few_shares(FewArgs& a) {
+  const int64_t want = ((int64_t)sm_count() * 4 + a.BH - 1) / a.BH;
+  const int64_t span = (a.Lk + want - 1) / want;
+  a.span = (int)((span + 63) / 64 * 64);
+  a.shares = (a.Lk + a.span - 1) / a.span;
+}
+
+static void few_fwd(const FewArgs& a, cudaStream_t stream) {
+  LaunchScope scope(kKSdpaAttn, stream);
+  const dim3 grid(a.shares, a.BH);
+  if (a.Lq == 1) few_fwd_k<1><<<grid, kFewThreads, 0, stream>>>(a);
+  else if (a.Lq == 2) few_fwd_k<2><<<grid, kFewThreads, 0, stream>>>(a);
+  else few_fwd_k<4><<<grid, kFewThreads, 0, stream>>>(a);
+}
+
+static void few_bwd(const FewArgs& a, cudaStream_t stream) {
+  LaunchScope scope(kKSdpaAttn, stream);
+  const dim3 grid(a.shares, a.BH);
+  if (a.Lq == 1) few_bwd_k<1><<<grid, kFewThreads, 0, stream>>>(a);
+  else if (a.Lq == 2) few_bwd_k<2><<<grid, kFewThreads, 0, stream>>>(a);
+  else few_bwd_k<4><<<grid, kFewThreads, 0, stream>>>(a);
+}
