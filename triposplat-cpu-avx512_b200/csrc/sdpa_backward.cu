@@ -213,6 +213,8 @@ struct Params {
   float* db;           // nullable: [cuts, 2, BH, Lt of the keys] sums of ds over each warpgroup's queries
   int H, BH;
   int key_items, items;
+  int keys_last;       // the queries' items come first (the longer ones do)
+  int* next;           // items handed out beyond the first of each CTA
   int* status;
 };
 
@@ -220,16 +222,19 @@ struct Maps {
   CUtensorMap q1h, q1l, q2h, q2l, k1h, k1l, k2h, k2l;
 };
 
-// Work item j: keys' items first; shares of a walk next to each other, then held tiles, then heads.
+// Work item j: the pass with the longer items first; shares of a walk next to each other, then held tiles,
+// then heads.  A CTA starts with item blockIdx.x and then takes the next one that is left, so that
+// items of different lengths fill the SMs evenly; which CTA works on an item changes no result.
 struct Item {
   bool keys;
   int bh, f0, t0, n, cut;  // head, first held row, walked tiles [t0, t0 + n)
 };
 __device__ __forceinline__ Item item_of(const Params& p, int j) {
   Item it;
-  it.keys = j < p.key_items;
+  const int first = p.keys_last ? p.items - p.key_items : p.key_items;
+  it.keys = (j < first) != (bool)p.keys_last;
   const Pass& s = it.keys ? p.keys : p.queries;
-  if (!it.keys) j -= p.key_items;
+  if (j >= first) j -= first;
   it.cut = j % s.cuts;
   j /= s.cuts;
   it.bh = j / s.Ft;
@@ -300,6 +305,9 @@ struct Shared {
   uint64_t* acc_free;     // [2] ... and folded into registers (8 warps)
   uint64_t* held_full;    // the item's held operands are in tensor memory (8 warps)
   uint64_t* all_done;
+  uint64_t* item_full;    // [2] the next item's number is in items[]
+  uint64_t* item_empty;   // [2] ... and read (MMA thread, 8 warps)
+  volatile int* items;    // [2]
   uint32_t* tmem_slot;
   volatile int* abort_flag;
 };
@@ -316,7 +324,10 @@ __device__ __forceinline__ Shared carve(uint8_t* raw) {
   s.acc_free = s.acc_full + 2;
   s.held_full = s.acc_free + 2;
   s.all_done = s.held_full + 1;
-  s.tmem_slot = reinterpret_cast<uint32_t*>(s.all_done + 1);
+  s.item_full = s.all_done + 1;
+  s.item_empty = s.item_full + 2;
+  s.items = reinterpret_cast<volatile int*>(s.item_empty + 2);
+  s.tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(s.items) + 2);
   s.abort_flag = reinterpret_cast<volatile int*>(s.tmem_slot + 1);
   return s;
 }
@@ -550,6 +561,8 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_bwd_tc(const __grid_constant
       mbar_init(&sh.ed_full[i], 8);
       mbar_init(&sh.acc_full[i], 1);
       mbar_init(&sh.acc_free[i], 8);
+      mbar_init(&sh.item_full[i], 1);
+      mbar_init(&sh.item_empty[i], 9);
     }
     mbar_init(sh.held_full, 8);
     mbar_init(sh.all_done, 1);
@@ -570,7 +583,12 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_bwd_tc(const __grid_constant
     setmaxnreg_dec<REGS_CONTROL>();
     if (warp == 0) {
       if (elect_one()) {
-        for (int j = blockIdx.x; j < p.items && ok; j += gridDim.x) {
+        for (int i = 0; ok; ++i) {
+          const int j = i == 0 ? (int)blockIdx.x : (int)gridDim.x + atomicAdd(p.next, 1);
+          if (i >= 2 && !mbar_wait(&sh.item_empty[i & 1], ((i >> 1) & 1) ^ 1, p.status, kDevTimeoutProducer, sh.abort_flag)) break;
+          sh.items[i & 1] = j;
+          mbar_arrive(&sh.item_full[i & 1]);
+          if (j >= p.items) break;
           const Item it = item_of(p, j);
           ok = it.keys ? load_item<true>(p, p.keys, it, &m.q1h, &m.q1l, &m.q2h, &m.q2l, sh, G)
                        : load_item<false>(p, p.queries, it, &m.k1h, &m.k1l, &m.k2h, &m.k2l, sh, G);
@@ -581,8 +599,12 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_bwd_tc(const __grid_constant
       }
     } else if (warp == 1) {
       if (elect_one()) {
-        int i = 0;
-        for (int j = blockIdx.x; j < p.items && ok; j += gridDim.x, ++i) {
+        for (int i = 0; ok; ++i) {
+          ok = mbar_wait(&sh.item_full[i & 1], (i >> 1) & 1, p.status, kDevTimeoutMma, sh.abort_flag);
+          if (!ok) break;
+          const int j = sh.items[i & 1];
+          mbar_arrive(&sh.item_empty[i & 1]);
+          if (j >= p.items) break;
           const Item it = item_of(p, j);
           ok = mbar_wait(sh.held_full, i & 1, p.status, kDevTimeoutMma, sh.abort_flag);
           if (!ok) break;
@@ -595,7 +617,13 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_bwd_tc(const __grid_constant
     }
   } else {
     setmaxnreg_inc<REGS_COMPUTE>();
-    for (int j = blockIdx.x; j < p.items && ok; j += gridDim.x) {
+    for (int i = 0; ok; ++i) {
+      ok = warp_wait(&sh.item_full[i & 1], (i >> 1) & 1, p.status, kDevTimeoutConsumer, sh.abort_flag);
+      if (!ok) break;
+      const int j = sh.items[i & 1];
+      __syncwarp();
+      if (lane_id() == 0) mbar_arrive(&sh.item_empty[i & 1]);
+      if (j >= p.items) break;
       const Item it = item_of(p, j);
       ok = it.keys ? compute_item<true, BIAS>(p, p.keys, it, sh, tmem, G, P)
                    : compute_item<false, BIAS>(p, p.queries, it, sh, tmem, G, P);
@@ -719,10 +747,11 @@ __device__ __forceinline__ float4 block_max4(float4 v, float4* sm) {
 // g = dO / l, 7 - m, -delta.
 __global__ void __launch_bounds__(256) bwd_split_k(Rows q, Rows dout, Rows out, Rows k, Rows v, Bias bias,
                                                    const float2* __restrict__ stats, int64_t stats_ld, int H, int vec,
-                                                   Side qs, Side ks) {
+                                                   Side qs, Side ks, int* next) {
   __shared__ float4 sm[8];
   const int bh = blockIdx.x, b = bh / H, h = bh - b * H, c0 = (threadIdx.x & 3) * 16;
   const int key_tiles = ks.Lt / HELD;
+  if (bh == 0 && blockIdx.y == 0 && threadIdx.x == 0) *next = 0;  // the main kernel's item counter
   const bool keys = (int)blockIdx.y < key_tiles;
   const Side& s = keys ? ks : qs;
   const int row0 = (keys ? blockIdx.y : blockIdx.y - key_tiles) * HELD + (threadIdx.x >> 2);
@@ -881,36 +910,55 @@ __global__ void __launch_bounds__(256) join_k(const float* __restrict__ part, in
   const int bh = (int)(i / D / L), b = bh / H, h = bh - b * H;
   const float* src = part + ((int64_t)bh * Lt + row) * D + d;
   float s = 0.0f;
-#pragma unroll 4
+#pragma unroll 16
   for (int c = 0; c < cuts; ++c) s += src[(int64_t)c * BH * Lt * D];
   out[b * sb + h * sh + row * sl + d] = s;
 }
 
 // Shares of the keys joined: partial outputs [cuts, BH or B, Lq, ...] as normalised by their own sums,
-// with their statistics.  A warp per row; the shares in their order.  last: the statistics' last row
-// has no bias kernel to set it.
+// with their statistics.  W warps per row (8 where there are more shares than that, else 1): warp w adds
+// shares w, w + W, ..., then the warps' sums are added in order.  last: the statistics' last row has
+// no bias kernel to set it.
+template <int W>
 __global__ void __launch_bounds__(256) attn_join_k(const float* __restrict__ o, const float2* __restrict__ st, int cuts,
-                                                   int64_t cut_o, int64_t cut_st, int64_t st_ld, int by_head, int BH, int H,
-                                                   int Lq, int last, float* __restrict__ out, float2* __restrict__ stats) {
-  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (i >= (int64_t)BH * Lq) return;
+                                                   int64_t cut_o, int64_t cut_st, int64_t st_ld, int by_head, int64_t n,
+                                                   int H, int Lq, int last, float* __restrict__ out,
+                                                   float2* __restrict__ stats) {
+  __shared__ float sm_l[8];
+  __shared__ float2 sm_v[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t i = W == 1 ? (int64_t)blockIdx.x * 8 + warp : blockIdx.x;
+  if (i >= n) return;
   const int bh = (int)(i / Lq), row = (int)(i - (int64_t)bh * Lq), b = bh / H, h = bh - b * H;
   const int64_t dst = (((int64_t)b * Lq + row) * H + h) * D + lane * 2;
   const float* src = o + (by_head ? i * D + lane * 2 : dst);
   const float2* s = st + bh * st_ld + row;
   float m = -INFINITY;
-  for (int c = 0; c < cuts; ++c) m = fmaxf(m, s[c * cut_st].x);
+  for (int c = lane; c < cuts; c += 32) m = fmaxf(m, s[c * cut_st].x);
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
   float l = 0.0f;
   float2 v = make_float2(0.0f, 0.0f);
-#pragma unroll 4
-  for (int c = 0; c < cuts; ++c) {
+#pragma unroll 8
+  for (int c = W == 1 ? 0 : warp; c < cuts; c += W) {
     const float2 ml = s[c * cut_st];
     const float w = ml.y * (ml.x == m ? 1.0f : ex2(ml.x - m));
     const float2 x = *reinterpret_cast<const float2*>(src + c * cut_o);
     l += w;
     v.x = fmaf(w, x.x, v.x);
     v.y = fmaf(w, x.y, v.y);
+  }
+  if (W > 1) {
+    sm_v[warp][lane] = v;
+    if (lane == 0) sm_l[warp] = l;
+    __syncthreads();
+    if (warp != 0) return;
+#pragma unroll
+    for (int w = 1; w < 8; ++w) {
+      l += sm_l[w];
+      v.x += sm_v[w][lane].x;
+      v.y += sm_v[w][lane].y;
+    }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   *reinterpret_cast<float2*>(out + dst) = make_float2(v.x * inv, v.y * inv);
@@ -1006,7 +1054,8 @@ static void cut_walks(Pass& keys, Pass& queries, int64_t BH) {
     s.span = s.T;
     const int64_t fair = share / (q ? 3 : 4) - 4;  // tiles
     if (s.T <= fair || s.T < 8) continue;
-    s.span = (int)(fair < 4 ? 4 : (fair + 1) / 2 * 2);
+    const int64_t most = fair < 4 ? 4 : fair, cuts = (s.T + most - 1) / most;
+    s.span = (int)(((s.T + cuts - 1) / cuts + 1) / 2 * 2);
     s.cuts = (s.T + s.span - 1) / s.span;
   }
 }
@@ -1070,8 +1119,12 @@ int triposplat_b200_attention_forward(const float* q, const float* k, const floa
   auto join = [&](const float* o, const float2* part, int cuts, int64_t cut_o, int64_t cut_st, int64_t st_ld, int by_head,
                   int last) {
     LaunchScope scope(kKSdpaSplit, stream);
-    attn_join_k<<<(unsigned)((BH * Lq + 7) / 8), 256, 0, stream>>>(o, part, cuts, cut_o, cut_st, st_ld, by_head, (int)BH, H,
-                                                                 Lq, last, out_blhd, rows);
+    if (cuts > 8)
+      attn_join_k<8><<<(unsigned)(BH * Lq), 256, 0, stream>>>(o, part, cuts, cut_o, cut_st, st_ld, by_head, BH * Lq, H, Lq,
+                                                            last, out_blhd, rows);
+    else
+      attn_join_k<1><<<(unsigned)((BH * Lq + 7) / 8), 256, 0, stream>>>(o, part, cuts, cut_o, cut_st, st_ld, by_head,
+                                                                      BH * Lq, H, Lq, last, out_blhd, rows);
   };
   if (Lq <= kFewRows) {
     FewArgs a{};
@@ -1189,7 +1242,7 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
   const size_t kpart = p.keys.cuts > 1 ? al256((size_t)p.keys.cuts * BH * ks.Lt * D * 4) : 0;
   const size_t qpart = p.queries.cuts > 1 ? al256((size_t)p.queries.cuts * BH * qs.Lt * D * 4) : 0;
   const size_t db_bytes = dbias ? al256((size_t)2 * p.keys.cuts * BH * ks.Lt * 4) : 0;
-  uint8_t* ws = static_cast<uint8_t*>(workspace(qbytes + kbytes + 2 * kpart + qpart + db_bytes, stream));
+  uint8_t* ws = static_cast<uint8_t*>(workspace(qbytes + kbytes + 2 * kpart + qpart + db_bytes + 256, stream));
   if (!ws) return kWorkspace;
   side_layout(ws, BH, Lq, true, qs);
   side_layout(ws + qbytes, BH, Lk, false, ks);
@@ -1207,6 +1260,8 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
   p.queries.s1b = go[0]; p.queries.s1h = go[1]; p.queries.s1l = go[2];
   p.queries.vec_out = vec_out;
   p.db = dbias ? reinterpret_cast<float*>(at + 2 * kpart + qpart) : nullptr;
+  p.next = reinterpret_cast<int*>(at + 2 * kpart + qpart + db_bytes);
+  p.keys_last = 4 * (p.keys.span + 4) < 3 * (p.queries.span + 4);
   p.head = rows + Lq;
   p.head_stride = Lq + 1;
   p.H = H;
@@ -1224,7 +1279,7 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
     LaunchScope scope(kKSdpaSplit, stream);
     bwd_split_k<<<dim3((unsigned)BH, (ks.Lt + qs.Lt) / HELD), 256, 0, stream>>>(
         rows_of(q, strides + 3), rows_of(dout, strides), rows_of(out, strides + 12), rows_of(k, strides + 6),
-        rows_of(v, strides + 9), bias, rows, Lq + 1, H, vec, qs, ks);
+        rows_of(v, strides + 9), bias, rows, Lq + 1, H, vec, qs, ks, p.next);
   }
   {
     LaunchScope scope(kKSdpaAttn, stream);

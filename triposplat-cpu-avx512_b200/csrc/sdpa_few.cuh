@@ -4,7 +4,7 @@
 // and walk them with one held tile per head.
 //
 // Four lanes per key, 16 of its 64 dimensions each; a score is 16 products per lane and two shuffles.
-// A block takes a share of a head's keys, eight warps of eight keys at a time.  Forward: each group
+// A block takes a share of a head's keys, four warps of eight keys at a time.  Forward: each group
 // of four lanes keeps a softmax of its own (integer reference m in log2 units, raised when a score
 // passes it by more than 8, so that its factor is a power of two; l; 16 output values per row),
 // joined over the warp by shuffles, over the block in shared memory, and over the shares of the keys by
@@ -14,7 +14,7 @@
 // Included by sdpa_backward.cu, whose Rows, Bias and helpers it uses.
 
 constexpr int kFewRows = 4;
-constexpr int kFewThreads = 256;
+constexpr int kFewThreads = 128;
 
 struct FewArgs {
   Rows q, k, v, out, dout;
@@ -67,6 +67,7 @@ __global__ void __launch_bounds__(kFewThreads) few_fwd_k(const FewArgs a) {
 #pragma unroll 1
   for (int jb = blockIdx.x * a.span + warp * 8; jb < j1; jb += kFewThreads / 4) {  // uniform over the warp
     const int j = jb + (lane >> 2);
+    asm volatile("" ::: "memory");  // the rows stay in shared memory: registers are short
     float off = -INFINITY, kv[16], vv[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) kv[e] = vv[e] = 0.0f;
@@ -147,7 +148,8 @@ __global__ void __launch_bounds__(kFewThreads) few_bwd_k(const FewArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = (lane & 3) * 16;
   const float2 head = a.bias.p ? a.head[bh * a.head_stride] : make_float2(0.0f, 1.0f);
   const float c = 0.125f * LOG2E * head.y;
-  if (warp < NQ) {  // a warp per row: q, g = dO / l, delta = g . O, m
+  static_assert(NQ <= kFewThreads / 32, "a warp per row");
+  if (warp < NQ) {  // q, g = dO / l, delta = g . O, m
     const int r = warp;
     float delta = 0.0f, m = INFINITY;
     float q[2] = {0.0f, 0.0f}, g[2] = {0.0f, 0.0f};
@@ -181,6 +183,7 @@ __global__ void __launch_bounds__(kFewThreads) few_bwd_k(const FewArgs a) {
 #pragma unroll 1
   for (int jb = blockIdx.x * a.span + warp * 8; jb < j1; jb += kFewThreads / 4) {
     const int j = jb + (lane >> 2);
+    asm volatile("" ::: "memory");  // the rows stay in shared memory: registers are short
     float off = -INFINITY, kv[16], vv[16], dk[16], dv[16], db = 0.0f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) kv[e] = vv[e] = dk[e] = dv[e] = 0.0f;
@@ -247,12 +250,12 @@ __global__ void __launch_bounds__(kFewThreads) few_bwd_k(const FewArgs a) {
   }
 }
 
-// Keys per block so that the GPU has some four blocks per SM, a multiple of the 64 that a block takes
-// at a time.
+// Keys per block so that the GPU has some eight blocks per SM, a multiple of the 32 that a block takes
+// at a time and no less than four times that.
 static void few_shares(FewArgs& a) {
-  const int64_t want = ((int64_t)sm_count() * 4 + a.BH - 1) / a.BH;
+  const int64_t want = ((int64_t)sm_count() * 8 + a.BH - 1) / a.BH;
   const int64_t span = (a.Lk + want - 1) / want;
-  a.span = (int)((span + 63) / 64 * 64);
+  a.span = (int)((span < 128 ? 128 : span + 31) / 32 * 32);
   a.shares = (a.Lk + a.span - 1) / a.span;
 }
 
