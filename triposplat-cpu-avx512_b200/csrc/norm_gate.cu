@@ -48,29 +48,61 @@ struct Args {
   float rho, eps;
 };
 
-// Sum over a row's threads: one warp, or the whole block (`sm` [2][32] float2, alternated by
-// `turn`, so one barrier per sum is enough).
-__device__ __forceinline__ float2 row_sum(float2 v, float2 (*sm)[32], int& turn) {
-  v.x = warp_sum(v.x);
-  v.y = warp_sum(v.y);
-  if (blockDim.x == 32) return v;
-  float2* s = sm[turn];
-  turn ^= 1;
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float2 r = make_float2(0.0f, 0.0f);
-  for (unsigned w = 0; w < blockDim.x / 32; ++w) {
-    r.x += s[w].x;
-    r.y += s[w].y;
+// Sums over a row's threads: one warp, or the whole block (`sm` [2][16] per summed value, alternated
+// by `turn`, so one barrier per sum is enough; slots of warps that a block lacks are zero).
+struct RowSum {
+  float2 (*sm)[16];
+  int turn;
+  __device__ __forceinline__ RowSum(float2 (*s)[16]) : sm(s), turn(0) {
+    const int t = threadIdx.y * blockDim.x + threadIdx.x;
+    if (t < 32) sm[t / 16][t % 16] = make_float2(0.0f, 0.0f);
+    if (blockDim.x > 32) __syncthreads();
   }
-  return r;
-}
+  __device__ __forceinline__ float2 operator()(float2 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+    if (blockDim.x == 32) return v;
+    const float4* s = share(v);
+    float4 r = s[0];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) {
+      if (w * 64 >= blockDim.x) break;
+      const float4 u = s[w];
+      r.x += u.x; r.y += u.y; r.z += u.z; r.w += u.w;
+    }
+    return make_float2(r.x + r.z, r.y + r.w);
+  }
+  __device__ __forceinline__ float operator()(float v) {
+    v = warp_sum(v);
+    if (blockDim.x == 32) return v;
+    const float4* s = share(make_float2(v, 0.0f));
+    float r = s[0].x + s[0].z;
+#pragma unroll
+    for (int w = 1; w < 8; ++w) {
+      if (w * 64 >= blockDim.x) break;
+      r += s[w].x + s[w].z;
+    }
+    return r;
+  }
+
+ private:
+  __device__ __forceinline__ const float4* share(float2 v) {
+    float2* s = sm[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return reinterpret_cast<const float4*>(s);
+  }
+};
 
 // mean (0 for rms) and r of a row held in registers; elements past C are zero and stay out of
-// the centred sum through `valid`
+// the centred sum
 template <int VEC, int NI>
-__device__ __forceinline__ float2 row_stats(const float (&v)[NI][VEC], int kind, int C, float eps,
-                                            float2 (*sm)[32], int& turn) {
+__device__ __forceinline__ float2 row_stats(const float (&v)[NI][VEC], int kind, int C, float inv_c, float eps,
+                                            RowSum& sum) {
   float mean = 0.0f;
   if (kind == kLayer) {
     float s = 0.0f;
@@ -78,26 +110,33 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[NI][VEC], int kind,
     for (int i = 0; i < NI; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) s += v[i][e];
-    mean = row_sum(make_float2(s, 0.0f), sm, turn).x / (float)C;
+    mean = sum(s) * inv_c;
   }
   float q = 0.0f;
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
+    // C is a multiple of VEC: a run is inside the row or not at all
+    if ((i * (int)blockDim.x + (int)threadIdx.x) * VEC < C) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const float d = v[i][e] - mean;
-      if (c + e < C) q = fmaf(d, d, q);
+      for (int e = 0; e < VEC; ++e) {
+        const float d = v[i][e] - mean;
+        q = fmaf(d, d, q);
+      }
     }
   }
-  q = row_sum(make_float2(q, 0.0f), sm, turn).x;
-  return make_float2(mean, 1.0f / sqrtf(q / (float)C + eps));
+  return make_float2(mean, rsqrtf(fmaf(sum(q), inv_c, eps)));
 }
 
 // A row's elements of one tensor as they lie in memory, and as numbers (zeros past C).
 template <class T, int VEC, int NI>
 struct RawRow {
   Pack<T, VEC> v[NI];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[i].v[e] = from_f32<T>(0.0f);
+  }
   __device__ __forceinline__ void load(const T* p, int C) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
@@ -105,13 +144,11 @@ struct RawRow {
       if (c < C) v[i] = *reinterpret_cast<const Pack<T, VEC>*>(p + c);
     }
   }
-  __device__ __forceinline__ void get(int C, float (&f)[NI][VEC]) const {
+  __device__ __forceinline__ void get(float (&f)[NI][VEC]) const {
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) f[i][e] = c < C ? to_f32(v[i].v[e]) : 0.0f;
-    }
+      for (int e = 0; e < VEC; ++e) f[i][e] = to_f32(v[i].v[e]);
   }
 };
 
@@ -139,18 +176,24 @@ __device__ __forceinline__ void load_coef(const float* a, const float* b, float 
 // Row group g of batch entry blockIdx.y takes the entry's rows g, g + groups, g + 2 groups, ...
 template <class T, int VEC, int NI, int MAXT>
 __global__ void __launch_bounds__(MAXT, 1) norm_gate_k(const Args a) {
-  __shared__ float2 sm[2][32];
-  int turn = 0;
+  __shared__ __align__(16) float2 sm[2][16];
+  RowSum sum(sm);
+  const float inv_c = 1.0f / (float)a.C;
   const int64_t b = blockIdx.y, g = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  const T* x = static_cast<const T*>(a.x) + b * a.xb;
-  const T* y = static_cast<const T*>(a.y) + b * a.yb;
+  const T* x = static_cast<const T*>(a.x) + b * a.xb + g * a.xl;
+  const T* y = static_cast<const T*>(a.y) + b * a.yb + g * a.yl;
+  const int64_t dx = a.groups * a.xl, dy = a.groups * a.yl;
   RawRow<T, VEC, NI> ry, rx;
-  auto fetch = [&](int64_t l) {
-    ry.load(y + l * a.yl, a.C);
-    rx.load(x + l * a.xl, a.C);
+  ry.clear();
+  rx.clear();
+  auto fetch = [&]() {  // the next row of the group
+    ry.load(y, a.C);
+    rx.load(x, a.C);
+    y += dy;
+    x += dx;
   };
   constexpr bool kAhead = NI * VEC <= 8;
-  if (kAhead && g < a.L) fetch(g);
+  if (kAhead && g < a.L) fetch();
   float gw[NI][VEC], sw[NI][VEC], sh[NI][VEC];
   load_coef<VEC, NI>(a.wpost, a.gate ? a.gate + b * a.C : nullptr, a.gate ? 0.0f : 1.0f, a.C, gw);
   load_coef<VEC, NI>(a.wpre, a.scale ? a.scale + b * a.C : nullptr, 1.0f, a.C, sw);
@@ -159,12 +202,12 @@ __global__ void __launch_bounds__(MAXT, 1) norm_gate_k(const Args a) {
   for (int64_t l = g; l < a.L; l += a.groups) {
     const int64_t r = b * a.L + l;
     float z[NI][VEC], m[NI][VEC];
-    if (!kAhead) fetch(l);
-    ry.get(a.C, m);
-    rx.get(a.C, z);
-    if (kAhead && l + a.groups < a.L) fetch(l + a.groups);
+    if (!kAhead) fetch();
+    ry.get(m);
+    rx.get(z);
+    if (kAhead && l + a.groups < a.L) fetch();
     float2 sp = make_float2(0.0f, 1.0f), sn = make_float2(0.0f, 1.0f);
-    if (a.post != kNone) sp = row_stats<VEC, NI>(m, a.post, a.C, a.eps, sm, turn);
+    if (a.post != kNone) sp = row_stats<VEC, NI>(m, a.post, a.C, inv_c, a.eps, sum);
     const float rs = sp.y * a.rho;
 #pragma unroll
     for (int i = 0; i < NI; ++i)
@@ -172,7 +215,7 @@ __global__ void __launch_bounds__(MAXT, 1) norm_gate_k(const Args a) {
       for (int e = 0; e < VEC; ++e) z[i][e] = fmaf((m[i][e] - sp.x) * rs, gw[i][e], z[i][e]);
     store_row<T, VEC, NI>(static_cast<T*>(a.out0) + r * a.C, a.C, z);
     if (a.pre != kNone) {
-      sn = row_stats<VEC, NI>(z, a.pre, a.C, a.eps, sm, turn);
+      sn = row_stats<VEC, NI>(z, a.pre, a.C, inv_c, a.eps, sum);
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -186,26 +229,37 @@ __global__ void __launch_bounds__(MAXT, 1) norm_gate_k(const Args a) {
 
 template <class T, int VEC, int NI, int MAXT>
 __global__ void __launch_bounds__(MAXT, 1) norm_gate_bwd_k(const Args a) {
-  __shared__ float2 sm[2][32];
-  int turn = 0;
+  __shared__ __align__(16) float2 sm[2][16];
+  RowSum sum(sm);
   const int64_t b = blockIdx.y, g = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const float inv_c = 1.0f / (float)a.C;
-  const T* x = static_cast<const T*>(a.x) + b * a.xb;
-  const T* y = static_cast<const T*>(a.y) + b * a.yb;
   const bool has_h = a.dh != nullptr, has_z = a.dz != nullptr;
-  const T* dh = has_h ? static_cast<const T*>(a.dh) + b * a.hb : nullptr;
-  const T* dz = has_z ? static_cast<const T*>(a.dz) + b * a.zb : nullptr;
+  const T* x = static_cast<const T*>(a.x) + b * a.xb + g * a.xl;
+  const T* y = static_cast<const T*>(a.y) + b * a.yb + g * a.yl;
+  const T* dh = has_h ? static_cast<const T*>(a.dh) + b * a.hb + g * a.hl : nullptr;
+  const T* dz = has_z ? static_cast<const T*>(a.dz) + b * a.zb + g * a.zl : nullptr;
+  const float4* stats = reinterpret_cast<const float4*>(a.stats) + b * a.L + g;
+  const int64_t ix = a.groups * a.xl, iy = a.groups * a.yl, ih = a.groups * a.hl, iz = a.groups * a.zl;
   RawRow<T, VEC, NI> ry, rx, rh, rz;
+  ry.clear();
+  rx.clear();
+  rh.clear();
+  rz.clear();
   float4 st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
-  auto fetch = [&](int64_t l) {
-    ry.load(y + l * a.yl, a.C);
-    rx.load(x + l * a.xl, a.C);
-    if (has_h) rh.load(dh + l * a.hl, a.C);
-    if (has_z) rz.load(dz + l * a.zl, a.C);
-    st = __ldg(reinterpret_cast<const float4*>(a.stats + 4 * (b * a.L + l)));
+  auto fetch = [&]() {  // the next row of the group
+    ry.load(y, a.C);
+    rx.load(x, a.C);
+    if (has_h) rh.load(dh, a.C);
+    if (has_z) rz.load(dz, a.C);
+    st = __ldg(stats);
+    y += iy;
+    x += ix;
+    dh += ih;
+    dz += iz;
+    stats += a.groups;
   };
   constexpr bool kAhead = NI * VEC <= 8;
-  if (kAhead && g < a.L) fetch(g);
+  if (kAhead && g < a.L) fetch();
   float gw[NI][VEC], sw[NI][VEC];
   load_coef<VEC, NI>(a.wpost, a.gate ? a.gate + b * a.C : nullptr, a.gate ? 0.0f : 1.0f, a.C, gw);
   load_coef<VEC, NI>(a.wpre, a.scale ? a.scale + b * a.C : nullptr, 1.0f, a.C, sw);
@@ -221,13 +275,13 @@ __global__ void __launch_bounds__(MAXT, 1) norm_gate_bwd_k(const Args a) {
   for (int64_t l = g; l < a.L; l += a.groups) {
     const int64_t r = b * a.L + l;
     float n[NI][VEC], m[NI][VEC], d[NI][VEC], dzv[NI][VEC];
-    if (!kAhead) fetch(l);
-    ry.get(a.C, m);
-    rx.get(a.C, n);
+    if (!kAhead) fetch();
+    ry.get(m);
+    rx.get(n);
     const float4 s4 = st;
-    if (has_h) rh.get(a.C, d);
-    if (has_z) rz.get(a.C, dzv);
-    if (kAhead && l + a.groups < a.L) fetch(l + a.groups);
+    if (has_h) rh.get(d);
+    if (has_z) rz.get(dzv);
+    if (kAhead && l + a.groups < a.L) fetch();
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -248,7 +302,7 @@ __global__ void __launch_bounds__(MAXT, 1) norm_gate_bwd_k(const Args a) {
           s.x += d[i][e];
           s.y = fmaf(d[i][e], n[i][e], s.y);
         }
-      s = row_sum(s, sm, turn);
+      s = sum(s);
       const float mean = a.pre == kLayer ? s.x * inv_c : 0.0f, dot = s.y * inv_c;
 #pragma unroll
       for (int i = 0; i < NI; ++i)
@@ -279,7 +333,7 @@ __global__ void __launch_bounds__(MAXT, 1) norm_gate_bwd_k(const Args a) {
         s.y = fmaf(d[i][e], m[i][e], s.y);
       }
     if (a.post != kNone) {
-      s = row_sum(s, sm, turn);
+      s = sum(s);
       const float mean = a.post == kLayer ? s.x * inv_c : 0.0f, dot = s.y * inv_c;
 #pragma unroll
       for (int i = 0; i < NI; ++i)
