@@ -15,12 +15,16 @@
 // order in registers and writes one partial row; a second kernel adds the partial rows in a
 // fixed order: no atomics, the same bits on every run.
 //
-// Bound by HBM: every tensor is read or written once.  A row is held in registers (8 or 16
-// elements per thread) by one warp (up to 256 columns) or one block, statistics are taken
+// Bound by HBM: every tensor is read or written once.  A row is held in registers (4, 8 or 16
+// elements per thread) by one warp (up to 128 columns) or one block, statistics are taken
 // in two passes over the registers (mean, then centred squares) in fp32.  A row group keeps its
 // columns' coefficients (rho gate w_post, (1 + scale) w_pre, shift) in registers over all its rows,
 // and (up to 4096 columns; beyond, registers are short) the next row's loads are in flight while a
-// row is worked on.
+// row is worked on.  Measured, 8193 x 1024 x 2 in fp32: forward 46 us (5.8 TB/s), backward 81 us (5.0)
+// and 7 for the column sums; with 4 elements per thread, twice the warps per barrier, 55 and 94 us,
+// with a warp per row and coefficients in shared memory (no barriers, 200 registers) 96 and 134.
+// Odd widths go element by element: 2051 x 1111 x 3 in bf16 34 and 63 us, bound by instructions (the
+// backward kernel held to 128 registers, two blocks per SM: with 208 only one fits, 80 us).
 #include <stdint.h>
 
 #include <initializer_list>
@@ -33,7 +37,7 @@ namespace tsb {
 namespace ng {
 
 enum Kind : int { kNone = 0, kLayer = 1, kRms = 2 };
-constexpr int kMaxThreads = 512;   // per row: 8 columns each up to 4096, 16 beyond
+constexpr int kMaxThreads = 512;   // per row: 4 columns each up to 512, 8 up to 4096, 16 beyond
 constexpr int kMaxColumns = 8192;
 
 struct Args {
@@ -228,7 +232,7 @@ __global__ void __launch_bounds__(MAXT, 1) norm_gate_k(const Args a) {
 }
 
 template <class T, int VEC, int NI, int MAXT>
-__global__ void __launch_bounds__(MAXT, 1) norm_gate_bwd_k(const Args a) {
+__global__ void __launch_bounds__(MAXT, MAXT == 256 && VEC == 1 ? 2 : 1) norm_gate_bwd_k(const Args a) {
   __shared__ __align__(16) float2 sm[2][16];
   RowSum sum(sm);
   const int64_t b = blockIdx.y, g = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
@@ -365,33 +369,47 @@ struct ReduceArgs {
 };
 
 // 32 columns of one of the three sums (blockIdx.y) per block, 32 threads per column; partial rows
-// added in a fixed order.
+// added in a fixed order, four batch entries at a time so that their loads overlap.
 __global__ void __launch_bounds__(1024) norm_gate_reduce_k(const ReduceArgs a) {
-  __shared__ float sm[32][33];
+  constexpr int NB = 4;
+  __shared__ float sm[NB][32][33];
   const int c = blockIdx.x * 32 + threadIdx.x, y = threadIdx.y, q = blockIdx.y;
   float dw = 0.0f;
-  for (int b = 0; b < a.B; ++b) {
-    float s = 0.0f;
-    if (c < a.C) {
-      const float* p = a.part + ((int64_t)b * a.groups * 3 + q) * a.C + c;
+  for (int b0 = 0; b0 < a.B; b0 += NB) {
+    float s[NB];
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      s[u] = 0.0f;
+      if (c < a.C && b0 + u < a.B) {
+        const float* p = a.part + ((int64_t)(b0 + u) * a.groups * 3 + q) * a.C + c;
 #pragma unroll 8
-      for (int g = y; g < a.groups; g += 32) s += p[(int64_t)g * 3 * a.C];
+        for (int g = y; g < a.groups; g += 32) s[u] += p[(int64_t)g * 3 * a.C];
+      }
     }
-    sm[threadIdx.x][y] = s;
+#pragma unroll
+    for (int u = 0; u < NB; ++u) sm[u][threadIdx.x][y] = s[u];
+    __syncthreads();
+    // warp u adds entry u's column sums
+    float t = 0.0f;
+    if (y < NB) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) t += sm[y][threadIdx.x][j];
+      sm[y][threadIdx.x][32] = t;
+    }
     __syncthreads();
     if (y == 0 && c < a.C) {
-      s = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 32; ++j) s += sm[threadIdx.x][j];
-      const int64_t bc = (int64_t)b * a.C + c;
-      if (q == 0) {
-        if (a.dshift) a.dshift[bc] = s;
-      } else if (q == 1) {
-        if (a.dscale) a.dscale[bc] = s * (a.wpre ? a.wpre[c] : 1.0f);
-        dw = fmaf(1.0f + (a.scale ? a.scale[bc] : 0.0f), s, dw);
-      } else {
-        if (a.dgate) a.dgate[bc] = s * a.rho * (a.wpost ? a.wpost[c] : 1.0f);
-        dw = fmaf(a.rho * (a.gate ? a.gate[bc] : 1.0f), s, dw);
+      for (int u = 0; u < NB && b0 + u < a.B; ++u) {
+        const float v = sm[u][threadIdx.x][32];
+        const int64_t bc = (int64_t)(b0 + u) * a.C + c;
+        if (q == 0) {
+          if (a.dshift) a.dshift[bc] = v;
+        } else if (q == 1) {
+          if (a.dscale) a.dscale[bc] = v * (a.wpre ? a.wpre[c] : 1.0f);
+          dw = fmaf(1.0f + (a.scale ? a.scale[bc] : 0.0f), v, dw);
+        } else {
+          if (a.dgate) a.dgate[bc] = v * a.rho * (a.wpost ? a.wpost[c] : 1.0f);
+          dw = fmaf(a.rho * (a.gate ? a.gate[bc] : 1.0f), v, dw);
+        }
       }
     }
     __syncthreads();
@@ -402,33 +420,35 @@ __global__ void __launch_bounds__(1024) norm_gate_reduce_k(const ReduceArgs a) {
   }
 }
 
-// 16-byte accesses where every row of every tensor starts on a 16-byte boundary, single
-// elements otherwise (odd widths, sliced views)
-static bool vec_ok(const Args& a, int size) {
-  const int64_t n = 16 / size;
-  auto bad = [&](const void* p, int64_t sb, int64_t sl) {
-    return p && ((reinterpret_cast<uintptr_t>(p) & 15) || sb % n || sl % n);
-  };
-  if (a.C % n) return false;
-  return !(bad(a.x, a.xb, a.xl) || bad(a.y, a.yb, a.yl) || bad(a.dz, a.zb, a.zl) || bad(a.dh, a.hb, a.hl) ||
-           bad(a.out0, 0, 0) || bad(a.out1, 0, 0));
+// The widest accesses, of 4, 2 or 1 elements, for which every row of every tensor starts on a boundary
+// of that size (odd widths and sliced views fall to the narrower ones).
+static int vec_of(const Args& a, int size) {
+  for (int n = 4; n > 1; n /= 2) {
+    auto bad = [&](const void* p, int64_t sb, int64_t sl) {
+      return p && ((reinterpret_cast<uintptr_t>(p) & (n * size - 1)) || sb % n || sl % n);
+    };
+    if (a.C % n == 0 && !bad(a.x, a.xb, a.xl) && !bad(a.y, a.yb, a.yl) && !bad(a.dz, a.zb, a.zl) &&
+        !bad(a.dh, a.hb, a.hl) && !bad(a.out0, 0, 0) && !bad(a.out1, 0, 0))
+      return n;
+  }
+  return 1;
 }
 
 struct Shape {
   dim3 block;
-  bool wide;  // 16 elements per thread
+  int per;  // elements per thread
 };
 
 static Shape shape_of(int C) {
   Shape s;
-  s.wide = C > 8 * kMaxThreads;
-  const int per = s.wide ? 16 : 8;
-  const int t = ((C + per - 1) / per + 31) / 32 * 32;
+  s.per = C <= 512 ? 4 : (C <= 8 * kMaxThreads ? 8 : 16);
+  const int t = ((C + s.per - 1) / s.per + 31) / 32 * 32;
   s.block = t == 32 ? dim3(32, 4) : dim3(t, 1);
   return s;
 }
 
-// Row groups per batch entry so that about `threads` threads per SM run, one row per group at least.
+// Row groups per batch entry so that about `threads` threads per SM are launched, one row per group at
+// least: twice what is resident evens out the SMs' shares (forward, 768 in place of 1024: 53 us).
 static dim3 grid_of(Args& a, const Shape& s, int threads) {
   const int64_t per_sm = threads / (int)s.block.x > 0 ? threads / (int)s.block.x : 1;
   const int64_t want = (sm_count() * per_sm + a.B - 1) / a.B;
@@ -436,17 +456,42 @@ static dim3 grid_of(Args& a, const Shape& s, int threads) {
   return dim3((a.groups + s.block.y - 1) / s.block.y, a.B);
 }
 
-template <class T, int VEC>
-static void launch_fwd(const Args& a, const Shape& s, dim3 grid, cudaStream_t st) {
-  if (s.wide) norm_gate_k<T, VEC, 16 / VEC, kMaxThreads><<<grid, s.block, 0, st>>>(a);
-  else if (s.block.x > 256) norm_gate_k<T, VEC, 8 / VEC, kMaxThreads><<<grid, s.block, 0, st>>>(a);
-  else norm_gate_k<T, VEC, 8 / VEC, 256><<<grid, s.block, 0, st>>>(a);
+// Blocks of up to 256 threads may take more registers than those of up to 512 (backward, single
+// elements: half of them, see above).
+template <class T, int VEC, int PER, bool BWD>
+static void start(const Args& a, const Shape& s, dim3 grid, cudaStream_t st) {
+  constexpr int NI = PER / VEC;
+  if (s.block.x * s.block.y > 256)
+    BWD ? norm_gate_bwd_k<T, VEC, NI, kMaxThreads><<<grid, s.block, 0, st>>>(a)
+        : norm_gate_k<T, VEC, NI, kMaxThreads><<<grid, s.block, 0, st>>>(a);
+  else if constexpr (PER <= 8)
+    BWD ? norm_gate_bwd_k<T, VEC, NI, 256><<<grid, s.block, 0, st>>>(a)
+        : norm_gate_k<T, VEC, NI, 256><<<grid, s.block, 0, st>>>(a);
 }
-template <class T, int VEC>
-static void launch_bwd(const Args& a, const Shape& s, dim3 grid, cudaStream_t st) {
-  if (s.wide) norm_gate_bwd_k<T, VEC, 16 / VEC, kMaxThreads><<<grid, s.block, 0, st>>>(a);
-  else if (s.block.x > 256) norm_gate_bwd_k<T, VEC, 8 / VEC, kMaxThreads><<<grid, s.block, 0, st>>>(a);
-  else norm_gate_bwd_k<T, VEC, 8 / VEC, 256><<<grid, s.block, 0, st>>>(a);
+
+template <class T, bool BWD>
+static void start_type(const Args& a, const Shape& s, int vec, dim3 grid, cudaStream_t st) {
+  if (s.per == 4) {
+    if (vec == 4) start<T, 4, 4, BWD>(a, s, grid, st);
+    else if (vec == 2) start<T, 2, 4, BWD>(a, s, grid, st);
+    else start<T, 1, 4, BWD>(a, s, grid, st);
+  } else if (s.per == 8) {
+    if (vec == 4) start<T, 4, 8, BWD>(a, s, grid, st);
+    else if (vec == 2) start<T, 2, 8, BWD>(a, s, grid, st);
+    else start<T, 1, 8, BWD>(a, s, grid, st);
+  } else {
+    if (vec == 4) start<T, 4, 16, BWD>(a, s, grid, st);
+    else start<T, 1, 16, BWD>(a, s, grid, st);
+  }
+}
+
+template <bool BWD>
+static void launch(const Args& a, const Shape& s, int dtype, dim3 grid, cudaStream_t st) {
+  const int vec = vec_of(a, dtype_size(dtype));
+  LaunchScope scope(kKElementwise, st);
+  if (dtype == kF32) start_type<float, BWD>(a, s, vec, grid, st);
+  else if (dtype == kBF16) start_type<__nv_bfloat16, BWD>(a, s, vec, grid, st);
+  else start_type<__half, BWD>(a, s, vec, grid, st);
 }
 
 // whether a tensor's pointer is not a multiple of its element's size
@@ -494,14 +539,8 @@ int triposplat_b200_norm_gate(const void* x, const void* y, const int64_t* strid
                         static_cast<const void*>(pre_weight), static_cast<const void*>(post_weight)})
     if (p && !is_device_pointer(p)) return kNotDevicePointer;
   const ng::Shape s = ng::shape_of(C);
-  const dim3 grid = ng::grid_of(a, s, 768);
-  const bool vec = ng::vec_ok(a, dtype_size(dtype));
-  cudaStream_t stream = current_stream();
-  LaunchScope scope(kKElementwise, stream);
-  if (dtype == kF32) vec ? ng::launch_fwd<float, 4>(a, s, grid, stream) : ng::launch_fwd<float, 1>(a, s, grid, stream);
-  else if (dtype == kBF16)
-    vec ? ng::launch_fwd<__nv_bfloat16, 8>(a, s, grid, stream) : ng::launch_fwd<__nv_bfloat16, 1>(a, s, grid, stream);
-  else vec ? ng::launch_fwd<__half, 8>(a, s, grid, stream) : ng::launch_fwd<__half, 1>(a, s, grid, stream);
+  const dim3 grid = ng::grid_of(a, s, 1024);
+  ng::launch<false>(a, s, dtype, grid, current_stream());
   return launch_status();
 }
 
@@ -541,15 +580,7 @@ int triposplat_b200_norm_gate_backward(const void* dz, const void* dh, const voi
     a.part = static_cast<float*>(workspace((size_t)B * a.groups * 3 * C * sizeof(float), stream));
     if (!a.part) return kWorkspace;
   }
-  const bool vec = ng::vec_ok(a, dtype_size(dtype));
-  {
-    LaunchScope scope(kKElementwise, stream);
-    if (dtype == kF32)
-      vec ? ng::launch_bwd<float, 4>(a, s, grid, stream) : ng::launch_bwd<float, 1>(a, s, grid, stream);
-    else if (dtype == kBF16)
-      vec ? ng::launch_bwd<__nv_bfloat16, 8>(a, s, grid, stream) : ng::launch_bwd<__nv_bfloat16, 1>(a, s, grid, stream);
-    else vec ? ng::launch_bwd<__half, 8>(a, s, grid, stream) : ng::launch_bwd<__half, 1>(a, s, grid, stream);
-  }
+  ng::launch<true>(a, s, dtype, grid, stream);
   if (sums) {
     const ng::ReduceArgs ra{a.part, gate, scale, pre_weight, post_weight, dgate, dscale, dshift, dpre_weight,
                             dpost_weight, B, C, a.groups, residual_scale};
