@@ -339,6 +339,39 @@ __device__ __forceinline__ uint64_t sw128_kmajor_desc(uint32_t smem_addr) {
   return d;
 }
 
+// The same descriptor as two words: the low one is the start address (in 16-byte units) under a
+// constant, the high one is constant, so that a step through a tile is one addition.  (K-major: 16
+// columns on is 2 units.  Read MN-major, the 64 columns being the operand's N and the rows its K, 16
+// rows on is 128 units; the distance to the next 64 columns, in the low word, is not used at N = 64.)
+constexpr uint32_t kSw128DescHi = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t sw128_desc_lo(uint32_t smem_addr) {
+  return (1024u >> 4) << 16 | ((smem_addr >> 4) & 0x3FFFu);
+}
+
+// D(tmem) (+)= A B with descriptors by their low words; a step of 128 x 64 x 16 takes the tensor core
+// 32 cycles, so the issuing thread has no more than that for its operands.
+template <bool ADD>
+__device__ __forceinline__ void mma_step_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "n"(kSw128DescHi), "r"(idesc), "n"(ADD ? 1 : 0)
+      : "memory");
+}
+template <bool ADD>
+__device__ __forceinline__ void mma_step_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %3};\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "n"(kSw128DescHi), "r"(idesc), "n"(ADD ? 1 : 0)
+      : "memory");
+}
+
 // Instruction descriptor, kind::f16 with fp16 A/B, fp32 accumulate, both K-major.
 __host__ __device__ constexpr uint32_t idesc_f16_f32(int M, int N) {
   return (1u << 4)                      // D format: f32

@@ -27,10 +27,11 @@
 //
 // Split precision as in sdpa.cu: every operand is an fp16 pair hi + lo after an exact power-of-two
 // scale (one per 128-row tile; 2^7 for e <= 2^8, and for ds a power of two from the tiles' largest
-// norms, |g . v - delta| <= |g| |v| + |delta|), each product is three tensor-core passes (hi.hi, hi.lo,
-// lo.hi), and the products of two walked tiles (24 steps) go into a fresh accumulator in tensor
-// memory that is added to fp32 registers: the tensor core's own fp32 accumulation truncates, and one
-// accumulator over thousands of rows would drift.
+// norms, |g . v - delta| <= |g| |v| + |delta|), each product is three tensor-core passes (hi.lo, lo.hi,
+// hi.hi), and the products of two walked tiles go into a fresh accumulator in tensor memory that is
+// added to fp32 registers: the tensor core's own fp32 accumulation truncates, and one accumulator over
+// thousands of rows would drift.  Measured at 8193 x 8193: errors of 5e-7 (dq, dk, dv; 2-norm), 1.2e-6
+// with hi.hi first; a tile per accumulator gives 4e-7 and takes 3% longer.
 //
 // CTA: 384 threads, one per SM, persistent over work items (pass, head, held tile, share of the walk).
 // Warp 0 loads walked tiles (64 rows: 32 KB of planes and the tile's vectors, kStages deep), warp 1
@@ -143,41 +144,21 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
       : "memory");
 }
 
-// Shared-memory descriptors of a 64-column fp16 tile (128-byte rows, 128-byte swizzle) as two words:
-// the low one is the start address (in 16-byte units) under a constant, the high one is constant.
-// K-major (columns contracted): 8-row groups 1024 bytes apart, 16 columns on is 32 bytes.
-// MN-major (rows contracted, the columns are the operand's N): the same groups, 16 rows on is 2048
-// bytes; the distance to the next 64 columns is not used at N = 64.
-constexpr uint32_t kDescHi = (1024u >> 4) | 1u << 14 | 2u << 29;
-constexpr uint32_t kDescLo = (1024u >> 4) << 16;
-__device__ __forceinline__ uint32_t desc_lo(uint32_t smem_addr) { return kDescLo | ((smem_addr >> 4) & 0x3FFFu); }
-
-// D(tmem) (+)= A(tmem) B(smem): one of a product's steps of 16 contracted elements.  The issuing
-// thread has 32 cycles of tensor-core time per call, so its operands are one addition each.
-template <bool ADD>
-__device__ __forceinline__ void mma_step(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
-      "mov.b64 b, {%2, %3};\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b_lo), "n"(kDescHi), "r"(idesc), "n"(ADD ? 1 : 0)
-      : "memory");
-}
-
 // D = A B (FRESH) or D += A B over 64 contracted elements in three passes.  A: hi and lo pairs A_STEP columns per
 // 16 elements apart, lo A_LO columns behind hi; B: tiles hi and lo (PLANE apart), B_STEP 16-byte units
-// per 16 elements.
+// per 16 elements.  The two small passes come first: every step truncates the sum so far, and this
+// way it is small (2^-11 of the result) for all steps of a fresh product but the last four.
 template <int A_STEP, int A_LO, int B_STEP, bool FRESH>
 __device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc) {
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) {
     const uint32_t ah = a + kk * A_STEP, bh = b_lo + kk * B_STEP;
-    if (FRESH && kk == 0) mma_step<false>(d, ah, bh, idesc);
-    else mma_step<true>(d, ah, bh, idesc);
-    mma_step<true>(d, ah, bh + (PLANE >> 4), idesc);
-    mma_step<true>(d, ah + A_LO, bh, idesc);
+    if (FRESH && kk == 0) mma_step_ts<false>(d, ah, bh + (PLANE >> 4), idesc);
+    else mma_step_ts<true>(d, ah, bh + (PLANE >> 4), idesc);
+    mma_step_ts<true>(d, ah + A_LO, bh, idesc);
   }
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk) mma_step_ts<true>(d, a + kk * A_STEP, b_lo + kk * B_STEP, idesc);
 }
 
 // One scale tile (128 rows) of the two tensors of a side.
@@ -368,7 +349,7 @@ __device__ __forceinline__ bool mma_item(const Params& p, int n, const Shared& s
     const int st = g_ % kStages;
     if (!mbar_wait(&sh.full[st], (g_ / kStages) & 1, p.status, kDevTimeoutMma, sh.abort_flag)) return false;
     tc_fence_after();
-    const uint32_t g = desc_lo(smem_u32(sh.tiles + st * STAGE));
+    const uint32_t g = sw128_desc_lo(smem_u32(sh.tiles + st * STAGE));
     const uint32_t x = tmem + XY_COL + (g_ & 1) * 128;
     product<8, 32, 32 / 16, true>(x, tmem + F_COL, g, idesc_xy);                                // F1 G1^T
     product<8, 32, 32 / 16, true>(x + 64, tmem + F_COL + 64, g + (2 * PLANE >> 4), idesc_xy);  // F2 G2^T
@@ -386,7 +367,7 @@ __device__ __forceinline__ bool mma_item(const Params& p, int n, const Shared& s
         !mbar_wait(&sh.acc_free[prev & 1], (prev >> 1) & 1, p.status, kDevTimeoutMma, sh.abort_flag))
       return false;
     tc_fence_after();
-    const uint32_t g = desc_lo(smem_u32(sh.tiles + st * STAGE));
+    const uint32_t g = sw128_desc_lo(smem_u32(sh.tiles + st * STAGE));
     const uint32_t x = tmem + XY_COL + (G & 1) * 128;
     const uint32_t acc1 = tmem + ACC_COL + (KEYS ? 0 : (P & 1) * 64);
     if (t & 1) {
