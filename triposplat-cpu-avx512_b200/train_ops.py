@@ -60,8 +60,12 @@ def _param(t, name, shape, device):
 
 
 def _rows(t):
-    """`t` itself if its last dimension is contiguous, a contiguous copy otherwise."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    """`t` with a contiguous last dimension (a copy only if it has none), and its strides."""
+    st = t.stride()
+    if st[-1] != 1 and t.shape[-1] != 1:
+        t = t.contiguous()
+        st = t.stride()
+    return t, st
 
 
 def _ptr(t):
@@ -70,57 +74,55 @@ def _ptr(t):
 
 # Host arrays of the C interface, as bytes: a small call spends most of its time in Python, and
 # packing takes a third of what filling a ctypes array does.
-_I64 = [struct.Struct(f"{n}q") for n in range(33)]
-
-
-def _i64(values):
-    return _I64[len(values)].pack(*values)
-
-
-def _strides(n, *tensors):
-    """The first n strides of each tensor (zeros for None)."""
-    values = []
-    for t in tensors:
-        values += (0,) * n if t is None else t.stride()[:n]
-    return _i64(values)
+_I64 = [struct.Struct(f"{n}q") for n in range(25)]
 
 
 # ------------------------------------------------------------------------ rotary positions
 def _rope_args(x, positions, inv_freq, axis_pairs, gamma, layout):
-    if x.dim() != 4 or x.dtype not in _DTYPES:
+    code = _DTYPES.get(x.dtype)
+    if x.dim() != 4 or code is None:
         raise ValueError("x must be [B, L, H, D] in float32, bfloat16 or float16")
     B, L, H, D = x.shape
-    if min(B, L, H, D) < 1 or D % 2 or D > 256 or B > 65535:
+    if D % 2 or not 0 < D <= 256 or not (B and L and H) or B > 65535:
         raise ValueError(f"unsupported shape {tuple(x.shape)}: no empty dimension, D even and up to 256")
     if layout not in _LAYOUTS:
         raise ValueError(f"layout must be 'interleaved' or 'halves', got {layout!r}")
-    pairs = [int(p) for p in axis_pairs]
-    if not 1 <= len(pairs) <= 4 or min(pairs) < 0 or sum(pairs) > D // 2:
-        raise ValueError(f"axis_pairs {pairs} must be 1 to 4 counts of at most {D // 2} pairs in all")
-    if positions.dtype not in _POSITIONS:
+    axes, total = len(axis_pairs), sum(axis_pairs)
+    if not 1 <= axes <= 4 or min(axis_pairs) < 0 or total > D // 2:
+        raise ValueError(f"axis_pairs {list(axis_pairs)} must be 1 to 4 counts of at most {D // 2} pairs in all")
+    device, kind = x.device, _POSITIONS.get(positions.dtype)
+    if kind is None:
         raise ValueError(f"positions must be int32, int64 or float32, got {positions.dtype}")
-    if tuple(positions.shape) not in ((L, len(pairs)), (B, L, len(pairs))):
+    if positions.shape == (L, axes):
+        apart = 0
+    elif positions.shape == (B, L, axes):
+        apart = L * axes
+    else:
         raise ValueError(f"positions must be [L, axes] or [B, L, axes], got {tuple(positions.shape)}")
-    if positions.device != x.device:
-        raise ValueError(f"positions must be on {x.device}")
-    inv_freq = _param(inv_freq, "inv_freq", (sum(pairs),), x.device)
-    gamma = _param(gamma, "gamma", (H, D), x.device)
-    positions = positions.contiguous()
-    how = (_DTYPES[x.dtype], _POSITIONS[positions.dtype], L * len(pairs) if positions.dim() == 3 else 0,
-           B, L, H, D, struct.pack(f"{len(pairs)}i", *pairs), len(pairs), _LAYOUTS[layout])
-    return positions, inv_freq, gamma, how
+    if positions.device != device:
+        raise ValueError(f"positions must be on {device}")
+    inv_freq = _check(inv_freq, "inv_freq", (total,), torch.float32, device).contiguous()
+    gamma = _param(gamma, "gamma", (H, D), device)
+    how = (code, kind, apart, B, L, H, D, _I32[axes].pack(*axis_pairs), axes, _LAYOUTS[layout])
+    return positions.contiguous(), inv_freq, gamma, how
+
+
+_I32 = [struct.Struct(f"{n}i") for n in range(5)]
 
 
 def _out_like(out, x, name):
-    """An output of x's shape and type: `out` if given (unit last stride), a new one otherwise."""
+    """An output of x's shape and type, and its strides: `out` if given (unit last stride), a new one
+    otherwise."""
     if out is None:
-        return x.new_empty(x.shape)
+        out = x.new_empty(x.shape)
+        return out, out.stride()
     _check(out, name, x.shape, x.dtype, x.device)
-    if out.stride(-1) != 1 and out.shape[-1] != 1:
+    st = out.stride()
+    if st[-1] != 1 and out.shape[-1] != 1:
         raise ValueError(f"{name} needs a contiguous last dimension")
-    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+    if any(n > 1 and s == 0 for n, s in zip(out.shape, st)):
         raise ValueError(f"{name} must not be expanded")
-    return out
+    return out, st
 
 
 def axis_rope(x, positions, inv_freq, *, axis_pairs, gamma=None, layout="interleaved", out=None):
@@ -131,12 +133,12 @@ def axis_rope(x, positions, inv_freq, *, axis_pairs, gamma=None, layout="interle
     or (p, P+p) ("halves").  With ``gamma`` [H, D] the rotated vector r becomes
     r * sqrt(D) / max(|r|, 1e-12) * gamma.  ``out`` may be x itself."""
     positions, inv_freq, gamma, how = _rope_args(x, positions, inv_freq, axis_pairs, gamma, layout)
-    x = _rows(x)
-    y = _out_like(out, x, "out")
+    x, xs = _rows(x)
+    y, ys = _out_like(out, x, "out")
     lib = _lib(x.device)
     _ok(lib, lib.triposplat_b200_axis_rope(
         x.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), _ptr(gamma), y.data_ptr(),
-        _strides(3, x, y), *how), "axis_rope")
+        _I64[6].pack(*xs[:3], *ys[:3]), *how), "axis_rope")
     return y
 
 
@@ -145,16 +147,16 @@ def axis_rope_backward(dy, x, positions, inv_freq, *, axis_pairs, gamma=None, la
     """Gradients (dx, dgamma) of ``axis_rope`` at x (read only with ``gamma``; dgamma is None
     without).  ``out`` receives dx and may be dy itself."""
     positions, inv_freq, gamma, how = _rope_args(dy, positions, inv_freq, axis_pairs, gamma, layout)
-    dy = _rows(dy)
+    dy, ds = _rows(dy)
+    dx, gs = _out_like(out, dy, "out")
+    px, xs, dgamma = None, (0, 0, 0), None
     if gamma is not None:
-        x = _rows(_check(x, "x", dy.shape, dy.dtype, dy.device))
-    dx = _out_like(out, dy, "out")
-    dgamma = None if gamma is None else torch.empty_like(gamma)
+        x, xs = _rows(_check(x, "x", dy.shape, dy.dtype, dy.device))
+        px, dgamma = x.data_ptr(), torch.empty_like(gamma)
     lib = _lib(dy.device)
     _ok(lib, lib.triposplat_b200_axis_rope_backward(
-        dy.data_ptr(), x.data_ptr() if gamma is not None else None, positions.data_ptr(),
-        inv_freq.data_ptr(), _ptr(gamma), dx.data_ptr(), _ptr(dgamma),
-        _strides(3, dy, x if gamma is not None else None, dx), *how), "axis_rope_backward")
+        dy.data_ptr(), px, positions.data_ptr(), inv_freq.data_ptr(), _ptr(gamma), dx.data_ptr(), _ptr(dgamma),
+        _I64[9].pack(*ds[:3], *xs[:3], *gs[:3]), *how), "axis_rope_backward")
     return dx, dgamma
 
 
@@ -163,7 +165,7 @@ def _norm_args(x, y, gate, scale, shift, pre, pre_weight, post, post_weight):
     if x.dim() != 3 or x.dtype not in _DTYPES:
         raise ValueError("x must be [B, L, C] in float32, bfloat16 or float16")
     B, L, C = x.shape
-    if min(B, L, C) < 1 or C > 8192 or B > 65535:
+    if not (B and L and C) or C > 8192 or B > 65535:
         raise ValueError(f"unsupported shape {tuple(x.shape)}: no empty dimension, C up to 8192")
     if pre not in _KINDS or post not in _KINDS:
         raise ValueError("pre and post must be 'layer', 'rms' or None")
@@ -190,14 +192,14 @@ def norm_gate(x, y, *, gate=None, scale=None, shift=None, pre="layer", pre_weigh
     shift are [B, C], the weights [C], all float32 and optional.  Returns (z, h, stats); stats
     [B, L, 4] goes to the backward pass."""
     gate, scale, shift, wpre, wpost = _norm_args(x, y, gate, scale, shift, pre, pre_weight, post, post_weight)
-    x, y = _rows(x), _rows(y)
+    (x, xs), (y, ys) = _rows(x), _rows(y)
     B, L, C = x.shape
     z = x.new_empty((B, L, C))
     h = x.new_empty((B, L, C)) if pre is not None else None
-    stats = x.new_empty((B, L, 4), dtype=torch.float32)
+    stats = torch.empty((B, L, 4), dtype=torch.float32, device=x.device)
     lib = _lib(x.device)
     _ok(lib, lib.triposplat_b200_norm_gate(
-        x.data_ptr(), y.data_ptr(), _strides(2, x, y), _ptr(gate), _ptr(scale), _ptr(shift),
+        x.data_ptr(), y.data_ptr(), _I64[4].pack(*xs[:2], *ys[:2]), _ptr(gate), _ptr(scale), _ptr(shift),
         _ptr(wpre), _ptr(wpost), z.data_ptr(), _ptr(h), stats.data_ptr(), _DTYPES[x.dtype], B, L, C, _KINDS[pre],
         _KINDS[post], float(residual_scale), float(eps)), "norm_gate")
     return z, h, stats
@@ -212,9 +214,12 @@ def norm_gate_backward(dz, dh, x, y, stats, *, gate=None, scale=None, shift=None
         raise ValueError("at least one of dz and dh is needed")
     if dh is not None and pre is None:
         raise ValueError("dh needs a pre norm")
-    dz, dh = (None if t is None else _rows(_check(t, n, x.shape, x.dtype, x.device))
-              for t, n in ((dz, "dz"), (dh, "dh")))
-    x, y = _rows(x), _rows(y)
+    zs = hs = (0, 0)
+    if dz is not None:
+        dz, zs = _rows(_check(dz, "dz", x.shape, x.dtype, x.device))
+    if dh is not None:
+        dh, hs = _rows(_check(dh, "dh", x.shape, x.dtype, x.device))
+    (x, xs), (y, ys) = _rows(x), _rows(y)
     B, L, C = x.shape
     stats = _check(stats, "stats", (B, L, 4), torch.float32, x.device).contiguous()
     g = {"x": x.new_empty((B, L, C)), "y": x.new_empty((B, L, C))}
@@ -223,7 +228,8 @@ def norm_gate_backward(dz, dh, x, y, stats, *, gate=None, scale=None, shift=None
         g[name] = None if t is None else torch.empty_like(t)
     lib = _lib(x.device)
     _ok(lib, lib.triposplat_b200_norm_gate_backward(
-        _ptr(dz), _ptr(dh), x.data_ptr(), y.data_ptr(), _strides(2, x, y, dz, dh), stats.data_ptr(), _ptr(gate), _ptr(scale),
+        _ptr(dz), _ptr(dh), x.data_ptr(), y.data_ptr(), _I64[8].pack(*xs[:2], *ys[:2], *zs[:2], *hs[:2]),
+        stats.data_ptr(), _ptr(gate), _ptr(scale),
         _ptr(wpre), _ptr(wpost), g["x"].data_ptr(), g["y"].data_ptr(), _ptr(g["gate"]), _ptr(g["scale"]),
         _ptr(g["shift"]), _ptr(g["pre_weight"]), _ptr(g["post_weight"]), _DTYPES[x.dtype], B, L, C, _KINDS[pre],
         _KINDS[post], float(residual_scale)), "norm_gate_backward")
@@ -232,23 +238,27 @@ def norm_gate_backward(dz, dh, x, y, stats, *, gate=None, scale=None, shift=None
 
 # --------------------------------------------------------------------------------- attention
 def _attention_args(q, k, v, key_bias):
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+    if q.dim() != 4 or k.dim() != 4:
         raise ValueError("q, k, v must be [B, H, L, 64]")
     B, H, Lq, D = q.shape
-    Lk = k.shape[2]
-    if D != 64 or min(B, H, Lq, Lk) < 1:
+    Lk, dev = k.shape[2], q.device
+    if D != 64 or not (B and H and Lq and Lk):
         raise ValueError(f"unsupported shapes {tuple(q.shape)}, {tuple(k.shape)}: head_dim 64, no empty dimension")
-    _check(q, "q", (B, H, Lq, 64), torch.float32, q.device)
-    _check(k, "k", (B, H, Lk, 64), torch.float32, q.device)
-    _check(v, "v", (B, H, Lk, 64), torch.float32, q.device)
-    bias_dims = (1, 1)
-    if key_bias is not None:
-        shape = tuple(key_bias.shape)
-        if shape not in ((Lk,), (B, Lk), (B, H, Lk)):
-            raise ValueError(f"key_bias must be [Lk], [B, Lk] or [B, H, Lk], got {shape}")
-        key_bias = _param(key_bias, "key_bias", shape, q.device)
-        bias_dims = ((1, 1), (B, 1), (B, H))[len(shape) - 1]
-    return key_bias, bias_dims, (B, H, Lq, Lk)
+    _check(q, "q", q.shape, torch.float32, dev)
+    _check(k, "k", (B, H, Lk, 64), torch.float32, dev)
+    _check(v, "v", k.shape, torch.float32, dev)
+    if key_bias is None:
+        return None, 1, 1, B, H, Lq, Lk
+    shape = key_bias.shape
+    if shape not in ((Lk,), (B, Lk), (B, H, Lk)):
+        raise ValueError(f"key_bias must be [Lk], [B, Lk] or [B, H, Lk], got {tuple(shape)}")
+    return (_param(key_bias, "key_bias", shape, dev), B if len(shape) > 1 else 1, H if len(shape) > 2 else 1,
+            B, H, Lq, Lk)
+
+
+def _token_major(like, B, H, L):
+    """A new [B, H, L, 64] in token-major storage [B, L, H, 64]."""
+    return like.new_empty_strided((B, H, L, 64), (L * H * 64, 64, H * 64, 1))
 
 
 def attention_forward(q, k, v, *, key_bias=None):
@@ -257,15 +267,15 @@ def attention_forward(q, k, v, *, key_bias=None):
     gives zeros.  Returns (out, stats): out [B, H, Lq, 64] in token-major storage
     ([B, Lq, H, 64], what the out-projection reads), stats [B, H, Lq + 1, 2] for the backward pass.
     Heads shared by several queries' heads are passed expanded."""
-    key_bias, bias_dims, (B, H, Lq, Lk) = _attention_args(q, k, v, key_bias)
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    out = q.new_empty((B, Lq, H, 64))
+    key_bias, bias_b, bias_h, B, H, Lq, Lk = _attention_args(q, k, v, key_bias)
+    (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
+    out = _token_major(q, B, H, Lq)
     stats = q.new_empty((B, H, Lq + 1, 2))
     lib = _lib(q.device)
     _ok(lib, lib.triposplat_b200_attention_forward(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(3, q, k, v),
-        _ptr(key_bias), *bias_dims, out.data_ptr(), stats.data_ptr(), B, H, Lq, Lk), "attention_forward")
-    return out.transpose(1, 2), stats
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _I64[9].pack(*qs[:3], *ks[:3], *vs[:3]), _ptr(key_bias), bias_b,
+        bias_h, out.data_ptr(), stats.data_ptr(), B, H, Lq, Lk), "attention_forward")
+    return out, stats
 
 
 def attention_backward(dout, q, k, v, out, stats, *, key_bias=None, grads=None, bias_grad=True):
@@ -274,22 +284,24 @@ def attention_backward(dout, q, k, v, out, stats, *, key_bias=None, grads=None, 
     ``grads`` may name the three tensors to write (e.g. slices of a packed gradient); otherwise they
     are new, in token-major storage.  dbias has key_bias's shape (None without a bias or with
     ``bias_grad=False``)."""
-    key_bias, bias_dims, (B, H, Lq, Lk) = _attention_args(q, k, v, key_bias)
+    key_bias, bias_b, bias_h, B, H, Lq, Lk = _attention_args(q, k, v, key_bias)
     dev = q.device
-    dout = _rows(_check(dout, "dout", q.shape, torch.float32, dev))
-    out = _rows(_check(out, "out", q.shape, torch.float32, dev))
+    dout, gs = _rows(_check(dout, "dout", q.shape, torch.float32, dev))
+    out, os = _rows(_check(out, "out", q.shape, torch.float32, dev))
     stats = _check(stats, "stats", (B, H, Lq + 1, 2), torch.float32, dev).contiguous()
-    q, k, v = _rows(q), _rows(k), _rows(v)
+    (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
     if grads is None:
-        dq, dk, dv = (q.new_empty((B, n, H, 64)).transpose(1, 2) for n in (Lq, Lk, Lk))
+        dq, dk, dv = _token_major(q, B, H, Lq), _token_major(k, B, H, Lk), _token_major(v, B, H, Lk)
+        dqs, dks, dvs = dq.stride(), dk.stride(), dv.stride()
     else:
-        dq, dk, dv = (_out_like(g, like, "grads") for g, like in zip(grads, (q, k, v), strict=True))
+        (dq, dqs), (dk, dks), (dv, dvs) = (_out_like(g, like, "grads") for g, like in zip(grads, (q, k, v), strict=True))
     dbias = torch.empty_like(key_bias) if key_bias is not None and bias_grad else None
+    strides = _I64[24].pack(*gs[:3], *qs[:3], *ks[:3], *vs[:3], *os[:3], *dqs[:3], *dks[:3], *dvs[:3])
     lib = _lib(dev)
     _ok(lib, lib.triposplat_b200_attention_backward(
-        dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), stats.data_ptr(),
-        _strides(3, dout, q, k, v, out, dq, dk, dv), _ptr(key_bias), *bias_dims,
-        dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dbias), B, H, Lq, Lk), "attention_backward")
+        dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), stats.data_ptr(), strides,
+        _ptr(key_bias), bias_b, bias_h, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dbias), B, H, Lq, Lk),
+        "attention_backward")
     return dq, dk, dv, dbias
 
 
