@@ -647,6 +647,7 @@ __global__ void __launch_bounds__(256) bias_rows_k(Bias bias, int H, float* __re
   const int bh = blockIdx.x, b = bh / H, h = bh - b * H;
   const float* src = bias.row(b, h);
   float mx = -INFINITY;
+#pragma unroll 8
   for (int j = threadIdx.x; j < bias.L; j += 256) mx = fmaxf(mx, src[j]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -665,17 +666,20 @@ struct Rows {
   __device__ __forceinline__ const float* at(int ib, int ih, int64_t il) const { return p + ib * b + ih * h + il * l; }
 };
 
-// 16 consecutive values
-__device__ __forceinline__ void load16(const float* p, bool vec, float (&v)[16]) {
+// Four lanes share a 64-dimensional row: lane q has columns col16(q, 0..15), four runs of four, 16
+// columns apart, so that one access of the four lanes covers 64 bytes side by side.
+__device__ __forceinline__ int col16(int q, int e) { return (e >> 2) * 16 + q * 4 + (e & 3); }
+
+__device__ __forceinline__ void load16(const float* row, int q, bool vec, float (&v)[16]) {
   if (vec) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float4 f = *reinterpret_cast<const float4*>(p + 4 * k);
+      const float4 f = *reinterpret_cast<const float4*>(row + col16(q, 4 * k));
       v[4 * k] = f.x; v[4 * k + 1] = f.y; v[4 * k + 2] = f.z; v[4 * k + 3] = f.w;
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) v[k] = p[k];
+    for (int k = 0; k < 16; ++k) v[k] = row[col16(q, k)];
   }
 }
 
@@ -686,20 +690,24 @@ __device__ __forceinline__ float absmax16(const float (&v)[16]) {
   return m;
 }
 
-__device__ __forceinline__ void store_split16(const float (&v)[16], float up, __half* hi, __half* lo) {
-  __align__(16) __half2 h[8], l[8];
+// hi / lo planes of four consecutive values times a power of two
+__device__ __forceinline__ void store_split4(const float* v, float up, __half* hi, __half* lo) {
+  __align__(8) __half2 h[2], l[2];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
+  for (int k = 0; k < 2; ++k) {
     const float a = v[2 * k] * up, b = v[2 * k + 1] * up;
     h[k] = __floats2half2_rn(a, b);
     const float2 f = __half22float2(h[k]);
     l[k] = __floats2half2_rn(a - f.x, b - f.y);
   }
+  *reinterpret_cast<uint2*>(hi) = *reinterpret_cast<const uint2*>(h);
+  *reinterpret_cast<uint2*>(lo) = *reinterpret_cast<const uint2*>(l);
+}
+
+// ... of a lane's 16 columns of a row
+__device__ __forceinline__ void store_split16(const float (&v)[16], int q, float up, __half* hi, __half* lo) {
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    reinterpret_cast<uint4*>(hi)[k] = reinterpret_cast<const uint4*>(h)[k];
-    reinterpret_cast<uint4*>(lo)[k] = reinterpret_cast<const uint4*>(l)[k];
-  }
+  for (int k = 0; k < 4; ++k) store_split4(v + 4 * k, up, hi + col16(q, 4 * k), lo + col16(q, 4 * k));
 }
 
 // largest of four values over a block of 256 threads
@@ -730,7 +738,7 @@ __global__ void __launch_bounds__(256) bwd_split_k(Rows q, Rows dout, Rows out, 
                                                    const float2* __restrict__ stats, int64_t stats_ld, int H, int vec,
                                                    Side qs, Side ks, int* next) {
   __shared__ float4 sm[8];
-  const int bh = blockIdx.x, b = bh / H, h = bh - b * H, c0 = (threadIdx.x & 3) * 16;
+  const int bh = blockIdx.x, b = bh / H, h = bh - b * H, lq = threadIdx.x & 3;
   const int key_tiles = ks.Lt / HELD;
   if (bh == 0 && blockIdx.y == 0 && threadIdx.x == 0) *next = 0;  // the main kernel's item counter
   const bool keys = (int)blockIdx.y < key_tiles;
@@ -746,8 +754,8 @@ __global__ void __launch_bounds__(256) bwd_split_k(Rows q, Rows dout, Rows out, 
       for (int e = 0; e < 16; ++e) x[u][e] = y[u][e] = 0.0f;
       if (row < s.L) col[u] = bias.p ? relative_bias(bias.row(b, h)[row], mx) * LOG2E : 0.0f;
       if (col[u] != -INFINITY) {
-        load16(k.at(b, h, row) + c0, vec, x[u]);
-        load16(v.at(b, h, row) + c0, vec, y[u]);
+        load16(k.at(b, h, row), lq, vec, x[u]);
+        load16(v.at(b, h, row), lq, vec, y[u]);
       }
     }
   } else {
@@ -759,9 +767,9 @@ __global__ void __launch_bounds__(256) bwd_split_k(Rows q, Rows dout, Rows out, 
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[u][e] = y[u][e] = ov[e] = 0.0f;
       if (row < s.L) {
-        load16(q.at(b, h, row) + c0, vec, x[u]);
-        load16(dout.at(b, h, row) + c0, vec, y[u]);
-        load16(out.at(b, h, row) + c0, vec, ov);
+        load16(q.at(b, h, row), lq, vec, x[u]);
+        load16(dout.at(b, h, row), lq, vec, y[u]);
+        load16(out.at(b, h, row), lq, vec, ov);
         ml = stats[bh * stats_ld + row];
       }
       const bool any = ml.y != 0.0f;  // a row without a key gives nothing, whatever dO holds
@@ -799,8 +807,8 @@ __global__ void __launch_bounds__(256) bwd_split_k(Rows q, Rows dout, Rows out, 
       s.col[prow] = col[u];
       if (!keys) s.delta[prow] = -delta[u];
     }
-    store_split16(x[u], pow2i(s1), s.hi1 + prow * D + c0, s.lo1 + prow * D + c0);
-    store_split16(y[u], pow2i(s2), s.hi2 + prow * D + c0, s.lo2 + prow * D + c0);
+    store_split16(x[u], lq, pow2i(s1), s.hi1 + prow * D, s.lo1 + prow * D);
+    store_split16(y[u], lq, pow2i(s2), s.hi2 + prow * D, s.lo2 + prow * D);
   }
 }
 
@@ -812,7 +820,7 @@ __global__ void __launch_bounds__(256) fwd_split_k(Rows q, Rows k, Rows v, Bias 
                                                    int H, int Lq, int Lk, int vec, SplitPlanesSdpa sp) {
   __shared__ float vt[KT][D + 1];
   __shared__ float4 sm[8];
-  const int bh = blockIdx.x, b = bh / H, h = bh - b * H, c0 = (threadIdx.x & 3) * 16;
+  const int bh = blockIdx.x, b = bh / H, h = bh - b * H, lq = threadIdx.x & 3;
   float x[2][16];
   if ((int)blockIdx.y >= sp.T) {
     const int row0 = (blockIdx.y - sp.T) * KT + (threadIdx.x >> 2);
@@ -823,7 +831,7 @@ __global__ void __launch_bounds__(256) fwd_split_k(Rows q, Rows k, Rows v, Bias 
     for (int u = 0; u < 2; ++u) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[u][e] = 0.0f;
-      if (row0 + 64 * u < Lq) load16(q.at(b, h, row0 + 64 * u) + c0, vec, x[u]);
+      if (row0 + 64 * u < Lq) load16(q.at(b, h, row0 + 64 * u), lq, vec, x[u]);
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -833,7 +841,7 @@ __global__ void __launch_bounds__(256) fwd_split_k(Rows q, Rows k, Rows v, Bias 
       if (row0 + 64 * u >= Lq) continue;
       const int s = scale_shift(mx);
       const int64_t prow = (int64_t)bh * Lq + row0 + 64 * u;
-      store_split16(x[u], pow2i(s), sp.qhi + prow * D + c0, sp.qlo + prow * D + c0);
+      store_split16(x[u], lq, pow2i(s), sp.qhi + prow * D, sp.qlo + prow * D);
       if ((threadIdx.x & 3) == 0) sp.qinv[prow] = pow2i(-s) * weight;
     }
     return;
@@ -847,11 +855,11 @@ __global__ void __launch_bounds__(256) fwd_split_k(Rows q, Rows k, Rows v, Bias 
 #pragma unroll
     for (int e = 0; e < 16; ++e) x[u][e] = y[e] = 0.0f;
     if (row < Lk && !(bias.p && bias.row(b, h)[row] == -INFINITY)) {
-      load16(k.at(b, h, row) + c0, vec, x[u]);
-      load16(v.at(b, h, row) + c0, vec, y);
+      load16(k.at(b, h, row), lq, vec, x[u]);
+      load16(v.at(b, h, row), lq, vec, y);
     }
 #pragma unroll
-    for (int e = 0; e < 16; ++e) vt[j][c0 + e] = y[e];
+    for (int e = 0; e < 16; ++e) vt[j][col16(lq, e)] = y[e];
     kmx = fmaxf(kmx, absmax16(x[u]));
     vmx = fmaxf(vmx, absmax16(y));
   }
@@ -864,15 +872,20 @@ __global__ void __launch_bounds__(256) fwd_split_k(Rows q, Rows k, Rows v, Bias 
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int64_t prow = (int64_t)bh * sp.Lkt + row0 + u * 64;
-    store_split16(x[u], pow2i(sk), sp.khi + prow * D + c0, sp.klo + prow * D + c0);
+    store_split16(x[u], lq, pow2i(sk), sp.khi + prow * D, sp.klo + prow * D);
   }
-  for (int e = threadIdx.x; e < D * (KT / 16); e += 256) {
-    const int d = e % D, jb = e / D * 16;
-    float y[16];
+  // a warp per row of V^T: two keys per lane, 128 bytes side by side
+  for (int d = threadIdx.x >> 5; d < D; d += 8) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) y[i] = vt[jb + i][d];
-    const int64_t off = ((int64_t)bh * D + d) * sp.Lkt + tile * KT + jb;
-    store_split16(y, pow2i(sv), sp.vhi + off, sp.vlo + off);
+    for (int u = 0; u < 2; ++u) {
+      const int j = 64 * u + 2 * (threadIdx.x & 31);
+      const float a0 = vt[j][d] * pow2i(sv), a1 = vt[j + 1][d] * pow2i(sv);
+      const __half2 h = __floats2half2_rn(a0, a1);
+      const float2 f = __half22float2(h);
+      const int64_t off = ((int64_t)bh * D + d) * sp.Lkt + tile * KT + j;
+      *reinterpret_cast<__half2*>(sp.vhi + off) = h;
+      *reinterpret_cast<__half2*>(sp.vlo + off) = __floats2half2_rn(a0 - f.x, a1 - f.y);
+    }
   }
   if (threadIdx.x == 0) {
     sp.kinv[(int64_t)bh * sp.T + tile] = pow2i(-sk);
@@ -880,19 +893,24 @@ __global__ void __launch_bounds__(256) fwd_split_k(Rows q, Rows k, Rows v, Bias 
   }
 }
 
-// Gradients of a pass whose walk was cut: its shares' partial sums [cuts, BH, Lt, 64] added in their
-// order, a thread per element.
+// Gradients of a pass whose walk was cut: its shares' partial sums [cuts, BH, Lt, 64] added.  A block
+// takes 32 elements of a row, eight threads each: thread y adds shares y, y + 8, ..., then the eight sums
+// are added in order.
 __global__ void __launch_bounds__(256) join_k(const float* __restrict__ part, int cuts, int H, int BH, int L, int Lt,
                                               float* __restrict__ out, int64_t sb, int64_t sh, int64_t sl) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (int64_t)BH * L * D) return;
-  const int d = (int)(i % D);
-  const int64_t row = i / D % L;
-  const int bh = (int)(i / D / L), b = bh / H, h = bh - b * H;
+  __shared__ float sm[8][32];
+  const int d = (blockIdx.x & 1) * 32 + threadIdx.x, y = threadIdx.y;
+  const int64_t i = blockIdx.x >> 1, row = i % L;
+  const int bh = (int)(i / L), b = bh / H, h = bh - b * H;
   const float* src = part + ((int64_t)bh * Lt + row) * D + d;
   float s = 0.0f;
-#pragma unroll 16
-  for (int c = 0; c < cuts; ++c) s += src[(int64_t)c * BH * Lt * D];
+#pragma unroll 8
+  for (int c = y; c < cuts; c += 8) s += src[(int64_t)c * BH * Lt * D];
+  sm[y][threadIdx.x] = s;
+  __syncthreads();
+  if (y != 0) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) s += sm[k][threadIdx.x];
   out[b * sb + h * sh + row * sl + d] = s;
 }
 
@@ -1180,7 +1198,7 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
   const Bias bias{key_bias, bias_batches, bias_heads, Lk};
   auto join = [&](const float* part, int cuts, int L, int Lt, float* dst, const int64_t* g) {
     LaunchScope scope(kKSdpaSplit, stream);
-    join_k<<<(unsigned)((BH * L * D + 255) / 256), 256, 0, stream>>>(part, cuts, H, (int)BH, L, Lt, dst, g[0], g[1], g[2]);
+    join_k<<<(unsigned)(BH * L * 2), dim3(32, 8), 0, stream>>>(part, cuts, H, (int)BH, L, Lt, dst, g[0], g[1], g[2]);
   };
   auto bias_grad = [&](const float* part, int parts, int Lt) {
     LaunchScope scope(kKSdpaSplit, stream);

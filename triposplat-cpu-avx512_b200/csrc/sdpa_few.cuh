@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(kFewThreads) few_fwd_k(const FewArgs a) {
   __shared__ float qs[NQ][D];
   __shared__ float sm_m[kFewThreads / 32][NQ], sm_l[kFewThreads / 32][NQ], sm_o[kFewThreads / 32][NQ][D];
   const int bh = blockIdx.y, b = bh / a.H, h = bh - b * a.H;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = (lane & 3) * 16;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lq = lane & 3;
   float2 head = make_float2(0.0f, 1.0f);
   if (a.bias.p) head = a.head[bh * a.head_stride];
   for (int i = threadIdx.x; i < NQ * D; i += kFewThreads) {
@@ -73,14 +73,14 @@ __global__ void __launch_bounds__(kFewThreads) few_fwd_k(const FewArgs a) {
     for (int e = 0; e < 16; ++e) kv[e] = vv[e] = 0.0f;
     if (j < j1) off = a.bias.p ? relative_bias(a.bias.row(b, h)[j], head.x) * LOG2E : 0.0f;
     if (off != -INFINITY) {
-      load16(a.k.at(b, h, j) + c0, a.vec, kv);
-      load16(a.v.at(b, h, j) + c0, a.vec, vv);
+      load16(a.k.at(b, h, j), lq, a.vec, kv);
+      load16(a.v.at(b, h, j), lq, a.vec, vv);
     }
 #pragma unroll
     for (int r = 0; r < NQ; ++r) {
       float s = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s = fmaf(qs[r][c0 + e], kv[e], s);
+      for (int e = 0; e < 16; ++e) s = fmaf(qs[r][col16(lq, e)], kv[e], s);
       s = sum_key(s) + off;
       if (s > m[r] + 8.0f) {  // the same in the key's four lanes
         const float up = ceilf(s), f = ex2(m[r] - up);  // 0 from -inf
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kFewThreads) few_fwd_k(const FewArgs a) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const float v = sum_groups(o[r][e] * f);
-      if (lane < 4) sm_o[warp][r][c0 + e] = v;
+      if (lane < 4) sm_o[warp][r][col16(lq, e)] = v;
     }
     if (lane == 0) {
       sm_m[warp][r] = top;
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kFewThreads) few_bwd_k(const FewArgs a) {
   __shared__ float qs[NQ][D], gs[NQ][D], sm_m[NQ], sm_d[NQ];
   __shared__ float sm_q[kFewThreads / 32][NQ][D];
   const int bh = blockIdx.y, b = bh / a.H, h = bh - b * a.H;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = (lane & 3) * 16;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lq = lane & 3;
   const float2 head = a.bias.p ? a.head[bh * a.head_stride] : make_float2(0.0f, 1.0f);
   const float c = 0.125f * LOG2E * head.y;
   static_assert(NQ <= kFewThreads / 32, "a warp per row");
@@ -189,16 +189,16 @@ __global__ void __launch_bounds__(kFewThreads) few_bwd_k(const FewArgs a) {
     for (int e = 0; e < 16; ++e) kv[e] = vv[e] = dk[e] = dv[e] = 0.0f;
     if (j < j1) off = a.bias.p ? relative_bias(a.bias.row(b, h)[j], head.x) * LOG2E : 0.0f;
     if (off != -INFINITY) {
-      load16(a.k.at(b, h, j) + c0, a.vec, kv);
-      load16(a.v.at(b, h, j) + c0, a.vec, vv);
+      load16(a.k.at(b, h, j), lq, a.vec, kv);
+      load16(a.v.at(b, h, j), lq, a.vec, vv);
     }
 #pragma unroll
     for (int r = 0; r < NQ; ++r) {
       float s = 0.0f, dp = 0.0f;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        s = fmaf(qs[r][c0 + e], kv[e], s);
-        dp = fmaf(gs[r][c0 + e], vv[e], dp);
+        s = fmaf(qs[r][col16(lq, e)], kv[e], s);
+        dp = fmaf(gs[r][col16(lq, e)], vv[e], dp);
       }
       s = sum_key(s);
       dp = sum_key(dp);
@@ -206,27 +206,27 @@ __global__ void __launch_bounds__(kFewThreads) few_bwd_k(const FewArgs a) {
       db += ds;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        dk[e] = fmaf(ds, qs[r][c0 + e], dk[e]);
-        dv[e] = fmaf(w, gs[r][c0 + e], dv[e]);
+        dk[e] = fmaf(ds, qs[r][col16(lq, e)], dk[e]);
+        dv[e] = fmaf(w, gs[r][col16(lq, e)], dv[e]);
         dq[r][e] = fmaf(ds, kv[e], dq[r][e]);
       }
     }
     if (j < j1) {
-      float* pk = a.dk + b * a.kb + h * a.kh + j * a.kl + c0;
-      float* pv = a.dv + b * a.vb + h * a.vh + j * a.vl + c0;
+      float* pk = a.dk + b * a.kb + h * a.kh + j * a.kl;
+      float* pv = a.dv + b * a.vb + h * a.vh + j * a.vl;
 #pragma unroll
       for (int e = 0; e < 16; ++e) dk[e] *= 0.125f;
       if (a.vec_out) {
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
-          *reinterpret_cast<float4*>(pk + e) = make_float4(dk[e], dk[e + 1], dk[e + 2], dk[e + 3]);
-          *reinterpret_cast<float4*>(pv + e) = make_float4(dv[e], dv[e + 1], dv[e + 2], dv[e + 3]);
+          *reinterpret_cast<float4*>(pk + col16(lq, e)) = make_float4(dk[e], dk[e + 1], dk[e + 2], dk[e + 3]);
+          *reinterpret_cast<float4*>(pv + col16(lq, e)) = make_float4(dv[e], dv[e + 1], dv[e + 2], dv[e + 3]);
         }
       } else {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          pk[e] = dk[e];
-          pv[e] = dv[e];
+          pk[col16(lq, e)] = dk[e];
+          pv[col16(lq, e)] = dv[e];
         }
       }
       if (a.db && (lane & 3) == 0) a.db[(int64_t)bh * a.Lk + j] = db;
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kFewThreads) few_bwd_k(const FewArgs a) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const float v = sum_groups(dq[r][e]);
-      if (lane < 4) sm_q[warp][r][c0 + e] = v;
+      if (lane < 4) sm_q[warp][r][col16(lq, e)] = v;
     }
   __syncthreads();
   for (int i = threadIdx.x; i < NQ * D; i += kFewThreads) {
