@@ -683,10 +683,15 @@ __device__ __forceinline__ void load16(const float* row, int q, bool vec, float 
   }
 }
 
+// largest finite magnitude: a scale is shared by the rows of a tile, and one that is not finite is
+// none of the others' business
 __device__ __forceinline__ float absmax16(const float (&v)[16]) {
   float m = 0.0f;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) m = fmaxf(m, fabsf(v[k]));
+  for (int k = 0; k < 16; ++k) {
+    const float a = fabsf(v[k]);
+    m = a <= 3.402823466e38f ? fmaxf(m, a) : m;
+  }
   return m;
 }
 
@@ -782,18 +787,22 @@ __global__ void __launch_bounds__(256) bwd_split_k(Rows q, Rows dout, Rows out, 
       }
     }
   }
-  float4 mx = make_float4(fmaxf(absmax16(x[0]), absmax16(x[1])), fmaxf(absmax16(y[0]), absmax16(y[1])), 0.0f, 0.0f);
+  const float top[2] = {absmax16(y[0]), absmax16(y[1])};
+  float4 mx = make_float4(fmaxf(absmax16(x[0]), absmax16(x[1])), fmaxf(top[0], top[1]), 0.0f, 0.0f);
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
+    float all = top[u];
 #pragma unroll
     for (int e = 0; e < 16; ++e) sq[u] = fmaf(y[u][e], y[u][e], sq[u]);
 #pragma unroll
     for (int i = 1; i < 4; i <<= 1) {
       sq[u] += __shfl_xor_sync(0xffffffffu, sq[u], i);
       delta[u] += __shfl_xor_sync(0xffffffffu, delta[u], i);
+      all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, i));
     }
-    mx.z = fmaxf(mx.z, sqrtf(sq[u]));
-    mx.w = fmaxf(mx.w, fabsf(delta[u]));
+    // the row's norm, or sqrt(64) times its largest element where the squares leave the type's range
+    mx.z = fmaxf(mx.z, sq[u] >= 0x1p-100f && sq[u] <= 0x1p120f ? sqrtf(sq[u]) : 8.0f * all);
+    if (fabsf(delta[u]) <= 3.402823466e38f) mx.w = fmaxf(mx.w, fabsf(delta[u]));
   }
   mx = block_max4(mx, sm);
   const int s1 = scale_shift(mx.x), s2 = scale_shift(mx.y);
