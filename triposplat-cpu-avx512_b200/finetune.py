@@ -12,6 +12,7 @@ velocity; its parameters are the blocks' adaLN tables, per-head gains and post-n
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 import _native
 import train_ops
@@ -36,6 +37,7 @@ class _Attention(torch.autograd.Function):
         return out.transpose(1, 2)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         qkv, gamma, positions, inv_freq, key_bias, qk, out, stats = ctx.saved_tensors
         B, L, _, H, _ = qkv.shape
@@ -62,6 +64,7 @@ class _NormGate(torch.autograd.Function):
         return z, h
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dz, dh):
         x, y, stats, gate, scale, shift, pre_weight, post_weight = ctx.saved_tensors
         if dz is None and dh is None:
@@ -81,6 +84,7 @@ class _FrozenLinear(torch.autograd.Function):
         return nf24_linear(x, p.code01, p.q2, p.scale, p.bias)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         lin = ctx.lin
         return nf24_linear(dy * lin.packed.scale, lin.code01_nk, lin.q2_nk, lin.ones, lin.zeros), None
