@@ -197,13 +197,14 @@ __global__ void __launch_bounds__(MAXT, 1) norm_gate_k(const Args a) {
     x += dx;
   };
   constexpr bool kAhead = NI * VEC <= 8;
-  if (kAhead && g < a.L) fetch();
+  const int64_t first = g < a.groups ? g : a.L;  // a block of several groups may hold more than there are
+  if (kAhead && first < a.L) fetch();
   float gw[NI][VEC], sw[NI][VEC], sh[NI][VEC];
   load_coef<VEC, NI>(a.wpost, a.gate ? a.gate + b * a.C : nullptr, a.gate ? 0.0f : 1.0f, a.C, gw);
   load_coef<VEC, NI>(a.wpre, a.scale ? a.scale + b * a.C : nullptr, 1.0f, a.C, sw);
   load_coef<VEC, NI>(nullptr, a.shift ? a.shift + b * a.C : nullptr, 0.0f, a.C, sh);
 #pragma unroll 1
-  for (int64_t l = g; l < a.L; l += a.groups) {
+  for (int64_t l = first; l < a.L; l += a.groups) {
     const int64_t r = b * a.L + l;
     float z[NI][VEC], m[NI][VEC];
     if (!kAhead) fetch();
@@ -263,7 +264,8 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 && VEC == 1 ? 2 : 1) norm_ga
     stats += a.groups;
   };
   constexpr bool kAhead = NI * VEC <= 8;
-  if (kAhead && g < a.L) fetch();
+  const int64_t first = g < a.groups ? g : a.L;  // a block of several groups may hold more than there are
+  if (kAhead && first < a.L) fetch();
   float gw[NI][VEC], sw[NI][VEC];
   load_coef<VEC, NI>(a.wpost, a.gate ? a.gate + b * a.C : nullptr, a.gate ? 0.0f : 1.0f, a.C, gw);
   load_coef<VEC, NI>(a.wpre, a.scale ? a.scale + b * a.C : nullptr, 1.0f, a.C, sw);
@@ -276,7 +278,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 && VEC == 1 ? 2 : 1) norm_ga
       gw[i][e] *= a.rho;
     }
 #pragma unroll 1
-  for (int64_t l = g; l < a.L; l += a.groups) {
+  for (int64_t l = first; l < a.L; l += a.groups) {
     const int64_t r = b * a.L + l;
     float n[NI][VEC], m[NI][VEC], d[NI][VEC], dzv[NI][VEC];
     if (!kAhead) fetch();
