@@ -116,10 +116,11 @@ struct Params {
   // training only: per row (final reference maximum, row sum) for the backward pass
   float2* stats;
   int64_t stats_ld;  // rows of stats per (b, h)
-  // a row's keys cut into `cuts` work items of T tiles each (the last may reach past the Tk tiles there
-  // are: those read as zeros and are masked), outputs and statistics cut_out / cut_stats apart
+  // a row's keys cut into `cuts` work items of T tiles each (the last ends with the Tk tiles there are),
+  // outputs and statistics cut_out / cut_stats apart
   int Tk, cuts;
   int64_t cut_out, cut_stats;
+  const int2* tiles;  // nullable, [BH]: first tile with a key and the one past the last; the others are left out
 };
 
 // 2^s for |s| <= 126 built in the exponent field: x * pow2i(s) is the correctly rounded
@@ -414,21 +415,33 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const int T = p.T;
   // persistent CTAs: work item j = blockIdx.x + i * gridDim.x (query tiles of one head
   // consecutive, so CTAs running together share the head's K / V in L2); every role walks
-  // the same items, and stages / barrier phases run on the global tile counter G = i*T + t
+  // the same items, and stages / barrier phases run on the global tile counter G (i*T + t, or
+  // with items of different lengths g0 + t)
   const int items = TRAIN ? p.Qt * p.BH * p.cuts : p.Qt * p.BH;
   const int Tk = TRAIN ? p.Tk : T;
   const int my_items = (int)blockIdx.x < items ? (items - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
-  // head, first query row, first key tile of work item i
-  auto item_of = [&](int i, int& bh, int& q0, int& t0) {
+  // work item i: head, first query row, key tiles [t0, t0 + n), share of the keys
+  auto item_of = [&](int i, int& bh, int& q0, int& t0, int& n, int& cut) {
     int j = blockIdx.x + i * gridDim.x;
     t0 = 0;
+    n = T;
+    cut = 0;
     if (TRAIN) {
-      const int c = j % p.cuts;
+      cut = j % p.cuts;
       j /= p.cuts;
-      t0 = c * T;
     }
     bh = j / p.Qt;
     q0 = (j - bh * p.Qt) * BQ;
+    if (TRAIN) {
+      t0 = cut * T;
+      int end = min(t0 + T, Tk);
+      if (p.tiles) {
+        const int2 r = __ldg(p.tiles + bh);
+        t0 = max(t0, r.x);
+        end = min(end, r.y);
+      }
+      n = max(end - t0, 0);
+    }
   };
 
   if (threadIdx.x == 0) {
@@ -474,9 +487,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       int issued[2] = {-1, -1};
       int q_issued = -1;
       bool ok = true;
+      int g0 = 0;
       for (int i = 0; i < my_items && ok; ++i) {
-        int bh, q0, t0;
-        item_of(i, bh, q0, t0);
+        int bh, q0, t0, nt, cut;
+        item_of(i, bh, q0, t0, nt, cut);
+        if (!TRAIN) g0 = i * T;
         if (is_k) {
           // the item's Q tile, once the previous item's QK MMAs have read the old one
           // (rows past Lq read as zeros)
@@ -486,8 +501,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           tma_load_3d(q_s + PLANE, &tm_qlo, q_full, 0, q0, bh);
           q_issued = i;
         }
-        for (int t = 0; t < T; ++t) {
-          const int G = i * T + t, st = G & 1;
+        for (int t = 0; t < nt; ++t) {
+          const int G = g0 + t, st = G & 1;
           if (G >= 2 && !mbar_wait(&empty[st], ((G >> 1) & 1) ^ 1, p.status, kDevTimeoutProducer, abort_flag)) {
             ok = false;
             break;
@@ -505,6 +520,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           }
           issued[st] = G;
         }
+        g0 += nt;
       }
       if (*abort_flag) {
         // never leave the CTA while a bulk copy may still write its shared memory
@@ -522,10 +538,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       constexpr uint32_t idesc_s = idesc_f16_f32(BQ, BKV);
       bool ok = true;
       const uint32_t qh = smem_u32(q_s), ql = qh + PLANE;
+      int g0 = 0;
       for (int i = 0; i < my_items && ok; ++i) {
+      int nt = T;
+      if (TRAIN) {
+        int bh, q0, t0, cut;
+        item_of(i, bh, q0, t0, nt, cut);
+      } else {
+        g0 = i * T;
+      }
       ok = mbar_wait(q_full, i & 1, p.status, kDevTimeoutMma, abort_flag);
-      for (int t = 0; t < T && ok; ++t) {
-        const int G = i * T + t, st = G & 1, sb = G % NSB;
+      for (int t = 0; t < nt && ok; ++t) {
+        const int G = g0 + t, st = G & 1, sb = G % NSB;
         ok = mbar_wait(&k_full[st], (G >> 1) & 1, p.status, kDevTimeoutMma, abort_flag) &&
              (G < NSB || mbar_wait(&pv_done[sb], ((G - NSB) / NSB) & 1, p.status, kDevTimeoutMma, abort_flag));
         if (!ok) break;
@@ -560,6 +584,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         mma_commit(&s_full[sb]);
       }
       if (ok) mma_commit(q_empty);  // this item's QK MMAs retire -> the next Q may land
+      g0 += nt;
       }
       mma_commit(qk_done);
       mbar_wait(qk_done, 0, p.status, kDevTimeoutMma, nullptr);
@@ -569,11 +594,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     if (elect_one()) {
       constexpr uint32_t idesc_o = idesc_f16_f32(BQ, D);
       bool ok = true;
-      const int nt0 = (T + 1) / 2, nt1 = T / 2;  // tiles of team 0 / team 1 per item
-      for (int i = 0; i < my_items && ok; ++i)
-      for (int t = 0; t < T && ok; ++t) {
-        const int G = i * T + t, st = G & 1, team = t & 1;
-        const int c = i * (team ? nt1 : nt0) + (t >> 1);  // the team's global tile count
+      int g0 = 0, c0 = 0, c1 = 0;  // tiles of the items so far: all, team 0's, team 1's
+      for (int i = 0; i < my_items && ok; ++i) {
+      int nt = T;
+      if (TRAIN) {
+        int bh, q0, t0, cut;
+        item_of(i, bh, q0, t0, nt, cut);
+      } else {
+        g0 = i * T;
+        c0 = i * ((T + 1) / 2);
+        c1 = i * (T / 2);
+      }
+      for (int t = 0; t < nt && ok; ++t) {
+        const int G = g0 + t, st = G & 1, team = t & 1;
+        const int c = (team ? c1 : c0) + (t >> 1);  // the team's global tile count
         ok = mbar_wait(&p_full[team], c & 1, p.status, kDevTimeoutMma, abort_flag) &&
              mbar_wait(&v_full[st], (G >> 1) & 1, p.status, kDevTimeoutMma, abort_flag);
         if (!ok) break;
@@ -608,6 +642,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         mma_commit(&v_empty[st]);
         mma_commit(&pv_done[G % NSB]);
       }
+      g0 += nt;
+      c0 += (nt + 1) / 2;
+      c1 += nt / 2;
+      }
       mma_commit(pv_all);
       mbar_wait(pv_all, 0, p.status, kDevTimeoutMma, nullptr);
     }
@@ -629,11 +667,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     constexpr int PF_V = 3;
     float pf_cq = 0.0f, pf_k0 = 0.0f, pf_v[PF_V];
     auto prefetch = [&](int i) {
-      int bh_, q0_, t0_;
-      item_of(i, bh_, q0_, t0_);
+      int bh_, q0_, t0_, nt_, cut_;
+      item_of(i, bh_, q0_, t0_, nt_, cut_);
       const int qr = q0_ + r;
       pf_cq = qr < p.Lq ? p.qinv[(int64_t)bh_ * p.Lq + qr] : 0.0f;
-      pf_k0 = team < T && (!TRAIN || t0_ + team < Tk) ? p.kinv[(int64_t)bh_ * Tk + t0_ + team] : 0.0f;
+      pf_k0 = team < nt_ ? p.kinv[(int64_t)bh_ * Tk + t0_ + team] : 0.0f;
 #pragma unroll
       for (int k = 0; k < PF_V; ++k) {
         const int t = lane + 32 * k;
@@ -641,9 +679,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       }
     };
     if (my_items > 0) prefetch(0);
+    int g0 = 0;
     for (int i = 0; i < my_items && ok; ++i) {
-    int bh, q0, t0;
-    item_of(i, bh, q0, t0);
+    int bh, q0, t0, nt, cut;
+    item_of(i, bh, q0, t0, nt, cut);
+    if (!TRAIN) g0 = i * T;
     const int qrow = q0 + r;
     const bool row_valid = qrow < p.Lq;
     const float cq = 0.125f * LOG2E * pf_cq;
@@ -659,7 +699,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     // the team's first tile's K and V scales (tile `team`: lane `team`'s first share)
     const float k0_cur = pf_k0;
     float v0_cur = __shfl_sync(0xffffffffu, pf_v[0], team);
-    if (TRAIN) v0_cur = t0 + team < Tk ? p.vinv[(int64_t)bh * Tk + t0 + team] : vref;
+    if (TRAIN) v0_cur = team < nt ? p.vinv[(int64_t)bh * Tk + t0 + team] : vref;
     // the next item's scales are requested after this item's first tile: right here the
     // previous item's output stores still fill the load / store queue
     bool pf_next = i + 1 < my_items;
@@ -669,8 +709,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
     for (int d = 0; d < D; ++d) o_acc[d] = 0.0f;
     int n = 0;  // tiles this team has processed in this item
-    for (int t = team; t < T; t += 2, ++n) {
-      const int G = i * T + t, sb = G % NSB;
+    for (int t = team; t < nt; t += 2, ++n) {
+      const int G = g0 + t, sb = G % NSB;
       const bool plain = bias_row == nullptr && (t0 + t + 1) * BKV <= p.Lk;  // no bias, no masking
       if (!plain) {
         // key bias (+ -inf past Lk) for this tile, staged in a warp-private buffer
@@ -683,7 +723,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         __syncwarp();
       }
-      const int tk = TRAIN ? min(t0 + t, Tk - 1) : t;  // tiles past the last one are masked: any scale serves
+      const int tk = t0 + t;
       const float c2 = cq * (n == 0 ? k0_cur : p.kinv[(int64_t)bh * Tk + tk]);
       // exponent offset folding this V tile's pre-scale relative to the head reference
       const float vshift =
@@ -722,7 +762,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     }
     if (ok && n > 0) {
       // the team's last O of the item
-      const int Gl = i * T + team + 2 * (n - 1);
+      const int Gl = g0 + team + 2 * (n - 1);
       ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[Gl % NSB], (Gl / NSB) & 1, p.status,
                                              kDevTimeoutEpilogue, abort_flag));
       if (ok) {
@@ -775,7 +815,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         float f = vref / l;
         if (TRAIN) {
           if (l == 0.0f) f = 0.0f;  // a row without a key is zeros
-          p.stats[(TRAIN ? t0 / T * p.cut_stats : 0) + bh * p.stats_ld + qrow] = make_float2(m, l * 0x1p-7f);  // the lift of P_LIFT taken out
+          p.stats[cut * p.cut_stats + bh * p.stats_ld + qrow] = make_float2(m, l * 0x1p-7f);  // the lift of P_LIFT taken out
         }
         // dimensions 0..31 as team 0's own (o0 f0 + o1 f1), 32..63 as team 1's own
 #pragma unroll
@@ -826,7 +866,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             *reinterpret_cast<uint2*>(p.olo + off) =
                 make_uint2(*reinterpret_cast<const uint32_t*>(&l01), *reinterpret_cast<const uint32_t*>(&l23));
           } else {
-            float* base = TRAIN ? p.out + t0 / T * p.cut_out : p.out;
+            float* base = TRAIN ? p.out + cut * p.cut_out : p.out;
             float* dst = p.out_blhd ? base + (((int64_t)b * p.Lq + qr) * p.H + hh) * D + c
                                     : base + ((int64_t)bh * p.Lq + qr) * D + c;
             *reinterpret_cast<float4*>(dst) = v;
@@ -838,6 +878,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(xfree);
     }
+    g0 += nt;
     }  // item loop
   }
 
@@ -1371,7 +1412,7 @@ static int sdpa_attend(const SplitPlanesSdpa& sp, const float* bias, int64_t bia
                        float* out, int64_t BH, int H, int Lq, int Lk, int out_blhd,
                        cudaStream_t stream, const OutSplit& osplit = OutSplit(),
                        float2* stats = nullptr, int64_t stats_ld = 0, int cuts = 1, int64_t cut_out = 0,
-                       int64_t cut_stats = 0) {
+                       int64_t cut_stats = 0, const int2* tiles = nullptr) {
   using namespace sdpa;
   CUtensorMap m_qhi, m_qlo, m_khi, m_klo, m_vhi, m_vlo;
   const uint32_t box_rows[3] = {64, 128, 1};
@@ -1423,7 +1464,7 @@ static int sdpa_attend(const SplitPlanesSdpa& sp, const float* bias, int64_t bia
   Params prm{sp.qinv, sp.kinv, sp.vinv, bias, (long long)bias_bh_stride, out, H, Lq, Lk,
              (sp.T + cuts - 1) / cuts, out_blhd,
              device_status(), Qt, (int)BH, osplit.hi, osplit.lo, osplit.rs, stats, stats_ld, sp.T, cuts,
-             cut_out, cut_stats};
+             cut_out, cut_stats, tiles};
   // persistent: one CTA per SM walking the (head, query tile) items
   static std::atomic<int> sm_count[64];
   int dev = 0;
@@ -1445,11 +1486,11 @@ static int sdpa_attend(const SplitPlanesSdpa& sp, const float* bias, int64_t bia
   return launch_status();
 }
 
-int sdpa_attend_stats(const SplitPlanesSdpa& sp, const float* bias, int64_t bias_bh_stride, float* out_blhd,
+int sdpa_attend_stats(const SplitPlanesSdpa& sp, const float* bias, int64_t bias_bh_stride, const int2* tiles, float* out_blhd,
                       float2* stats, int64_t stats_ld, int64_t BH, int H, int Lq, int Lk, int cuts, int64_t cut_out,
                       int64_t cut_stats, cudaStream_t stream) {
   return sdpa_attend(sp, bias, bias_bh_stride, out_blhd, BH, H, Lq, Lk, 1, stream, OutSplit(), stats, stats_ld, cuts,
-                     cut_out, cut_stats);
+                     cut_out, cut_stats, tiles);
 }
 
 // k/v element (bh, j, d) at base + bh*bh_stride + j*j_stride + d*d_stride

@@ -191,6 +191,7 @@ struct Params {
   Pass keys, queries;
   const float2* head;  // [BH] head_stride apart: .y = 0 where the bias leaves the scores no weight, 1 otherwise
   int64_t head_stride;
+  const int2* tiles;   // with a bias, [BH]: first 128-key tile with a key and the one past the last
   float* db;           // nullable: [cuts, 2, BH, Lt of the keys] sums of ds over each warpgroup's queries
   int H, BH;
   int key_items, items;
@@ -206,10 +207,12 @@ struct Maps {
 // Work item j: the pass with the longer items first; shares of a walk next to each other, then held tiles,
 // then heads.  A CTA starts with item blockIdx.x and then takes the next one that is left, so that
 // items of different lengths fill the SMs evenly; which CTA works on an item changes no result.
+// Tiles without a key at either end (padding) are left out: held ones have nothing to walk.
 struct Item {
   bool keys;
   int bh, f0, t0, n, cut;  // head, first held row, walked tiles [t0, t0 + n)
 };
+template <bool BIAS>
 __device__ __forceinline__ Item item_of(const Params& p, int j) {
   Item it;
   const int first = p.keys_last ? p.items - p.key_items : p.key_items;
@@ -222,6 +225,16 @@ __device__ __forceinline__ Item item_of(const Params& p, int j) {
   it.f0 = (j - it.bh * s.Ft) * HELD;
   it.t0 = it.cut * s.span;
   it.n = min(s.span, s.T - it.t0);
+  if (BIAS) {
+    const int2 r = __ldg(p.tiles + it.bh);
+    if (it.keys) {
+      if (it.f0 < r.x * HELD || it.f0 >= r.y * HELD) it.n = 0;
+    } else {
+      const int end = min(it.t0 + it.n, r.y * (HELD / WALK));
+      it.t0 = max(it.t0, r.x * (HELD / WALK));
+      it.n = max(end - it.t0, 0);
+    }
+  }
   return it;
 }
 
@@ -356,7 +369,7 @@ __device__ __forceinline__ bool mma_item(const Params& p, int n, const Shared& s
     mma_commit(&sh.xy_full[g_ & 1]);
     return true;
   };
-  if (!form_xy(G)) return false;
+  if (n > 0 && !form_xy(G)) return false;
   for (int t = 0; t < n; ++t, ++G) {
     const int st = G % kStages;
     if (t + 1 < n && !form_xy(G + 1)) return false;
@@ -491,7 +504,7 @@ __device__ __forceinline__ bool compute_item(const Params& p, const Pass& ps, co
       db = fmaf(d0 + d1, down, db);
     }
   }
-  if (!fold()) return false;
+  if (it.n > 0 && !fold()) return false;
   // ---- the held rows' gradients ----
   const bool first = !KEYS || w == 1;  // out1 (dK, dQ) or out2 (dV)
   float* dst = first ? ps.out1 : ps.out2;
@@ -570,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_bwd_tc(const __grid_constant
           sh.items[i & 1] = j;
           mbar_arrive(&sh.item_full[i & 1]);
           if (j >= p.items) break;
-          const Item it = item_of(p, j);
+          const Item it = item_of<BIAS>(p, j);
           ok = it.keys ? load_item<true>(p, p.keys, it, &m.q1h, &m.q1l, &m.q2h, &m.q2l, sh, G)
                        : load_item<false>(p, p.queries, it, &m.k1h, &m.k1l, &m.k2h, &m.k2l, sh, G);
         }
@@ -586,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_bwd_tc(const __grid_constant
           const int j = sh.items[i & 1];
           mbar_arrive(&sh.item_empty[i & 1]);
           if (j >= p.items) break;
-          const Item it = item_of(p, j);
+          const Item it = item_of<BIAS>(p, j);
           ok = mbar_wait(sh.held_full, i & 1, p.status, kDevTimeoutMma, sh.abort_flag);
           if (!ok) break;
           tc_fence_after();
@@ -605,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_bwd_tc(const __grid_constant
       __syncwarp();
       if (lane_id() == 0) mbar_arrive(&sh.item_empty[i & 1]);
       if (j >= p.items) break;
-      const Item it = item_of(p, j);
+      const Item it = item_of<BIAS>(p, j);
       ok = it.keys ? compute_item<true, BIAS>(p, p.keys, it, sh, tmem, G, P)
                    : compute_item<false, BIAS>(p, p.queries, it, sh, tmem, G, P);
     }
@@ -639,25 +652,51 @@ struct Bias {
   }
 };
 
+// The first 128-key tile of a bias row with a key and the one past the last; (0, 0) without any.  A block
+// of 256 threads; lo, hi: of the keys that the thread has seen.
+__device__ __forceinline__ int2 tile_range(int lo, int hi, int2* sm) {
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = make_int2(lo, hi);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    lo = min(lo, sm[k].x);
+    hi = max(hi, sm[k].y);
+  }
+  return hi < 0 ? make_int2(0, 0) : make_int2(lo / HELD, hi / HELD + 1);
+}
+
 // One block per (b, h): the row's largest bias, where it leaves the scores weight (head = 0 beyond
 // 2^60 in magnitude), both behind the statistics for the backward pass, and (out not null) the
-// relative bias.
-__global__ void __launch_bounds__(256) bias_rows_k(Bias bias, int H, float* __restrict__ out, float2* head, int64_t head_stride) {
+// relative bias and the range of tiles with a key.
+__global__ void __launch_bounds__(256) bias_rows_k(Bias bias, int H, float* __restrict__ out, int2* __restrict__ tiles,
+                                                   float2* head, int64_t head_stride) {
   __shared__ float sm[8];
+  __shared__ int2 sm_range[8];
   const int bh = blockIdx.x, b = bh / H, h = bh - b * H;
   const float* src = bias.row(b, h);
   float mx = -INFINITY;
+  int lo = 0x7fffffff, hi = -1;
 #pragma unroll 8
-  for (int j = threadIdx.x; j < bias.L; j += 256) mx = fmaxf(mx, src[j]);
+  for (int j = threadIdx.x; j < bias.L; j += 256) {
+    const float v = src[j];
+    mx = fmaxf(mx, v);
+    if (v != -INFINITY) {
+      lo = min(lo, j);
+      hi = j;
+    }
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = mx;
-  __syncthreads();
+  const int2 range = tile_range(lo, hi, sm_range);  // also orders sm
 #pragma unroll
   for (int k = 0; k < 8; ++k) mx = fmaxf(mx, sm[k]);
   if (threadIdx.x == 0) head[bh * head_stride] = make_float2(mx, mx > -INFINITY && fabsf(mx) > 0x1p60f ? 0.0f : 1.0f);
-  if (out)
-    for (int j = threadIdx.x; j < bias.L; j += 256) out[(int64_t)bh * bias.L + j] = relative_bias(src[j], mx);
+  if (!out) return;
+  if (threadIdx.x == 0) tiles[bh] = range;
+  for (int j = threadIdx.x; j < bias.L; j += 256) out[(int64_t)bh * bias.L + j] = relative_bias(src[j], mx);
 }
 
 struct Rows {
@@ -738,15 +777,29 @@ __device__ __forceinline__ float4 block_max4(float4 v, float4* sm) {
 // The planes, vectors and scales of both sides of the backward pass.  One block per (b h, 128-row
 // tile), the keys' tiles first; a thread has a quarter of rows j and j + 64.  Keys: K and V, rows with
 // a bias of -inf as zeros, the relative bias in log2 units (-inf past the end).  Queries: Q and
-// g = dO / l, 7 - m, -delta.
+// g = dO / l, 7 - m, -delta; the first of them also finds the head's range of tiles with a key.
 __global__ void __launch_bounds__(256) bwd_split_k(Rows q, Rows dout, Rows out, Rows k, Rows v, Bias bias,
                                                    const float2* __restrict__ stats, int64_t stats_ld, int H, int vec,
-                                                   Side qs, Side ks, int* next) {
+                                                   Side qs, Side ks, int* next, int2* __restrict__ tiles) {
   __shared__ float4 sm[8];
+  __shared__ int2 sm_range[8];
   const int bh = blockIdx.x, b = bh / H, h = bh - b * H, lq = threadIdx.x & 3;
   const int key_tiles = ks.Lt / HELD;
   if (bh == 0 && blockIdx.y == 0 && threadIdx.x == 0) *next = 0;  // the main kernel's item counter
   const bool keys = (int)blockIdx.y < key_tiles;
+  if (bias.p && (int)blockIdx.y == key_tiles) {
+    const float* src = bias.row(b, h);
+    int lo = 0x7fffffff, hi = -1;
+#pragma unroll 8
+    for (int j = threadIdx.x; j < ks.L; j += 256) {
+      if (src[j] != -INFINITY) {
+        lo = min(lo, j);
+        hi = j;
+      }
+    }
+    const int2 range = tile_range(lo, hi, sm_range);
+    if (threadIdx.x == 0) tiles[bh] = range;
+  }
   const Side& s = keys ? ks : qs;
   const int row0 = (keys ? blockIdx.y : blockIdx.y - key_tiles) * HELD + (threadIdx.x >> 2);
   float x[2][16], y[2][16], sq[2] = {0.0f, 0.0f}, delta[2] = {0.0f, 0.0f}, col[2] = {-INFINITY, -INFINITY};
@@ -1120,9 +1173,9 @@ int triposplat_b200_attention_forward(const float* q, const float* k, const floa
   float2* rows = reinterpret_cast<float2*>(stats);
   const Bias bias{key_bias, bias_batches, bias_heads, Lk};
   const int vec = rows16({q, k, v}, strides, 3);
-  auto bias_rows = [&](float* relative) {
+  auto bias_rows = [&](float* relative, int2* tiles) {
     LaunchScope scope(kKSdpaSplit, stream);
-    bias_rows_k<<<(unsigned)BH, 256, 0, stream>>>(bias, H, relative, rows + Lq, Lq + 1);
+    bias_rows_k<<<(unsigned)BH, 256, 0, stream>>>(bias, H, relative, tiles, rows + Lq, Lq + 1);
   };
   auto join = [&](const float* o, const float2* part, int cuts, int64_t cut_o, int64_t cut_st, int64_t st_ld, int by_head,
                   int last) {
@@ -1149,7 +1202,7 @@ int triposplat_b200_attention_forward(const float* q, const float* k, const floa
       a.o = reinterpret_cast<float*>(ws);
       a.stats_out = reinterpret_cast<float2*>(ws + obytes);
     }
-    if (key_bias) bias_rows(nullptr);
+    if (key_bias) bias_rows(nullptr, nullptr);
     few_fwd(a, stream);
     if (a.shares > 1) join(a.o, a.stats_out, a.shares, BH * Lq * D, BH * Lq, Lq, 1, key_bias == nullptr);
     return launch_status();
@@ -1158,7 +1211,8 @@ int triposplat_b200_attention_forward(const float* q, const float* k, const floa
   const int Qt = (Lq + KT - 1) / KT, T = (Lk + KT - 1) / KT;
   const int64_t fit = sm_count() / (Qt * BH);
   const int cuts = fit < 2 || T < 4 ? 1 : (int)(fit < T / 2 ? fit : T / 2);
-  const size_t bias_bytes = key_bias ? al256((size_t)BH * Lk * 4) : 0;
+  const size_t row_bytes = key_bias ? al256((size_t)BH * Lk * 4) : 0;
+  const size_t bias_bytes = key_bias ? row_bytes + al256((size_t)BH * sizeof(int2)) : 0;
   const size_t part_bytes = cuts > 1 ? al256((size_t)cuts * BH * Lq * D * 4) : 0;
   SplitPlanesSdpa sp;
   void* behind = nullptr;
@@ -1166,9 +1220,10 @@ int triposplat_b200_attention_forward(const float* q, const float* k, const floa
                          &behind);
   if (st != kOk) return st;
   float* relative = key_bias ? static_cast<float*>(behind) : nullptr;
+  int2* tiles = key_bias ? reinterpret_cast<int2*>(static_cast<uint8_t*>(behind) + row_bytes) : nullptr;
   float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(behind) + bias_bytes);
   float2* part_st = reinterpret_cast<float2*>(static_cast<uint8_t*>(behind) + bias_bytes + part_bytes);
-  if (key_bias) bias_rows(relative);
+  if (key_bias) bias_rows(relative, tiles);
   {
     LaunchScope scope(kKSdpaSplit, stream);
     fwd_split_k<<<dim3((unsigned)BH, sp.T + Qt), 256, 0, stream>>>(rows_of(q, strides), rows_of(k, strides + 3),
@@ -1176,8 +1231,9 @@ int triposplat_b200_attention_forward(const float* q, const float* k, const floa
                                                                 Lk, vec, sp);
   }
   if ((st = launch_status()) != kOk) return st;
-  if (cuts == 1) return sdpa_attend_stats(sp, relative, Lk, out_blhd, rows, Lq + 1, BH, H, Lq, Lk, 1, 0, 0, stream);
-  st = sdpa_attend_stats(sp, relative, Lk, part, part_st, Lq, BH, H, Lq, Lk, cuts, BH * Lq * D, BH * Lq, stream);
+  if (cuts == 1)
+    return sdpa_attend_stats(sp, relative, Lk, tiles, out_blhd, rows, Lq + 1, BH, H, Lq, Lk, 1, 0, 0, stream);
+  st = sdpa_attend_stats(sp, relative, Lk, tiles, part, part_st, Lq, BH, H, Lq, Lk, cuts, BH * Lq * D, BH * Lq, stream);
   if (st != kOk) return st;
   join(part, part_st, cuts, BH * Lq * D, BH * Lq, Lq, 0, 0);
   return launch_status();
@@ -1250,7 +1306,8 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
   const size_t kpart = p.keys.cuts > 1 ? al256((size_t)p.keys.cuts * BH * ks.Lt * D * 4) : 0;
   const size_t qpart = p.queries.cuts > 1 ? al256((size_t)p.queries.cuts * BH * qs.Lt * D * 4) : 0;
   const size_t db_bytes = dbias ? al256((size_t)2 * p.keys.cuts * BH * ks.Lt * 4) : 0;
-  uint8_t* ws = static_cast<uint8_t*>(workspace(qbytes + kbytes + 2 * kpart + qpart + db_bytes + 256, stream));
+  const size_t tile_bytes = key_bias ? al256((size_t)BH * sizeof(int2)) : 0;
+  uint8_t* ws = static_cast<uint8_t*>(workspace(qbytes + kbytes + 2 * kpart + qpart + db_bytes + tile_bytes + 256, stream));
   if (!ws) return kWorkspace;
   side_layout(ws, BH, Lq, true, qs);
   side_layout(ws + qbytes, BH, Lk, false, ks);
@@ -1268,7 +1325,9 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
   p.queries.s1b = go[0]; p.queries.s1h = go[1]; p.queries.s1l = go[2];
   p.queries.vec_out = vec_out;
   p.db = dbias ? reinterpret_cast<float*>(at + 2 * kpart + qpart) : nullptr;
-  p.next = reinterpret_cast<int*>(at + 2 * kpart + qpart + db_bytes);
+  int2* tiles = key_bias ? reinterpret_cast<int2*>(at + 2 * kpart + qpart + db_bytes) : nullptr;
+  p.tiles = tiles;
+  p.next = reinterpret_cast<int*>(at + 2 * kpart + qpart + db_bytes + tile_bytes);
   p.keys_last = 4 * (p.keys.span + 4) < 3 * (p.queries.span + 4);
   p.head = rows + Lq;
   p.head_stride = Lq + 1;
@@ -1287,7 +1346,7 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
     LaunchScope scope(kKSdpaSplit, stream);
     bwd_split_k<<<dim3((unsigned)BH, (ks.Lt + qs.Lt) / HELD), 256, 0, stream>>>(
         rows_of(q, strides + 3), rows_of(dout, strides), rows_of(out, strides + 12), rows_of(k, strides + 6),
-        rows_of(v, strides + 9), bias, rows, Lq + 1, H, vec, qs, ks, p.next);
+        rows_of(v, strides + 9), bias, rows, Lq + 1, H, vec, qs, ks, p.next, tiles);
   }
   {
     LaunchScope scope(kKSdpaAttn, stream);
