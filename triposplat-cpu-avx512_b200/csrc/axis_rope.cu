@@ -120,6 +120,7 @@ __global__ void __launch_bounds__(kThreads, K > 1 ? 1 : 2) axis_rope_k(const Arg
   constexpr int U = tokens_at_once<BWD, K>();
   // [chunk tokens][VEC][D / 2 / VEC]: the lanes of a vector read neighbouring entries
   extern __shared__ float2 cs[];
+  if (BWD) grid_release();
   const int half = a.D / 2, step_tokens = a.token_groups * U, chunk_tokens = step_tokens * a.steps;
   const int lane = threadIdx.x & (a.lanes - 1), group = threadIdx.x / a.lanes;
   const int tg = group / a.heads, h = blockIdx.y * a.heads + group - tg * a.heads;
@@ -281,6 +282,8 @@ __global__ void __launch_bounds__(kThreads, K > 1 ? 1 : 2) axis_rope_k(const Arg
 __global__ void __launch_bounds__(1024) column_sum_k(const float* __restrict__ part, int64_t rows, int cols,
                                                      float* __restrict__ out) {
   __shared__ float sm[32][33];
+  grid_release();
+  grid_wait();
   const int c = blockIdx.x * 32 + threadIdx.x, y = threadIdx.y;
   float s = 0.0f;
   if (c < cols) {
@@ -454,7 +457,7 @@ int triposplat_b200_axis_rope_backward(const void* dy, const void* x, const void
   rope::launch<true>(a, plan, dtype, stream);
   if (dgamma) {
     LaunchScope scope(kKElementwise, stream);
-    rope::column_sum_k<<<(H * D + 31) / 32, dim3(32, 32), 0, stream>>>(a.part, rows, H * D, dgamma);
+    launch_chained(rope::column_sum_k, dim3((H * D + 31) / 32), dim3(32, 32), 0, stream, a.part, rows, H * D, dgamma);
   }
   return launch_status();
 }

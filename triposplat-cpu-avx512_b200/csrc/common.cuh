@@ -11,6 +11,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <utility>
+
 namespace tsb {
 
 // ---------------------------------------------------------------------------
@@ -70,6 +72,28 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
+}
+
+// Chained launches: a kernel launched with launch_chained may start while the one before it on the
+// stream still runs (its own start, and on the host the launch, then cost nothing), once every block of that
+// one has passed grid_release or ended.  grid_wait holds it until that one has ended and its writes are
+// seen: before the first access to anything an earlier kernel of the stream reads or writes, in every block.
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <class... P, class... A>
+inline void launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A&&... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);  // an error stays for launch_status
 }
 
 __device__ __forceinline__ void fence_barrier_init() {

@@ -108,6 +108,8 @@ __device__ __forceinline__ void chunk_scale(const T* p, T* o, int n, float c) {
 
 template <int N>
 __global__ void __launch_bounds__(kThreads) square_sum_k(const __grid_constant__ Table<N> t, double* part) {
+  grid_release();
+  grid_wait();
   double acc = 0.0;
   for (int64_t u = blockIdx.x; u < t.first[t.n]; u += gridDim.x) {
     const Chunk c = chunk_of(t, u);
@@ -124,6 +126,8 @@ __global__ void __launch_bounds__(kThreads) square_sum_k(const __grid_constant__
 template <int N>
 __global__ void __launch_bounds__(kThreads) scale_k(const __grid_constant__ Table<N> t, const double* part,
                                                     int parts, float max_norm, float* norm) {
+  grid_release();
+  grid_wait();
   double s = 0.0;
   for (int i = threadIdx.x; i < parts; i += kThreads) s += part[i];
   const float total = (float)sqrt(block_sum(s));
@@ -162,7 +166,8 @@ static void launch(const void* const* grads, void* const* outs, const int64_t* s
     ++t.n;
   }
   LaunchScope scope(kKElementwise, stream);
-  if (scale) scale_k<N><<<blocks, kThreads, 0, stream>>>(t, part, parts, max_norm, norm);
+  if (scale) launch_chained(scale_k<N>, dim3(blocks), dim3(kThreads), 0, stream, t, part, parts, max_norm, norm);
+  else if (from > 0) launch_chained(square_sum_k<N>, dim3(blocks), dim3(kThreads), 0, stream, t, part);
   else square_sum_k<N><<<blocks, kThreads, 0, stream>>>(t, part);
 }
 

@@ -235,6 +235,7 @@ __global__ void __launch_bounds__(MAXT, 1) norm_gate_k(const Args a) {
 template <class T, int VEC, int NI, int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT == 256 && VEC == 1 ? 2 : 1) norm_gate_bwd_k(const Args a) {
   __shared__ __align__(16) float2 sm[2][16];
+  grid_release();
   RowSum sum(sm);
   const int64_t b = blockIdx.y, g = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const float inv_c = 1.0f / (float)a.C;
@@ -375,6 +376,8 @@ struct ReduceArgs {
 __global__ void __launch_bounds__(1024) norm_gate_reduce_k(const ReduceArgs a) {
   constexpr int NB = 4;
   __shared__ float sm[NB][32][33];
+  grid_release();
+  grid_wait();
   const int c = blockIdx.x * 32 + threadIdx.x, y = threadIdx.y, q = blockIdx.y;
   float dw = 0.0f;
   for (int b0 = 0; b0 < a.B; b0 += NB) {
@@ -587,7 +590,7 @@ int triposplat_b200_norm_gate_backward(const void* dz, const void* dh, const voi
     const ng::ReduceArgs ra{a.part, gate, scale, pre_weight, post_weight, dgate, dscale, dshift, dpre_weight,
                             dpost_weight, B, C, a.groups, residual_scale};
     LaunchScope scope(kKElementwise, stream);
-    ng::norm_gate_reduce_k<<<dim3((C + 31) / 32, 3), dim3(32, 32), 0, stream>>>(ra);
+    launch_chained(ng::norm_gate_reduce_k, dim3((C + 31) / 32, 3), dim3(32, 32), 0, stream, ra);
   }
   return launch_status();
 }

@@ -474,6 +474,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if (TRAIN) {
+    grid_release();
+    grid_wait();
+  }
 
   if (warp < 4) {
     setmaxnreg_dec<REGS_CONTROL>();
@@ -1480,7 +1484,7 @@ static int sdpa_attend(const SplitPlanesSdpa& sp, const float* bias, int64_t bia
   const dim3 grid((unsigned)(items < sms ? items : sms));
   {
     LaunchScope scope(kKSdpaAttn, stream);
-    if (stats) sdpa_fwd_tc<true><<<grid, NUM_THREADS, SMEM_BYTES, stream>>>(m_qhi, m_qlo, m_khi, m_klo, m_vhi, m_vlo, prm);
+    if (stats) launch_chained(sdpa_fwd_tc<true>, grid, NUM_THREADS, SMEM_BYTES, stream, m_qhi, m_qlo, m_khi, m_klo, m_vhi, m_vlo, prm);
     else sdpa_fwd_tc<false><<<grid, NUM_THREADS, SMEM_BYTES, stream>>>(m_qhi, m_qlo, m_khi, m_klo, m_vhi, m_vlo, prm);
   }
   return launch_status();

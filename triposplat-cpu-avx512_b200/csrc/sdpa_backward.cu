@@ -571,6 +571,8 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_bwd_tc(const __grid_constant
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *sh.tmem_slot;
+  grid_release();
+  grid_wait();
   int G = 0, P = 0;
   bool ok = true;
   if (warp < 4) {
@@ -674,6 +676,7 @@ __global__ void __launch_bounds__(256) bias_rows_k(Bias bias, int H, float* __re
                                                    float2* head, int64_t head_stride) {
   __shared__ float sm[8];
   __shared__ int2 sm_range[8];
+  grid_release();
   const int bh = blockIdx.x, b = bh / H, h = bh - b * H;
   const float* src = bias.row(b, h);
   float mx = -INFINITY;
@@ -783,6 +786,7 @@ __global__ void __launch_bounds__(256) bwd_split_k(Rows q, Rows dout, Rows out, 
                                                    Side qs, Side ks, int* next, int2* __restrict__ tiles) {
   __shared__ float4 sm[8];
   __shared__ int2 sm_range[8];
+  grid_release();
   const int bh = blockIdx.x, b = bh / H, h = bh - b * H, lq = threadIdx.x & 3;
   const int key_tiles = ks.Lt / HELD;
   if (bh == 0 && blockIdx.y == 0 && threadIdx.x == 0) *next = 0;  // the main kernel's item counter
@@ -882,6 +886,8 @@ __global__ void __launch_bounds__(256) fwd_split_k(Rows q, Rows k, Rows v, Bias 
                                                    int H, int Lq, int Lk, int vec, SplitPlanesSdpa sp) {
   __shared__ float vt[KT][D + 1];
   __shared__ float4 sm[8];
+  grid_release();
+  grid_wait();
   const int bh = blockIdx.x, b = bh / H, h = bh - b * H, lq = threadIdx.x & 3;
   float x[2][16];
   if ((int)blockIdx.y >= sp.T) {
@@ -961,6 +967,8 @@ __global__ void __launch_bounds__(256) fwd_split_k(Rows q, Rows k, Rows v, Bias 
 __global__ void __launch_bounds__(256) join_k(const float* __restrict__ part, int cuts, int H, int BH, int L, int Lt,
                                               float* __restrict__ out, int64_t sb, int64_t sh, int64_t sl) {
   __shared__ float sm[8][32];
+  grid_release();
+  grid_wait();
   const int d = (blockIdx.x & 1) * 32 + threadIdx.x, y = threadIdx.y;
   const int64_t i = blockIdx.x >> 1, row = i % L;
   const int bh = (int)(i / L), b = bh / H, h = bh - b * H;
@@ -987,6 +995,8 @@ __global__ void __launch_bounds__(256) attn_join_k(const float* __restrict__ o, 
                                                    float2* __restrict__ stats) {
   __shared__ float sm_l[8];
   __shared__ float2 sm_v[8][32];
+  grid_release();
+  grid_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t i = W == 1 ? (int64_t)blockIdx.x * 8 + warp : blockIdx.x;
   if (i >= n) return;
@@ -1031,6 +1041,8 @@ __global__ void __launch_bounds__(256) attn_join_k(const float* __restrict__ o, 
 // that share a row, in their order.
 __global__ void __launch_bounds__(256) bias_grad_k(const float* __restrict__ part, int parts, int B, int H, int bias_b,
                                                    int bias_h, int Lk, int Lt, float* __restrict__ db) {
+  grid_release();
+  grid_wait();
   const int j = blockIdx.x * 256 + threadIdx.x, row = blockIdx.y;
   if (j >= Lk) return;
   const int rb = row / bias_h, rh = row - rb * bias_h;
@@ -1181,11 +1193,11 @@ int triposplat_b200_attention_forward(const float* q, const float* k, const floa
                   int last) {
     LaunchScope scope(kKSdpaSplit, stream);
     if (cuts > 8)
-      attn_join_k<8><<<(unsigned)(BH * Lq), 256, 0, stream>>>(o, part, cuts, cut_o, cut_st, st_ld, by_head, BH * Lq, H, Lq,
-                                                            last, out_blhd, rows);
+      launch_chained(attn_join_k<8>, dim3((unsigned)(BH * Lq)), dim3(256), 0, stream, o, part, cuts, cut_o, cut_st, st_ld, by_head,
+                     BH * Lq, H, Lq, last, out_blhd, rows);
     else
-      attn_join_k<1><<<(unsigned)((BH * Lq + 7) / 8), 256, 0, stream>>>(o, part, cuts, cut_o, cut_st, st_ld, by_head,
-                                                                      BH * Lq, H, Lq, last, out_blhd, rows);
+      launch_chained(attn_join_k<1>, dim3((unsigned)((BH * Lq + 7) / 8)), dim3(256), 0, stream, o, part, cuts, cut_o, cut_st, st_ld,
+                     by_head, BH * Lq, H, Lq, last, out_blhd, rows);
   };
   if (Lq <= kFewRows) {
     FewArgs a{};
@@ -1203,7 +1215,7 @@ int triposplat_b200_attention_forward(const float* q, const float* k, const floa
       a.stats_out = reinterpret_cast<float2*>(ws + obytes);
     }
     if (key_bias) bias_rows(nullptr, nullptr);
-    few_fwd(a, stream);
+    few_fwd(a, key_bias != nullptr, stream);
     if (a.shares > 1) join(a.o, a.stats_out, a.shares, BH * Lq * D, BH * Lq, Lq, 1, key_bias == nullptr);
     return launch_status();
   }
@@ -1226,9 +1238,10 @@ int triposplat_b200_attention_forward(const float* q, const float* k, const floa
   if (key_bias) bias_rows(relative, tiles);
   {
     LaunchScope scope(kKSdpaSplit, stream);
-    fwd_split_k<<<dim3((unsigned)BH, sp.T + Qt), 256, 0, stream>>>(rows_of(q, strides), rows_of(k, strides + 3),
-                                                                rows_of(v, strides + 6), bias, rows + Lq, Lq + 1, H, Lq,
-                                                                Lk, vec, sp);
+    const dim3 grid((unsigned)BH, sp.T + Qt);
+    const Rows rq = rows_of(q, strides), rk = rows_of(k, strides + 3), rv = rows_of(v, strides + 6);
+    if (key_bias) launch_chained(fwd_split_k, grid, dim3(256), 0, stream, rq, rk, rv, bias, rows + Lq, Lq + 1, H, Lq, Lk, vec, sp);
+    else fwd_split_k<<<grid, 256, 0, stream>>>(rq, rk, rv, bias, rows + Lq, Lq + 1, H, Lq, Lk, vec, sp);
   }
   if ((st = launch_status()) != kOk) return st;
   if (cuts == 1)
@@ -1263,12 +1276,13 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
   const Bias bias{key_bias, bias_batches, bias_heads, Lk};
   auto join = [&](const float* part, int cuts, int L, int Lt, float* dst, const int64_t* g) {
     LaunchScope scope(kKSdpaSplit, stream);
-    join_k<<<(unsigned)(BH * L * 2), dim3(32, 8), 0, stream>>>(part, cuts, H, (int)BH, L, Lt, dst, g[0], g[1], g[2]);
+    launch_chained(join_k, dim3((unsigned)(BH * L * 2)), dim3(32, 8), 0, stream, part, cuts, H, (int)BH, L, Lt, dst, g[0], g[1],
+                   g[2]);
   };
   auto bias_grad = [&](const float* part, int parts, int Lt) {
     LaunchScope scope(kKSdpaSplit, stream);
-    bias_grad_k<<<dim3((Lk + 255) / 256, bias_batches * bias_heads), 256, 0, stream>>>(part, parts, B, H, bias_batches,
-                                                                                     bias_heads, Lk, Lt, dbias);
+    launch_chained(bias_grad_k, dim3((Lk + 255) / 256, bias_batches * bias_heads), dim3(256), 0, stream, part, parts, B, H,
+                   bias_batches, bias_heads, Lk, Lt, dbias);
   };
   if (Lq <= kFewRows) {
     FewArgs a{};
@@ -1351,8 +1365,7 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
   {
     LaunchScope scope(kKSdpaAttn, stream);
     const unsigned grid = (unsigned)(p.items < sm_count() ? p.items : sm_count());
-    if (key_bias) sdpa_bwd_tc<true><<<grid, kThreads, SMEM_BYTES, stream>>>(m, p);
-    else sdpa_bwd_tc<false><<<grid, kThreads, SMEM_BYTES, stream>>>(m, p);
+    launch_chained(key_bias ? sdpa_bwd_tc<true> : sdpa_bwd_tc<false>, dim3(grid), dim3(kThreads), SMEM_BYTES, stream, m, p);
   }
   if (qpart) join(p.queries.out1, p.queries.cuts, Lq, qs.Lt, dq, go);
   if (kpart) {

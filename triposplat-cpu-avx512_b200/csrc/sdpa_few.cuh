@@ -46,6 +46,8 @@ template <int NQ>
 __global__ void __launch_bounds__(kFewThreads) few_fwd_k(const FewArgs a) {
   __shared__ float qs[NQ][D];
   __shared__ float sm_m[kFewThreads / 32][NQ], sm_l[kFewThreads / 32][NQ], sm_o[kFewThreads / 32][NQ][D];
+  grid_release();
+  grid_wait();
   const int bh = blockIdx.y, b = bh / a.H, h = bh - b * a.H;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lq = lane & 3;
   float2 head = make_float2(0.0f, 1.0f);
@@ -144,6 +146,7 @@ template <int NQ>
 __global__ void __launch_bounds__(kFewThreads) few_bwd_k(const FewArgs a) {
   __shared__ float qs[NQ][D], gs[NQ][D], sm_m[NQ], sm_d[NQ];
   __shared__ float sm_q[kFewThreads / 32][NQ][D];
+  grid_release();
   const int bh = blockIdx.y, b = bh / a.H, h = bh - b * a.H;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lq = lane & 3;
   const float2 head = a.bias.p ? a.head[bh * a.head_stride] : make_float2(0.0f, 1.0f);
@@ -259,12 +262,13 @@ static void few_shares(FewArgs& a) {
   a.shares = (a.Lk + a.span - 1) / a.span;
 }
 
-static void few_fwd(const FewArgs& a, cudaStream_t stream) {
+// chained: behind the bias's rows
+static void few_fwd(const FewArgs& a, bool chained, cudaStream_t stream) {
   LaunchScope scope(kKSdpaAttn, stream);
   const dim3 grid(a.shares, a.BH);
-  if (a.Lq == 1) few_fwd_k<1><<<grid, kFewThreads, 0, stream>>>(a);
-  else if (a.Lq == 2) few_fwd_k<2><<<grid, kFewThreads, 0, stream>>>(a);
-  else few_fwd_k<4><<<grid, kFewThreads, 0, stream>>>(a);
+  auto kernel = a.Lq == 1 ? few_fwd_k<1> : (a.Lq == 2 ? few_fwd_k<2> : few_fwd_k<4>);
+  if (chained) launch_chained(kernel, grid, dim3(kFewThreads), 0, stream, a);
+  else kernel<<<grid, kFewThreads, 0, stream>>>(a);
 }
 
 static void few_bwd(const FewArgs& a, cudaStream_t stream) {
