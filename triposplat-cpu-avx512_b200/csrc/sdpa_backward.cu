@@ -961,27 +961,57 @@ __global__ void __launch_bounds__(256) fwd_split_k(Rows q, Rows k, Rows v, Bias 
   }
 }
 
-// Gradients of a pass whose walk was cut: its shares' partial sums [cuts, BH, Lt, 64] added.  A block
-// takes 32 elements of a row, eight threads each: thread y adds shares y, y + 8, ..., then the eight sums
-// are added in order.
-__global__ void __launch_bounds__(256) join_k(const float* __restrict__ part, int cuts, int H, int BH, int L, int Lt,
-                                              float* __restrict__ out, int64_t sb, int64_t sh, int64_t sl) {
-  __shared__ float sm[8][32];
+// Gradients of passes whose walks were cut: a tensor's partial sums [cuts, BH, Lt, 64] added over the shares.
+// blockIdx.y is the tensor; a thread has 4 of a row's 64 elements and every W-th share (W = 8 where there
+// are more than that: few rows), whose sums are then added in order.
+struct Join {
+  const float* part;
+  float* out;
+  int64_t sb, sh, sl;  // element strides of out
+  int cuts, L, Lt;
+};
+struct Joins {
+  Join t[3];
+  int H, BH, vec_out;
+};
+template <int W>
+__global__ void __launch_bounds__(256) join_k(const Joins a) {
+  __shared__ float4 sm[W == 1 ? 1 : 256];
   grid_release();
   grid_wait();
-  const int d = (blockIdx.x & 1) * 32 + threadIdx.x, y = threadIdx.y;
-  const int64_t i = blockIdx.x >> 1, row = i % L;
-  const int bh = (int)(i / L), b = bh / H, h = bh - b * H;
-  const float* src = part + ((int64_t)bh * Lt + row) * D + d;
-  float s = 0.0f;
-#pragma unroll 8
-  for (int c = y; c < cuts; c += 8) s += src[(int64_t)c * BH * Lt * D];
-  sm[y][threadIdx.x] = s;
-  __syncthreads();
-  if (y != 0) return;
+  const Join& t = a.t[blockIdx.y];
+  const int lane = threadIdx.x % 16, y = threadIdx.x / 16 % W;
+  const int64_t i = (int64_t)blockIdx.x * (16 / W) + threadIdx.x / (16 * W);
+  const bool here = i < (int64_t)a.BH * t.L;
+  const int64_t row = i % t.L;
+  const int bh = (int)(i / t.L), b = bh / a.H, h = bh - b * a.H;
+  const int64_t step = (int64_t)a.BH * t.Lt * (D / 4);
+  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (here) {
+    const float4* src = reinterpret_cast<const float4*>(t.part) + ((int64_t)bh * t.Lt + row) * (D / 4) + lane;
+#pragma unroll 4
+    for (int c = y; c < t.cuts; c += W) {
+      const float4 v = src[c * step];
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+  }
+  if (W > 1) {
+    sm[threadIdx.x] = s;
+    __syncthreads();
+    if (y != 0) return;
 #pragma unroll
-  for (int k = 1; k < 8; ++k) s += sm[k][threadIdx.x];
-  out[b * sb + h * sh + row * sl + d] = s;
+    for (int k = 1; k < W; ++k) {
+      const float4 v = sm[threadIdx.x + 16 * k];
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+  }
+  if (!here) return;
+  float* dst = t.out + b * t.sb + h * t.sh + row * t.sl + lane * 4;
+  if (a.vec_out) {
+    *reinterpret_cast<float4*>(dst) = s;
+  } else {
+    dst[0] = s.x; dst[1] = s.y; dst[2] = s.z; dst[3] = s.w;
+  }
 }
 
 // Shares of the keys joined: partial outputs [cuts, BH or B, Lq, ...] as normalised by their own sums,
@@ -1038,23 +1068,32 @@ __global__ void __launch_bounds__(256) attn_join_k(const float* __restrict__ o, 
 }
 
 // db [bias_b, bias_h, Lk]: part [parts, B, H, Lt] added over the parts and the batch entries and heads
-// that share a row, in their order.
+// that share a row.  32 columns per block, eight threads each: thread y adds terms y, y + 8, ..., then the
+// eight sums are added in order.
 __global__ void __launch_bounds__(256) bias_grad_k(const float* __restrict__ part, int parts, int B, int H, int bias_b,
                                                    int bias_h, int Lk, int Lt, float* __restrict__ db) {
+  __shared__ float sm[8][32];
   grid_release();
   grid_wait();
-  const int j = blockIdx.x * 256 + threadIdx.x, row = blockIdx.y;
-  if (j >= Lk) return;
+  const int j = blockIdx.x * 32 + threadIdx.x, y = threadIdx.y, row = blockIdx.y;
   const int rb = row / bias_h, rh = row - rb * bias_h;
-  const int b0 = bias_b == 1 ? 0 : rb, b1 = bias_b == 1 ? B : rb + 1;
-  const int h0 = bias_h == 1 ? 0 : rh, h1 = bias_h == 1 ? H : rh + 1;
+  const int b0 = bias_b == 1 ? 0 : rb, nb = bias_b == 1 ? B : 1;
+  const int h0 = bias_h == 1 ? 0 : rh, nh = bias_h == 1 ? H : 1;
   float s = 0.0f;
-  for (int g = 0; g < parts; ++g)
-    for (int b = b0; b < b1; ++b) {
-      const float* p = part + ((int64_t)g * B + b) * H * Lt + j;
-#pragma unroll 8
-      for (int h = h0; h < h1; ++h) s += p[(int64_t)h * Lt];
+  if (j < Lk) {
+    const float* p = part + ((int64_t)b0 * H + h0) * Lt + j;
+    const int n = parts * nb * nh;
+#pragma unroll 4
+    for (int i = y; i < n; i += 8) {
+      const int h = i % nh, gb = i / nh, b = gb % nb, g = gb / nb;
+      s += p[(((int64_t)g * B + b) * H + h) * Lt];
     }
+  }
+  sm[y][threadIdx.x] = s;
+  __syncthreads();
+  if (y != 0 || j >= Lk) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) s += sm[k][threadIdx.x];
   db[(int64_t)row * Lk + j] = s;
 }
 
@@ -1111,25 +1150,56 @@ static int ensure_kernel() {
   return kOk;
 }
 
-// Cuts a pass's walk where one item would be longer than an SM's share of both passes.  Costs in
-// products of a 64-row tile (keys' pass 4, queries' pass 3), an item's start as much as 4 tiles.
-static void cut_walks(Pass& keys, Pass& queries, int64_t BH) {
-  const int64_t sms = sm_count();
-  int64_t total = 0;
-  for (int q = 0; q < 2; ++q) {
-    const Pass& s = q ? queries : keys;
-    total += BH * s.Ft * (s.T + 4) * (q ? 3 : 4);
+// When the last of the SMs is done that take n1 items of c1 and then n2 items of c2 <= c1 one by one.
+static int64_t makespan(int64_t n1, int64_t c1, int64_t n2, int64_t c2, int64_t sms) {
+  // two groups of SMs, those with one item of the first kind more than the others
+  int64_t more = n1 % sms, less = sms - more, low = n1 / sms * c1, high = low + c1, end = more ? high : low;
+  while (n2 > 0) {
+    const bool to_low = !more || low <= high;
+    int64_t &load = to_low ? low : high, size = to_low ? less : more;
+    load += c2;
+    n2 -= size;
+    if (load > end) end = load;
   }
-  const int64_t share = (total + sms - 1) / sms;
-  for (int q = 0; q < 2; ++q) {
-    Pass& s = q ? queries : keys;
-    s.cuts = 1;
-    s.span = s.T;
-    const int64_t fair = share / (q ? 3 : 4) - 4;  // tiles
-    if (s.T <= fair || s.T < 8) continue;
-    const int64_t most = fair < 4 ? 4 : fair, cuts = (s.T + most - 1) / most;
-    s.span = (int)(((s.T + cuts - 1) / cuts + 1) / 2 * 2);
-    s.cuts = (s.T + s.span - 1) / s.span;
+  return end;
+}
+
+// Into how many shares the two passes' walks are cut (few held tiles: their items would leave SMs idle or
+// end at very different times), by the time until the last SM is done.  Costs in products of a 64-row tile,
+// some 0.38 us (keys' pass 4 per tile, queries' pass 3), an item's start as much as 4 tiles; a cut costs the
+// join of its partial sums: 8, and 1 per MB of them.  (2000 x 2000, 4 heads, uncut by this rule: 57 us; its
+// 128 + 64 items of a rule that cuts down to an SM's fair share 61 and 18 for the joins.)
+static void cut_walks(Pass& keys, Pass& queries, int64_t BH) {
+  static const int kCuts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+  const int64_t sms = sm_count();
+  Pass* s[2] = {&keys, &queries};
+  for (Pass* q : s) {
+    q->cuts = 1;
+    q->span = q->T;
+  }
+  if (BH * (keys.Ft + queries.Ft) > 8 * sms) return;
+  int64_t best = -1;
+  int span[2] = {keys.T, queries.T};
+  for (int a : kCuts) {
+    const int sk = ((keys.T + a - 1) / a + 1) / 2 * 2;
+    if (a > 1 && sk < 4) break;
+    const int64_t nk = BH * keys.Ft * (a == 1 ? 1 : (keys.T + sk - 1) / sk), ck = ((a == 1 ? keys.T : sk) + 4) * 4;
+    for (int b : kCuts) {
+      const int sq = ((queries.T + b - 1) / b + 1) / 2 * 2;
+      if (b > 1 && sq < 4) break;
+      const int64_t nq = BH * queries.Ft * (b == 1 ? 1 : (queries.T + sq - 1) / sq), cq = ((b == 1 ? queries.T : sq) + 4) * 3;
+      int64_t t = ck >= cq ? makespan(nk, ck, nq, cq, sms) : makespan(nq, cq, nk, ck, sms);
+      if (a > 1 || b > 1) t += 8 + ((a > 1 ? 2 * nk : 0) + (b > 1 ? nq : 0)) * HELD * D * 4 / (1 << 20);
+      if (best < 0 || t < best) {
+        best = t;
+        span[0] = a == 1 ? keys.T : sk;
+        span[1] = b == 1 ? queries.T : sq;
+      }
+    }
+  }
+  for (int i = 0; i < 2; ++i) {
+    s[i]->span = span[i];
+    s[i]->cuts = (s[i]->T + span[i] - 1) / span[i];
   }
 }
 
@@ -1274,14 +1344,25 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
   const int vec = rows16({dout, q, k, v, out}, strides, 5), vec_out = rows16({dq, dk, dv}, go, 3);
   const float2* rows = reinterpret_cast<const float2*>(stats);
   const Bias bias{key_bias, bias_batches, bias_heads, Lk};
-  auto join = [&](const float* part, int cuts, int L, int Lt, float* dst, const int64_t* g) {
-    LaunchScope scope(kKSdpaSplit, stream);
-    launch_chained(join_k, dim3((unsigned)(BH * L * 2)), dim3(32, 8), 0, stream, part, cuts, H, (int)BH, L, Lt, dst, g[0], g[1],
-                   g[2]);
+  Joins joins{{}, H, (int)BH, vec_out};
+  int parts = 0;
+  auto add_join = [&](const float* part, int cuts, int L, int Lt, float* dst, const int64_t* g) {
+    joins.t[parts++] = {part, dst, g[0], g[1], g[2], cuts, L, Lt};
   };
-  auto bias_grad = [&](const float* part, int parts, int Lt) {
+  auto join = [&]() {
+    if (parts == 0) return;
+    int most = 0, L = 0;
+    for (int i = 0; i < parts; ++i) {
+      most = joins.t[i].cuts > most ? joins.t[i].cuts : most;
+      L = joins.t[i].L > L ? joins.t[i].L : L;
+    }
     LaunchScope scope(kKSdpaSplit, stream);
-    launch_chained(bias_grad_k, dim3((Lk + 255) / 256, bias_batches * bias_heads), dim3(256), 0, stream, part, parts, B, H,
+    if (most > 8) launch_chained(join_k<8>, dim3((unsigned)((BH * L + 1) / 2), parts), dim3(256), 0, stream, joins);
+    else launch_chained(join_k<1>, dim3((unsigned)((BH * L + 15) / 16), parts), dim3(256), 0, stream, joins);
+  };
+  auto bias_grad = [&](const float* part, int terms, int Lt) {
+    LaunchScope scope(kKSdpaSplit, stream);
+    launch_chained(bias_grad_k, dim3((Lk + 31) / 32, bias_batches * bias_heads), dim3(32, 8), 0, stream, part, terms, B, H,
                    bias_batches, bias_heads, Lk, Lt, dbias);
   };
   if (Lq <= kFewRows) {
@@ -1301,7 +1382,8 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
     a.dq = reinterpret_cast<float*>(ws);
     a.db = dbias ? reinterpret_cast<float*>(ws + qbytes) : nullptr;
     few_bwd(a, stream);
-    join(a.dq, a.shares, Lq, Lq, dq, go);
+    add_join(a.dq, a.shares, Lq, Lq, dq, go);
+    join();
     if (dbias) bias_grad(a.db, 1, Lk);
     return launch_status();
   }
@@ -1367,11 +1449,12 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
     const unsigned grid = (unsigned)(p.items < sm_count() ? p.items : sm_count());
     launch_chained(key_bias ? sdpa_bwd_tc<true> : sdpa_bwd_tc<false>, dim3(grid), dim3(kThreads), SMEM_BYTES, stream, m, p);
   }
-  if (qpart) join(p.queries.out1, p.queries.cuts, Lq, qs.Lt, dq, go);
+  if (qpart) add_join(p.queries.out1, p.queries.cuts, Lq, qs.Lt, dq, go);
   if (kpart) {
-    join(p.keys.out1, p.keys.cuts, Lk, ks.Lt, dk, go + 3);
-    join(p.keys.out2, p.keys.cuts, Lk, ks.Lt, dv, go + 6);
+    add_join(p.keys.out1, p.keys.cuts, Lk, ks.Lt, dk, go + 3);
+    add_join(p.keys.out2, p.keys.cuts, Lk, ks.Lt, dv, go + 6);
   }
+  join();
   if (dbias) bias_grad(p.db, 2 * p.keys.cuts, ks.Lt);
   return launch_status();
 }
