@@ -73,40 +73,47 @@ __device__ __forceinline__ float2 turn_of(double pos, float f) {
 // VEC pairs of a head, as two runs of VEC elements.  Interleaved, the runs follow each other and
 // pair i is (2i, 2i + 1) of both together; in halves, pair i is element i of each run.  A single
 // pair is the same either way and uses the second form.
-template <class T, int VEC>
-struct Slot {
-  Pack<T, VEC> a, b;
-  __device__ __forceinline__ void load(const T* p, int e0, int e1) {
-    a = *reinterpret_cast<const Pack<T, VEC>*>(p + e0);
-    b = *reinterpret_cast<const Pack<T, VEC>*>(p + e1);
-  }
-  __device__ __forceinline__ void store(T* p, int e0, int e1) const {
-    *reinterpret_cast<Pack<T, VEC>*>(p + e0) = a;
-    *reinterpret_cast<Pack<T, VEC>*>(p + e1) = b;
-  }
+template <int VEC>
+struct Runs {
+  float v[2][VEC];
   template <bool HALVES>
   __device__ __forceinline__ float2 pair(int i) const {
-    if (HALVES) return make_float2(to_f32(a.v[i]), to_f32(b.v[i]));
-    const int e = 2 * i;
-    return e < VEC ? make_float2(to_f32(a.v[e]), to_f32(e + 1 < VEC ? a.v[(e + 1) % VEC] : b.v[0]))
-                   : make_float2(to_f32(b.v[e - VEC]), to_f32(b.v[(e + 1 - VEC) % VEC]));
+    if (HALVES) return make_float2(v[0][i], v[1][i]);
+    return make_float2(v[2 * i / VEC][2 * i % VEC], v[(2 * i + 1) / VEC][(2 * i + 1) % VEC]);
   }
   template <bool HALVES>
-  __device__ __forceinline__ void put(int i, float2 v) {
+  __device__ __forceinline__ void put(int i, float2 p) {
     if (HALVES) {
-      a.v[i] = from_f32<T>(v.x);
-      b.v[i] = from_f32<T>(v.y);
-      return;
-    }
-    const int e = 2 * i;
-    if (e < VEC) {
-      a.v[e] = from_f32<T>(v.x);
-      if (e + 1 < VEC) a.v[(e + 1) % VEC] = from_f32<T>(v.y);
-      else b.v[0] = from_f32<T>(v.y);
+      v[0][i] = p.x;
+      v[1][i] = p.y;
     } else {
-      b.v[e - VEC] = from_f32<T>(v.x);
-      b.v[(e + 1 - VEC) % VEC] = from_f32<T>(v.y);
+      v[2 * i / VEC][2 * i % VEC] = p.x;
+      v[(2 * i + 1) / VEC][(2 * i + 1) % VEC] = p.y;
     }
+  }
+  template <class T>
+  __device__ __forceinline__ void store(T* p, int e0, int e1) const {
+    store_vec<T, VEC>(p + e0, v[0]);
+    store_vec<T, VEC>(p + e1, v[1]);
+  }
+};
+
+// ... as they lie in memory
+template <class T, int VEC>
+struct Slot {
+  Raw<T, VEC> a, b;
+  __device__ __forceinline__ void load(const T* p, int e0, int e1) {
+    a.load(p + e0);
+    b.load(p + e1);
+  }
+  __device__ __forceinline__ Runs<VEC> get() const {
+    Runs<VEC> r;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      r.v[0][i] = a[i];
+      r.v[1][i] = b[i];
+    }
+    return r;
   }
 };
 
@@ -136,11 +143,11 @@ __global__ void __launch_bounds__(kThreads, K > 1 ? 1 : 2) axis_rope_k(const Arg
     e0[k] = apart ? p0[k] : 2 * p0[k];
     e1[k] = apart ? a.P + p0[k] : e0[k] + VEC;
     if (NORM) {
-      Slot<float, VEC> gs;
+      Runs<VEC> gs;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        gs.a.v[i] = live[k] ? __ldg(a.gamma + (int64_t)h * a.D + e0[k] + i) : 0.0f;
-        gs.b.v[i] = live[k] ? __ldg(a.gamma + (int64_t)h * a.D + e1[k] + i) : 0.0f;
+        gs.v[0][i] = live[k] ? __ldg(a.gamma + (int64_t)h * a.D + e0[k] + i) : 0.0f;
+        gs.v[1][i] = live[k] ? __ldg(a.gamma + (int64_t)h * a.D + e1[k] + i) : 0.0f;
       }
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
@@ -200,6 +207,12 @@ __global__ void __launch_bounds__(kThreads, K > 1 ? 1 : 2) axis_rope_k(const Arg
         const int t = t0 + u * a.token_groups + tg;
         const bool here = t < tokens;
         const float2* w = cs + (here ? t : 0) * half + lane;
+        Runs<VEC> xr[K], dr[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (!BWD || NORM) xr[k] = xc[u][k].get();
+          if (BWD) dr[k] = dc[u][k].get();
+        }
         float2 r[K][VEC];
         float ss = 0.0f, dot = 0.0f;
         if (!BWD || NORM) {
@@ -209,12 +222,12 @@ __global__ void __launch_bounds__(kThreads, K > 1 ? 1 : 2) axis_rope_k(const Arg
             for (int i = 0; i < VEC; ++i) {
               r[k][i] = make_float2(0.0f, 0.0f);
               if (!live[k] || !here) continue;
-              const float2 c = w[i * slots + k * a.lanes], v = xc[u][k].template pair<HALVES>(i);
+              const float2 c = w[i * slots + k * a.lanes], v = xr[k].template pair<HALVES>(i);
               r[k][i] = make_float2(v.x * c.x - v.y * c.y, v.x * c.y + v.y * c.x);
               if (NORM) {
                 ss = fmaf(r[k][i].x, r[k][i].x, fmaf(r[k][i].y, r[k][i].y, ss));
                 if (BWD) {
-                  const float2 d = dc[u][k].template pair<HALVES>(i);
+                  const float2 d = dr[k].template pair<HALVES>(i);
                   dot = fmaf(d.x * g[k][i].x, r[k][i].x, fmaf(d.y * g[k][i].y, r[k][i].y, dot));
                 }
               }
@@ -233,12 +246,12 @@ __global__ void __launch_bounds__(kThreads, K > 1 ? 1 : 2) axis_rope_k(const Arg
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           if (!live[k] || !here) continue;
-          Slot<T, VEC> o;
+          Runs<VEC> o;
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
             float2 v;
             if (BWD) {
-              const float2 d = dc[u][k].template pair<HALVES>(i), c = w[i * slots + k * a.lanes];
+              const float2 d = dr[k].template pair<HALVES>(i), c = w[i * slots + k * a.lanes];
               float2 e = d;
               if (NORM) {
                 const float2 q = r[k][i];
@@ -265,13 +278,13 @@ __global__ void __launch_bounds__(kThreads, K > 1 ? 1 : 2) axis_rope_k(const Arg
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (!live[k]) continue;
-      Slot<float, VEC> o;
+      Runs<VEC> o;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) o.template put<HALVES>(i, acc[k][i]);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        q[e0[k] + i] = o.a.v[i];
-        q[e1[k] + i] = o.b.v[i];
+        q[e0[k] + i] = o.v[0][i];
+        q[e1[k] + i] = o.v[1][i];
       }
     }
   }

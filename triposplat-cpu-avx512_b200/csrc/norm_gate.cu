@@ -134,25 +134,23 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[NI][VEC], int kind,
 // A row's elements of one tensor as they lie in memory, and as numbers (zeros past C).
 template <class T, int VEC, int NI>
 struct RawRow {
-  Pack<T, VEC> v[NI];
-  __device__ __forceinline__ void clear() {
+  Raw<T, VEC> v[NI];
+  __device__ __forceinline__ void clear() {  // all types' zero is zero bits
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[i].v[e] = from_f32<T>(0.0f);
+    for (int i = 0; i < NI; ++i) v[i].b = {};
   }
   __device__ __forceinline__ void load(const T* p, int C) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
-      if (c < C) v[i] = *reinterpret_cast<const Pack<T, VEC>*>(p + c);
+      if (c < C) v[i].load(p + c);
     }
   }
   __device__ __forceinline__ void get(float (&f)[NI][VEC]) const {
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) f[i][e] = to_f32(v[i].v[e]);
+      for (int e = 0; e < VEC; ++e) f[i][e] = v[i][e];
   }
 };
 
