@@ -27,6 +27,7 @@
 // backward kernel held to 128 registers, two blocks per SM: with 208 only one fits, 80 us).
 #include <stdint.h>
 
+#include <atomic>
 #include <initializer_list>
 
 #include "common.cuh"
@@ -102,12 +103,36 @@ struct RowSum {
   }
 };
 
+// Which columns a thread has: runs of VEC, one every blockDim.x * VEC.  Rows of an odd width start between
+// two access boundaries; there (SHIFT) a thread's runs lie on the boundaries, `shift` elements before
+// the row's own multiples, and the first and the last run of a row may be partly outside it: their bits there
+// are cleared after the load (keep), whatever the neighbouring rows hold.  Nothing of this branches but the
+// stores: a branch around what is fetched ahead, or around its use, took what the wide accesses gain.
+template <class T, int VEC, int NI, bool SHIFT>
+struct Columns {
+  int C, shift;
+  Raw<T, VEC> keep[SHIFT ? NI : 1];
+  __device__ __forceinline__ Columns(int c, int s) : C(c), shift(s) {
+    if constexpr (SHIFT) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) keep[i].mask(-at(i), C - at(i));
+    }
+  }
+  __device__ __forceinline__ int at(int i) const {
+    return (i * (int)blockDim.x + (int)threadIdx.x) * VEC - (SHIFT ? shift : 0);
+  }
+  __device__ __forceinline__ bool whole(int i) const { return (!SHIFT || at(i) >= 0) && at(i) + (SHIFT ? VEC : 1) <= C; }
+  __device__ __forceinline__ bool has(int i, int e) const {
+    return SHIFT ? (unsigned)(at(i) + e) < (unsigned)C : at(i) < C;
+  }
+};
+
 // mean (0 for rms) and r of a row held in registers; elements past C are zero and stay out of
 // the centred sum
-template <int VEC, int NI>
-__device__ __forceinline__ float2 row_stats(const float (&v)[NI][VEC], int kind, int C, float inv_c, float eps,
-                                            RowSum& sum) {
-  float mean = 0.0f;
+template <class T, int VEC, int NI, bool SHIFT>
+__device__ __forceinline__ float2 row_stats(const float (&v)[NI][VEC], int kind, const Columns<T, VEC, NI, SHIFT>& cols,
+                                            float inv_c, float eps, RowSum& sum) {
+  float mean = 0.0f, q = 0.0f;
   if (kind == kLayer) {
     float s = 0.0f;
 #pragma unroll
@@ -115,68 +140,87 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[NI][VEC], int kind,
 #pragma unroll
       for (int e = 0; e < VEC; ++e) s += v[i][e];
     mean = sum(s) * inv_c;
-  }
-  float q = 0.0f;
 #pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    // C is a multiple of VEC: a run is inside the row or not at all
-    if ((i * (int)blockDim.x + (int)threadIdx.x) * VEC < C) {
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float d = v[i][e] - mean;
+        const float d = cols.has(i, e) ? v[i][e] - mean : 0.0f;
         q = fmaf(d, d, q);
       }
-    }
+  } else {  // elements outside are zeros
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) q = fmaf(v[i][e], v[i][e], q);
   }
   return make_float2(mean, rsqrtf(fmaf(sum(q), inv_c, eps)));
 }
 
-// A row's elements of one tensor as they lie in memory, and as numbers (zeros past C).
-template <class T, int VEC, int NI>
+// A row's elements of one tensor as they lie in memory, and as numbers (zeros outside the row).  With a shift, runs
+// at a row's ends read on into its neighbours; only where that would pass the end of the tensor (`room`
+// elements behind the row's start: the last row) are they read word by word.
+template <class T, int VEC, int NI, bool SHIFT>
 struct RawRow {
   Raw<T, VEC> v[NI];
   __device__ __forceinline__ void clear() {  // all types' zero is zero bits
 #pragma unroll
     for (int i = 0; i < NI; ++i) v[i].b = {};
   }
-  __device__ __forceinline__ void load(const T* p, int C) {
+  __device__ __forceinline__ void load(const T* p, const Columns<T, VEC, NI, SHIFT>& cols, int64_t room) {
+    if constexpr (SHIFT) {
+      if (room < cols.C + VEC - 1) {  // the same in all threads of the row
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+          if (cols.at(i) < cols.C) v[i].load_first(p + cols.at(i), cols.C - cols.at(i));
+        return;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
-      if (c < C) v[i].load(p + c);
+      const int c = cols.at(i);  // where it is negative: the boundary before the row, inside the tensor
+      if (c < cols.C) v[i].load(p + c);
     }
   }
-  __device__ __forceinline__ void get(float (&f)[NI][VEC]) const {
+  __device__ __forceinline__ void get(float (&f)[NI][VEC], const Columns<T, VEC, NI, SHIFT>& cols) const {
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
+    for (int i = 0; i < NI; ++i) {
+      Raw<T, VEC> r = v[i];
+      if constexpr (SHIFT) r = r & cols.keep[i];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) f[i][e] = v[i][e];
+      for (int e = 0; e < VEC; ++e) f[i][e] = r[e];
+    }
   }
 };
 
-template <class T, int VEC, int NI>
-__device__ __forceinline__ void store_row(T* p, int C, const float (&v)[NI][VEC]) {
+template <class T, int VEC, int NI, bool SHIFT>
+__device__ __forceinline__ void store_row(T* p, const Columns<T, VEC, NI, SHIFT>& cols, const float (&v)[NI][VEC]) {
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
-    if (c < C) store_vec<T, VEC>(p + c, v[i]);
+    const int c = cols.at(i);
+    if (cols.whole(i)) store_vec<T, VEC>(p + c, v[i]);
+    else if (SHIFT && c < cols.C) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (cols.has(i, e)) p[c + e] = from_f32<T>(v[i][e]);
+    }
   }
 }
 
-// a[c] * (b[c] + add) (null: a = 1, b = 0), zeros past C
-template <int VEC, int NI>
-__device__ __forceinline__ void load_coef(const float* a, const float* b, float add, int C, float (&v)[NI][VEC]) {
+// a[c] * (b[c] + add) (null: a = 1, b = 0), zeros outside the row
+template <class T, int VEC, int NI, bool SHIFT>
+__device__ __forceinline__ void load_coef(const float* a, const float* b, float add, const Columns<T, VEC, NI, SHIFT>& cols,
+                                          float (&v)[NI][VEC]) {
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
+    const int c = cols.at(i);
 #pragma unroll
     for (int e = 0; e < VEC; ++e)
-      v[i][e] = c < C ? (a ? __ldg(a + c + e) : 1.0f) * ((b ? __ldg(b + c + e) : 0.0f) + add) : 0.0f;
+      v[i][e] = cols.has(i, e) ? (a ? __ldg(a + c + e) : 1.0f) * ((b ? __ldg(b + c + e) : 0.0f) + add) : 0.0f;
   }
 }
 
 // Row group g of batch entry blockIdx.y takes the entry's rows g, g + groups, g + 2 groups, ...
-template <class T, int VEC, int NI, int MAXT>
+template <class T, int VEC, int NI, int MAXT, bool SHIFT>
 __global__ void __launch_bounds__(MAXT, 1) norm_gate_k(const Args a) {
   __shared__ __align__(16) float2 sm[2][16];
   RowSum sum(sm);
@@ -185,52 +229,58 @@ __global__ void __launch_bounds__(MAXT, 1) norm_gate_k(const Args a) {
   const T* x = static_cast<const T*>(a.x) + b * a.xb + g * a.xl;
   const T* y = static_cast<const T*>(a.y) + b * a.yb + g * a.yl;
   const int64_t dx = a.groups * a.xl, dy = a.groups * a.yl;
-  RawRow<T, VEC, NI> ry, rx;
+  // the same shift in all tensors and all rows of the group (see launch)
+  const Columns<T, VEC, NI, SHIFT> cols(a.C, SHIFT ? (int)((b * a.xb + g * a.xl) % VEC) : 0);
+  int64_t roomx = (a.B - 1 - b) * a.xb + (a.L - 1 - g) * a.xl + a.C;
+  int64_t roomy = (a.B - 1 - b) * a.yb + (a.L - 1 - g) * a.yl + a.C;
+  RawRow<T, VEC, NI, SHIFT> ry, rx;
   ry.clear();
   rx.clear();
   auto fetch = [&]() {  // the next row of the group
-    ry.load(y, a.C);
-    rx.load(x, a.C);
+    ry.load(y, cols, roomy);
+    rx.load(x, cols, roomx);
     y += dy;
     x += dx;
+    roomy -= dy;
+    roomx -= dx;
   };
   constexpr bool kAhead = NI * VEC <= 8;
   const int64_t first = g < a.groups ? g : a.L;  // a block of several groups may hold more than there are
   if (kAhead && first < a.L) fetch();
   float gw[NI][VEC], sw[NI][VEC], sh[NI][VEC];
-  load_coef<VEC, NI>(a.wpost, a.gate ? a.gate + b * a.C : nullptr, a.gate ? 0.0f : 1.0f, a.C, gw);
-  load_coef<VEC, NI>(a.wpre, a.scale ? a.scale + b * a.C : nullptr, 1.0f, a.C, sw);
-  load_coef<VEC, NI>(nullptr, a.shift ? a.shift + b * a.C : nullptr, 0.0f, a.C, sh);
+  load_coef<T, VEC, NI, SHIFT>(a.wpost, a.gate ? a.gate + b * a.C : nullptr, a.gate ? 0.0f : 1.0f, cols, gw);
+  load_coef<T, VEC, NI, SHIFT>(a.wpre, a.scale ? a.scale + b * a.C : nullptr, 1.0f, cols, sw);
+  load_coef<T, VEC, NI, SHIFT>(nullptr, a.shift ? a.shift + b * a.C : nullptr, 0.0f, cols, sh);
 #pragma unroll 1
   for (int64_t l = first; l < a.L; l += a.groups) {
     const int64_t r = b * a.L + l;
     float z[NI][VEC], m[NI][VEC];
     if (!kAhead) fetch();
-    ry.get(m);
-    rx.get(z);
+    ry.get(m, cols);
+    rx.get(z, cols);
     if (kAhead && l + a.groups < a.L) fetch();
     float2 sp = make_float2(0.0f, 1.0f), sn = make_float2(0.0f, 1.0f);
-    if (a.post != kNone) sp = row_stats<VEC, NI>(m, a.post, a.C, inv_c, a.eps, sum);
+    if (a.post != kNone) sp = row_stats<T, VEC, NI, SHIFT>(m, a.post, cols, inv_c, a.eps, sum);
     const float rs = sp.y * a.rho;
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) z[i][e] = fmaf((m[i][e] - sp.x) * rs, gw[i][e], z[i][e]);
-    store_row<T, VEC, NI>(static_cast<T*>(a.out0) + r * a.C, a.C, z);
+    store_row<T, VEC, NI, SHIFT>(static_cast<T*>(a.out0) + r * a.C, cols, z);
     if (a.pre != kNone) {
-      sn = row_stats<VEC, NI>(z, a.pre, a.C, inv_c, a.eps, sum);
+      sn = row_stats<T, VEC, NI, SHIFT>(z, a.pre, cols, inv_c, a.eps, sum);
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) z[i][e] = fmaf((z[i][e] - sn.x) * sn.y, sw[i][e], sh[i][e]);
-      store_row<T, VEC, NI>(static_cast<T*>(a.out1) + r * a.C, a.C, z);
+      store_row<T, VEC, NI, SHIFT>(static_cast<T*>(a.out1) + r * a.C, cols, z);
     }
     if (threadIdx.x == 0)
       *reinterpret_cast<float4*>(a.stats + 4 * r) = make_float4(sp.x, sp.y, sn.x, sn.y);
   }
 }
 
-template <class T, int VEC, int NI, int MAXT>
+template <class T, int VEC, int NI, int MAXT, bool SHIFT>
 __global__ void __launch_bounds__(MAXT, MAXT == 256 && VEC == 1 ? 2 : 1) norm_gate_bwd_k(const Args a) {
   __shared__ __align__(16) float2 sm[2][16];
   grid_release();
@@ -244,17 +294,24 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 && VEC == 1 ? 2 : 1) norm_ga
   const T* dz = has_z ? static_cast<const T*>(a.dz) + b * a.zb + g * a.zl : nullptr;
   const float4* stats = reinterpret_cast<const float4*>(a.stats) + b * a.L + g;
   const int64_t ix = a.groups * a.xl, iy = a.groups * a.yl, ih = a.groups * a.hl, iz = a.groups * a.zl;
-  RawRow<T, VEC, NI> ry, rx, rh, rz;
+  const Columns<T, VEC, NI, SHIFT> cols(a.C, SHIFT ? (int)((b * a.xb + g * a.xl) % VEC) : 0);
+  // elements from this row's start to the tensors' ends: the least of the four
+  auto room_of = [&](int64_t sb, int64_t sl) { return (a.B - 1 - b) * sb + (a.L - 1 - g) * sl + a.C; };
+  int64_t room = SHIFT ? min(room_of(a.xb, a.xl), room_of(a.yb, a.yl)) : 0, step = SHIFT ? max(ix, iy) : 0;
+  if (SHIFT && has_h) { room = min(room, room_of(a.hb, a.hl)); step = max(step, ih); }
+  if (SHIFT && has_z) { room = min(room, room_of(a.zb, a.zl)); step = max(step, iz); }
+  RawRow<T, VEC, NI, SHIFT> ry, rx, rh, rz;
   ry.clear();
   rx.clear();
   rh.clear();
   rz.clear();
   float4 st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
   auto fetch = [&]() {  // the next row of the group
-    ry.load(y, a.C);
-    rx.load(x, a.C);
-    if (has_h) rh.load(dh, a.C);
-    if (has_z) rz.load(dz, a.C);
+    ry.load(y, cols, room);
+    rx.load(x, cols, room);
+    if (has_h) rh.load(dh, cols, room);
+    if (has_z) rz.load(dz, cols, room);
+    room -= step;
     st = __ldg(stats);
     y += iy;
     x += ix;
@@ -266,8 +323,8 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 && VEC == 1 ? 2 : 1) norm_ga
   const int64_t first = g < a.groups ? g : a.L;  // a block of several groups may hold more than there are
   if (kAhead && first < a.L) fetch();
   float gw[NI][VEC], sw[NI][VEC];
-  load_coef<VEC, NI>(a.wpost, a.gate ? a.gate + b * a.C : nullptr, a.gate ? 0.0f : 1.0f, a.C, gw);
-  load_coef<VEC, NI>(a.wpre, a.scale ? a.scale + b * a.C : nullptr, 1.0f, a.C, sw);
+  load_coef<T, VEC, NI, SHIFT>(a.wpost, a.gate ? a.gate + b * a.C : nullptr, a.gate ? 0.0f : 1.0f, cols, gw);
+  load_coef<T, VEC, NI, SHIFT>(a.wpre, a.scale ? a.scale + b * a.C : nullptr, 1.0f, cols, sw);
   float a0[NI][VEC], a1[NI][VEC], a2[NI][VEC];
 #pragma unroll
   for (int i = 0; i < NI; ++i)
@@ -281,11 +338,11 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 && VEC == 1 ? 2 : 1) norm_ga
     const int64_t r = b * a.L + l;
     float n[NI][VEC], m[NI][VEC], d[NI][VEC], dzv[NI][VEC];
     if (!kAhead) fetch();
-    ry.get(m);
-    rx.get(n);
+    ry.get(m, cols);
+    rx.get(n, cols);
     const float4 s4 = st;
-    if (has_h) rh.get(d);
-    if (has_z) rz.get(dzv);
+    if (has_h) rh.get(d, cols);
+    if (has_z) rz.get(dzv, cols);
     if (kAhead && l + a.groups < a.L) fetch();
 #pragma unroll
     for (int i = 0; i < NI; ++i)
@@ -325,7 +382,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 && VEC == 1 ? 2 : 1) norm_ga
 #pragma unroll
         for (int e = 0; e < VEC; ++e) d[i][e] += dzv[i][e];
     }
-    store_row<T, VEC, NI>(static_cast<T*>(a.out0) + r * a.C, a.C, d);
+    store_row<T, VEC, NI, SHIFT>(static_cast<T*>(a.out0) + r * a.C, cols, d);
     // gw is 0 past C: those columns stay out of the sums, and a2 there is never stored
     float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -345,16 +402,16 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 && VEC == 1 ? 2 : 1) norm_ga
 #pragma unroll
         for (int e = 0; e < VEC; ++e) d[i][e] = s4.y * (d[i][e] - mean - m[i][e] * dot);
     }
-    store_row<T, VEC, NI>(static_cast<T*>(a.out1) + r * a.C, a.C, d);
+    store_row<T, VEC, NI, SHIFT>(static_cast<T*>(a.out1) + r * a.C, cols, d);
   }
   if (a.part == nullptr || g >= a.groups) return;
   float* p = a.part + (b * a.groups + g) * 3 * a.C;
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const int c = (i * (int)blockDim.x + (int)threadIdx.x) * VEC;
+    const int c = cols.at(i);
 #pragma unroll
     for (int e = 0; e < VEC; ++e)
-      if (c + e < a.C) {
+      if (cols.has(i, e)) {
         p[c + e] = a0[i][e];
         p[a.C + c + e] = a1[i][e];
         p[2 * a.C + c + e] = a2[i][e];
@@ -423,78 +480,106 @@ __global__ void __launch_bounds__(1024) norm_gate_reduce_k(const ReduceArgs a) {
   }
 }
 
-// The widest accesses, of 4, 2 or 1 elements, for which every row of every tensor starts on a boundary
-// of that size (odd widths and sliced views fall to the narrower ones).
-static int vec_of(const Args& a, int size) {
-  for (int n = 4; n > 1; n /= 2) {
-    auto bad = [&](const void* p, int64_t sb, int64_t sl) {
-      return p && ((reinterpret_cast<uintptr_t>(p) & (n * size - 1)) || sb % n || sl % n);
-    };
-    if (a.C % n == 0 && !bad(a.x, a.xb, a.xl) && !bad(a.y, a.yb, a.yl) && !bad(a.dz, a.zb, a.zl) &&
-        !bad(a.dh, a.hb, a.hl) && !bad(a.out0, 0, 0) && !bad(a.out1, 0, 0))
-      return n;
-  }
-  return 1;
+// How rows are accessed: by runs of four elements where every row of every tensor starts on a boundary of
+// four (kWide); where the tensors start on one and their strides leave the same remainder, as contiguous
+// ones of odd width do, by runs of four with a shift (kShifted); element by element otherwise (some sliced
+// views).  6000 x 1999 in bf16, shifted and by elements: see above.
+enum Access : int { kWide = 0, kShifted = 1, kSingle = 2 };
+
+static Access access_of(const Args& a, int size) {
+  bool wide = a.C % 4 == 0, shifted = a.C <= kMaxColumns - 3;
+  auto look = [&](const void* p, int64_t sb, int64_t sl) {
+    if (!p) return;
+    if (reinterpret_cast<uintptr_t>(p) & (4 * size - 1)) wide = shifted = false;
+    if (sb % 4 || sl % 4) wide = false;
+    if ((sb - a.L * a.C) % 4 || (sl - a.C) % 4 || sb < 0 || sl < 0) shifted = false;
+  };
+  look(a.x, a.xb, a.xl);
+  look(a.y, a.yb, a.yl);
+  look(a.dz, a.zb, a.zl);
+  look(a.dh, a.hb, a.hl);
+  look(a.out0, a.L * a.C, a.C);
+  look(a.out1, a.L * a.C, a.C);
+  return wide ? kWide : (shifted ? kShifted : kSingle);
 }
 
 struct Shape {
+  Access access;
   dim3 block;
   int per;  // elements per thread
 };
 
-static Shape shape_of(int C) {
+static Shape shape_of(const Args& a, int size) {
   Shape s;
+  s.access = access_of(a, size);
+  const int C = a.C + (s.access == kShifted ? 3 : 0);
   s.per = C <= 512 ? 4 : (C <= 8 * kMaxThreads ? 8 : 16);
   const int t = ((C + s.per - 1) / s.per + 31) / 32 * 32;
   s.block = t == 32 ? dim3(32, 4) : dim3(t, 1);
   return s;
 }
 
-// Row groups per batch entry so that about `threads` threads per SM are launched, one row per group at
-// least: twice what is resident evens out the SMs' shares (forward, 768 in place of 1024: 53 us).
-static dim3 grid_of(Args& a, const Shape& s, int threads) {
-  const int64_t per_sm = threads / (int)s.block.x > 0 ? threads / (int)s.block.x : 1;
-  const int64_t want = (sm_count() * per_sm + a.B - 1) / a.B;
-  a.groups = (int)(want < a.L ? want : a.L);
-  return dim3((a.groups + s.block.y - 1) / s.block.y, a.B);
+using Kernel = void (*)(Args);
+
+template <class T, int VEC, int PER, bool BWD, bool SHIFT>
+static Kernel kernel_for(const Shape& s) {
+  constexpr int NI = PER / VEC;
+  // blocks of up to 256 threads may take more registers than those of up to 512 (backward, single elements: half of
+  // them, see above)
+  if (s.block.x * s.block.y > 256)
+    return BWD ? norm_gate_bwd_k<T, VEC, NI, kMaxThreads, SHIFT> : norm_gate_k<T, VEC, NI, kMaxThreads, SHIFT>;
+  if constexpr (PER <= 8) return BWD ? norm_gate_bwd_k<T, VEC, NI, 256, SHIFT> : norm_gate_k<T, VEC, NI, 256, SHIFT>;
+  return nullptr;  // 16 elements per thread: more than 4096 columns, more than 256 threads
 }
 
-// Blocks of up to 256 threads may take more registers than those of up to 512 (backward, single
-// elements: half of them, see above).
-template <class T, int VEC, int PER, bool BWD>
-static void start(const Args& a, const Shape& s, dim3 grid, cudaStream_t st) {
-  constexpr int NI = PER / VEC;
-  if (s.block.x * s.block.y > 256)
-    BWD ? norm_gate_bwd_k<T, VEC, NI, kMaxThreads><<<grid, s.block, 0, st>>>(a)
-        : norm_gate_k<T, VEC, NI, kMaxThreads><<<grid, s.block, 0, st>>>(a);
-  else if constexpr (PER <= 8)
-    BWD ? norm_gate_bwd_k<T, VEC, NI, 256><<<grid, s.block, 0, st>>>(a)
-        : norm_gate_k<T, VEC, NI, 256><<<grid, s.block, 0, st>>>(a);
+template <class T, int PER, bool BWD>
+static Kernel kernel_for_access(const Shape& s) {
+  if (s.access == kWide) return kernel_for<T, 4, PER, BWD, false>(s);
+  if (s.access == kShifted) return kernel_for<T, 4, PER, BWD, true>(s);
+  return kernel_for<T, 1, PER, BWD, false>(s);
 }
 
 template <class T, bool BWD>
-static void start_type(const Args& a, const Shape& s, int vec, dim3 grid, cudaStream_t st) {
-  if (s.per == 4) {
-    if (vec == 4) start<T, 4, 4, BWD>(a, s, grid, st);
-    else if (vec == 2) start<T, 2, 4, BWD>(a, s, grid, st);
-    else start<T, 1, 4, BWD>(a, s, grid, st);
-  } else if (s.per == 8) {
-    if (vec == 4) start<T, 4, 8, BWD>(a, s, grid, st);
-    else if (vec == 2) start<T, 2, 8, BWD>(a, s, grid, st);
-    else start<T, 1, 8, BWD>(a, s, grid, st);
-  } else {
-    if (vec == 4) start<T, 4, 16, BWD>(a, s, grid, st);
-    else start<T, 1, 16, BWD>(a, s, grid, st);
-  }
+static Kernel kernel_for_type(const Shape& s) {
+  if (s.per == 4) return kernel_for_access<T, 4, BWD>(s);
+  if (s.per == 8) return kernel_for_access<T, 8, BWD>(s);
+  return kernel_for_access<T, 16, BWD>(s);
 }
 
+struct Plan {
+  Kernel kernel;
+  dim3 grid, block;
+};
+
+// The kernel of a call, and as many row groups per batch entry as fill the GPU once, one row per group at least
+// (8193 x 1024 x 2: with twice as many, whose second half waits for the first, 46 us forward and 82 backward, with 1.5
+// times as many 53 and more).  With a shift, a multiple of four, so that all rows of a group have the same one.
 template <bool BWD>
-static void launch(const Args& a, const Shape& s, int dtype, dim3 grid, cudaStream_t st) {
-  const int vec = vec_of(a, dtype_size(dtype));
-  LaunchScope scope(kKElementwise, st);
-  if (dtype == kF32) start_type<float, BWD>(a, s, vec, grid, st);
-  else if (dtype == kBF16) start_type<__nv_bfloat16, BWD>(a, s, vec, grid, st);
-  else start_type<__half, BWD>(a, s, vec, grid, st);
+static Plan plan_of(Args& a, int dtype) {
+  const Shape s = shape_of(a, dtype_size(dtype));
+  Plan p;
+  p.kernel = dtype == kF32 ? kernel_for_type<float, BWD>(s)
+                           : (dtype == kBF16 ? kernel_for_type<__nv_bfloat16, BWD>(s) : kernel_for_type<__half, BWD>(s));
+  p.block = s.block;
+  const int threads = (int)(s.block.x * s.block.y);
+  // resident blocks per SM, asked for once per kernel and block size
+  static std::atomic<int> known[3][3][3][kMaxThreads / 32 + 1];
+  std::atomic<int>& blocks = known[dtype][s.access][s.per / 8][threads / 32];
+  int n = blocks.load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, p.kernel, threads, 0) != cudaSuccess || n < 1) n = 1;
+    blocks.store(n, std::memory_order_relaxed);
+  }
+  const int64_t want = ((int64_t)sm_count() * n * s.block.y + a.B - 1) / a.B;
+  a.groups = (int)(want < a.L ? want : a.L);
+  if (s.access == kShifted && a.groups < a.L) a.groups = a.groups < 4 ? 4 : a.groups / 4 * 4;
+  p.grid = dim3((a.groups + s.block.y - 1) / s.block.y, a.B);
+  return p;
+}
+
+static void launch(const Args& a, const Plan& p, cudaStream_t stream) {
+  LaunchScope scope(kKElementwise, stream);
+  p.kernel<<<p.grid, p.block, 0, stream>>>(a);
 }
 
 // whether a tensor's pointer is not a multiple of its element's size
@@ -541,9 +626,8 @@ int triposplat_b200_norm_gate(const void* x, const void* y, const int64_t* strid
                         static_cast<const void*>(scale), static_cast<const void*>(shift),
                         static_cast<const void*>(pre_weight), static_cast<const void*>(post_weight)})
     if (p && !is_device_pointer(p)) return kNotDevicePointer;
-  const ng::Shape s = ng::shape_of(C);
-  const dim3 grid = ng::grid_of(a, s, 1024);
-  ng::launch<false>(a, s, dtype, grid, current_stream());
+  const ng::Plan plan = ng::plan_of<false>(a, dtype);
+  ng::launch(a, plan, current_stream());
   return launch_status();
 }
 
@@ -575,15 +659,14 @@ int triposplat_b200_norm_gate_backward(const void* dz, const void* dh, const voi
                         static_cast<const void*>(dscale), static_cast<const void*>(dshift),
                         static_cast<const void*>(dpre_weight), static_cast<const void*>(dpost_weight)})
     if (p && !is_device_pointer(p)) return kNotDevicePointer;
-  const ng::Shape s = ng::shape_of(C);
   cudaStream_t stream = current_stream();
-  const dim3 grid = ng::grid_of(a, s, 512);
+  const ng::Plan plan = ng::plan_of<true>(a, dtype);
   const bool sums = dgate || dscale || dshift || dpre_weight || dpost_weight;
   if (sums) {
     a.part = static_cast<float*>(workspace((size_t)B * a.groups * 3 * C * sizeof(float), stream));
     if (!a.part) return kWorkspace;
   }
-  ng::launch<true>(a, s, dtype, grid, stream);
+  ng::launch(a, plan, stream);
   if (sums) {
     const ng::ReduceArgs ra{a.part, gate, scale, pre_weight, post_weight, dgate, dscale, dshift, dpre_weight,
                             dpost_weight, B, C, a.groups, residual_scale};

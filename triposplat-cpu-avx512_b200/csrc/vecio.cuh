@@ -49,6 +49,44 @@ struct Raw {
   typename Bits<sizeof(T) * VEC>::type b;
   __device__ __forceinline__ void load(const T* p) { b = *reinterpret_cast<const decltype(b)*>(p); }
   __device__ __forceinline__ float operator[](int i) const;
+  // Elements [0, n) alone, word by word (n odd in a 16-bit type: the last is the low half of its word, so it too
+  // lands in its register as it is); the rest keeps its bits.
+  __device__ __forceinline__ void load_first(const T* p, int n) {
+    constexpr int PER = 4 / sizeof(T), WORDS = VEC / PER;
+    static_assert(WORDS >= 1, "whole words");
+    uint32_t w[WORDS];
+    memcpy(w, &b, sizeof(w));
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      if ((i + 1) * PER <= n) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+      else if (i * PER < n) w[i] = *reinterpret_cast<const uint16_t*>(p + i * PER);
+    }
+    memcpy(&b, w, sizeof(w));
+  }
+  // the bits of the elements [from, to) set
+  __device__ __forceinline__ void mask(int from, int to) {
+    constexpr int PER = 4 / sizeof(T), WORDS = VEC / PER;
+    uint32_t w[WORDS];
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      w[i] = 0;
+#pragma unroll
+      for (int e = 0; e < PER; ++e)
+        if (i * PER + e >= from && i * PER + e < to) w[i] |= (PER == 1 ? 0xffffffffu : 0xffffu) << (16 * e);
+    }
+    memcpy(&b, w, sizeof(w));
+  }
+  __device__ __forceinline__ Raw operator&(const Raw& m) const {
+    constexpr int WORDS = VEC * sizeof(T) / 4;
+    uint32_t x[WORDS], y[WORDS];
+    memcpy(x, &b, sizeof(x));
+    memcpy(y, &m.b, sizeof(y));
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) x[i] &= y[i];
+    Raw r;
+    memcpy(&r.b, x, sizeof(x));
+    return r;
+  }
 };
 template <int VEC>
 __device__ __forceinline__ float raw_get(const Raw<float, VEC>& r, int i) { return __uint_as_float(word(r.b, i)); }
@@ -78,6 +116,23 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// VEC values as one access's bits
+template <class T, int VEC>
+__device__ __forceinline__ typename Bits<sizeof(T) * VEC>::type bits_of(const float (&in)[VEC]) {
+  typename Bits<sizeof(T) * VEC>::type b;
+  if constexpr (sizeof(T) == 4) {
+    memcpy(&b, in, sizeof(b));
+  } else if constexpr (VEC == 1) {
+    const T v = from_f32<T>(in[0]);
+    memcpy(&b, &v, sizeof(b));
+  } else {
+    uint32_t w[VEC / 2];
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) w[i] = pack2<T>(in[2 * i], in[2 * i + 1]);
+    memcpy(&b, w, sizeof(b));
+  }
+  return b;
+}
 template <class T, int VEC>
 __device__ __forceinline__ void load_vec(const T* p, float (&out)[VEC]) {
   Raw<T, VEC> r;
@@ -88,20 +143,7 @@ __device__ __forceinline__ void load_vec(const T* p, float (&out)[VEC]) {
 
 template <class T, int VEC>
 __device__ __forceinline__ void store_vec(T* p, const float (&in)[VEC]) {
-  if constexpr (VEC == 1) {
-    *p = from_f32<T>(in[0]);
-  } else if constexpr (sizeof(T) == 4) {
-    typename Bits<4 * VEC>::type b;
-    memcpy(&b, in, sizeof(b));
-    *reinterpret_cast<decltype(b)*>(p) = b;
-  } else {
-    uint32_t w[VEC / 2];
-#pragma unroll
-    for (int i = 0; i < VEC / 2; ++i) w[i] = pack2<T>(in[2 * i], in[2 * i + 1]);
-    typename Bits<2 * VEC>::type b;
-    memcpy(&b, w, sizeof(b));
-    *reinterpret_cast<decltype(b)*>(p) = b;
-  }
+  *reinterpret_cast<typename Bits<sizeof(T) * VEC>::type*>(p) = bits_of<T, VEC>(in);
 }
 
 }  // namespace tsb
