@@ -39,6 +39,9 @@ namespace ng {
 
 enum Kind : int { kNone = 0, kLayer = 1, kRms = 2 };
 constexpr int kMaxThreads = 512;   // per row: 4 columns each up to 512, 8 up to 4096, 16 beyond
+// blocks of up to this many threads: up to 168 registers, three warps in each quarter of an SM (free to take
+// more, the backward kernel takes 176 to 192, and only two fit: 8193 x 1024 x 2 80 us)
+constexpr int kFewThreads = 384;
 constexpr int kMaxColumns = 8192;
 
 struct Args {
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(MAXT, 1) norm_gate_k(const Args a) {
 }
 
 template <class T, int VEC, int NI, int MAXT, bool SHIFT>
-__global__ void __launch_bounds__(MAXT, MAXT == 256 && VEC == 1 ? 2 : 1) norm_gate_bwd_k(const Args a) {
+__global__ void __launch_bounds__(MAXT, 1) norm_gate_bwd_k(const Args a) {
   __shared__ __align__(16) float2 sm[2][16];
   grid_release();
   RowSum sum(sm);
@@ -524,12 +527,9 @@ using Kernel = void (*)(Args);
 template <class T, int VEC, int PER, bool BWD, bool SHIFT>
 static Kernel kernel_for(const Shape& s) {
   constexpr int NI = PER / VEC;
-  // blocks of up to 256 threads may take more registers than those of up to 512 (backward, single elements: half of
-  // them, see above)
-  if (s.block.x * s.block.y > 256)
+  if (s.block.x * s.block.y > kFewThreads)
     return BWD ? norm_gate_bwd_k<T, VEC, NI, kMaxThreads, SHIFT> : norm_gate_k<T, VEC, NI, kMaxThreads, SHIFT>;
-  if constexpr (PER <= 8) return BWD ? norm_gate_bwd_k<T, VEC, NI, 256, SHIFT> : norm_gate_k<T, VEC, NI, 256, SHIFT>;
-  return nullptr;  // 16 elements per thread: more than 4096 columns, more than 256 threads
+  return BWD ? norm_gate_bwd_k<T, VEC, NI, kFewThreads, SHIFT> : norm_gate_k<T, VEC, NI, kFewThreads, SHIFT>;
 }
 
 template <class T, int PER, bool BWD>
