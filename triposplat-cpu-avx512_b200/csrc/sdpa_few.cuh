@@ -11,6 +11,10 @@
 // a last kernel in their order.  Backward: per key e and ds of every row give its dK, dV at once, dQ is
 // kept in registers and joined the same way.
 //
+// Bound by HBM: 32 heads of 8193 keys are 134 MB of K and V, 28 us forward for one query (4.8 TB/s), and 268 MB with
+// their gradients, 45 us backward (6.0); four queries take 50 and 72 us, bound by instructions (80 FMAs per
+// key, lane and query backward).
+//
 // Included by sdpa_backward.cu, whose Rows, Bias and helpers it uses.
 
 constexpr int kFewRows = 4;
