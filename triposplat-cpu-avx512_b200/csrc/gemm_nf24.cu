@@ -618,7 +618,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if constexpr (MODE == kGatedResidual) {
           const int b0 = mbase / p.rows_per_batch;
           jb = (b0 + 1) * p.rows_per_batch - mbase;
-          g0 = col_ok ? p.gate[(int64_t)b0 * p.gate_ld + n] : 0.0f;
+          // (the second half of the last tile may lie past M, and b0 then past the gate's rows)
+          g0 = col_ok && mbase < p.M ? p.gate[(int64_t)b0 * p.gate_ld + n] : 0.0f;
           g1 = (col_ok && jb < EPI_COLS && mbase + jb < p.M) ? p.gate[(int64_t)(b0 + 1) * p.gate_ld + n] : 0.0f;
         }
         float* wst = ostage + (warp - 6) * 2 * OUT_CHUNK;
