@@ -92,7 +92,7 @@ def build_calls(force: bool = False) -> Path:
         return CALLS
     include = [torch_dir / "include", torch_dir / "include/torch/csrc/api/include", sysconfig.get_paths()["include"],
                Path(nvcc()).resolve().parent.parent / "include"]
-    libs = ["-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
+    libs = ["-ltorch_python", "-ltorch_cpu", "-ltorch", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
     tmp = CALLS.with_suffix(".so.tmp")
     cmd = ["g++", *flags, *(f"-I{d}" for d in include), str(source), "-o", str(tmp),
            f"-L{torch_dir / 'lib'}", f"-Wl,-rpath,{torch_dir / 'lib'}", *libs]

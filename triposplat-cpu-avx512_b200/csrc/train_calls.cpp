@@ -6,6 +6,7 @@
 // A refused argument is a ValueError, a status of the library a RuntimeError.  The library's functions come
 // as addresses (bind), so that it is loaded in one place, from whatever file the environment names.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -117,9 +118,16 @@ Tensor param(PyObject* o, const char* name, IntArrayRef shape, at::Device device
 // a tensor with a contiguous last dimension (a copy only if it has none)
 Tensor rows(const Tensor& t) { return t.stride(-1) != 1 && t.size(-1) != 1 ? t.contiguous() : t; }
 
+// New tensors, past the dispatcher (half of an allocation's time).
+Tensor fresh(IntArrayRef sizes, ScalarType dtype, at::Device device) {
+  if (!device.is_cuda()) refuse("expected CUDA tensors, got ", device);
+  return Tensor(at::detail::empty_cuda(sizes, dtype, device, std::nullopt));
+}
+Tensor fresh(const Tensor& like) { return fresh(like.sizes(), like.scalar_type(), like.device()); }
+
 // an output of x's shape and type: `o` if given (unit last stride), a new one otherwise
 Tensor out_like(PyObject* o, const Tensor& x, const char* name) {
-  if (o == Py_None) return at::empty(x.sizes(), x.options());
+  if (o == Py_None) return fresh(x);
   const Tensor& t = check(tensor(o, name), name, x.sizes(), x.scalar_type(), x.device());
   if (t.stride(-1) != 1 && t.size(-1) != 1) refuse(name, " needs a contiguous last dimension");
   for (int64_t i = 0; i < t.dim(); ++i)
@@ -130,7 +138,7 @@ Tensor out_like(PyObject* o, const Tensor& x, const char* name) {
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* fptr(const Tensor& t) { return static_cast<float*>(ptr(t)); }
 
-Tensor like_param(const Tensor& t) { return t.defined() ? at::empty(t.sizes(), t.options()) : t; }
+Tensor like_param(const Tensor& t) { return t.defined() ? fresh(t) : t; }
 
 // the first `n` strides of each tensor, one after the other (zeros for one that is not there)
 template <int N, size_t M>
@@ -289,9 +297,7 @@ Norm norm_args(PyObject* px, PyObject* py, PyObject* const* a) {
 PyObject* norm_gate(PyObject* const* a) {  // x, y, the eight of norm_args, eps
   const Norm n = norm_args(a[0], a[1], a + 2);
   const float eps = (float)number(a[10]);
-  const Tensor z = at::empty(n.x.sizes(), n.x.options());
-  const Tensor h = n.pre ? at::empty(n.x.sizes(), n.x.options()) : Tensor();
-  const Tensor stats = at::empty({n.B, n.L, 4}, n.x.options().dtype(at::kFloat));
+  const Tensor z = fresh(n.x), h = n.pre ? fresh(n.x) : Tensor(), stats = fresh({n.B, n.L, 4}, at::kFloat, n.x.device());
   const auto s = strides<2, 2>({&n.x, &n.y});
   use_stream(n.x.device());
   ok(lib.norm_gate(ptr(n.x), ptr(n.y), s.data(), fptr(n.gate), fptr(n.scale), fptr(n.shift), fptr(n.wpre), fptr(n.wpost),
@@ -308,7 +314,7 @@ PyObject* norm_gate_backward(PyObject* const* a) {  // dz, dh, x, y, stats, the 
   };
   const Tensor dz = grad(a[0], "dz"), dh = grad(a[1], "dh");
   const Tensor stats = check(tensor(a[4], "stats"), "stats", {n.B, n.L, 4}, at::kFloat, n.x.device()).contiguous();
-  const Tensor dx = at::empty(n.x.sizes(), n.x.options()), dy = at::empty(n.x.sizes(), n.x.options());
+  const Tensor dx = fresh(n.x), dy = fresh(n.x);
   const Tensor dgate = like_param(n.gate), dscale = like_param(n.scale), dshift = like_param(n.shift),
                dwpre = like_param(n.wpre), dwpost = like_param(n.wpost);
   const auto s = strides<2, 4>({&n.x, &n.y, &dz, &dh});
@@ -352,12 +358,13 @@ Attention attention_args(PyObject* pq, PyObject* pk, PyObject* pv, PyObject* pbi
 
 // a new [B, H, L, 64] in token-major storage [B, L, H, 64]
 Tensor token_major(const Attention& t, int64_t L) {
-  return at::empty_strided({t.B, t.H, L, 64}, {L * t.H * 64, 64, (int64_t)t.H * 64, 1}, t.q.options());
+  if (!t.device.is_cuda()) refuse("expected CUDA tensors, got ", t.device);
+  return Tensor(at::detail::empty_strided_cuda({t.B, t.H, L, 64}, {L * t.H * 64, 64, (int64_t)t.H * 64, 1}, at::kFloat, t.device));
 }
 
 PyObject* attention_forward(PyObject* const* a) {  // q, k, v, key_bias
   const Attention t = attention_args(a[0], a[1], a[2], a[3]);
-  const Tensor out = token_major(t, t.Lq), stats = at::empty({t.B, t.H, t.Lq + 1, 2}, t.q.options());
+  const Tensor out = token_major(t, t.Lq), stats = fresh({t.B, t.H, t.Lq + 1, 2}, at::kFloat, t.device);
   const auto s = strides<3, 3>({&t.q, &t.k, &t.v});
   use_stream(t.device);
   ok(lib.attention_forward(fptr(t.q), fptr(t.k), fptr(t.v), s.data(), fptr(t.bias), t.bias_b, t.bias_h, fptr(out),
@@ -424,7 +431,7 @@ PyObject* clip_grad_norm(PyObject* const* a) {  // grads, max_norm, out
     sizes[i] = g.numel();
   }
   use_stream(device);
-  const Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(device));
+  const Tensor norm = fresh({}, at::kFloat, device);
   ok(lib.clip_grad_norm(in.data(), a[2] == Py_None ? nullptr : to.data(), sizes.data(), types.data(), (int)n, max_norm,
                         fptr(norm)), "clip_grad_norm");
   return wrap(norm);
