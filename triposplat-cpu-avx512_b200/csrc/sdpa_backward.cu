@@ -968,23 +968,24 @@ __global__ void __launch_bounds__(256) fwd_split_k(Rows q, Rows k, Rows v, Bias 
 
 // Gradients of passes whose walks were cut: a tensor's partial sums [cuts, BH, Lt, 64] added over the shares.
 // blockIdx.y is the tensor; a thread has 4 of a row's 64 elements and every W-th share (W = 8 where there
-// are more than that: few rows), whose sums are then added in order.
+// are more than that: few rows, else 1), whose sums are then added in order.
 struct Join {
   const float* part;
   float* out;
   int64_t sb, sh, sl;  // element strides of out
   int cuts, L, Lt;
+  __host__ __device__ int threads() const { return cuts > 8 ? 8 : 1; }  // per 4 elements
 };
 struct Joins {
   Join t[3];
   int H, BH, vec_out;
 };
-template <int W>
 __global__ void __launch_bounds__(256) join_k(const Joins a) {
-  __shared__ float4 sm[W == 1 ? 1 : 256];
+  __shared__ float4 sm[256];
   grid_release();
   grid_wait();
   const Join& t = a.t[blockIdx.y];
+  const int W = t.threads();
   const int lane = threadIdx.x % 16, y = threadIdx.x / 16 % W;
   const int64_t i = (int64_t)blockIdx.x * (16 / W) + threadIdx.x / (16 * W);
   const bool here = i < (int64_t)a.BH * t.L;
@@ -1005,7 +1006,7 @@ __global__ void __launch_bounds__(256) join_k(const Joins a) {
     __syncthreads();
     if (y != 0) return;
 #pragma unroll
-    for (int k = 1; k < W; ++k) {
+    for (int k = 1; k < 8; ++k) {
       const float4 v = sm[threadIdx.x + 16 * k];
       s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
     }
@@ -1274,14 +1275,14 @@ int triposplat_b200_attention_forward(const float* q, const float* k, const floa
       launch_chained(attn_join_k<1>, dim3((unsigned)((BH * Lq + 7) / 8)), dim3(256), 0, stream, o, part, cuts, cut_o, cut_st, st_ld,
                      by_head, BH * Lq, H, Lq, last, out_blhd, rows);
   };
-  if (Lq <= kFewRows) {
-    FewArgs a{};
+  FewArgs a{};
+  a.H = H; a.BH = (int)BH; a.Lq = Lq; a.Lk = Lk;
+  if (few(a)) {
     a.q = rows_of(q, strides); a.k = rows_of(k, strides + 3); a.v = rows_of(v, strides + 6);
     a.bias = bias;
     a.head = rows + Lq; a.head_stride = Lq + 1;
     a.o = out_blhd; a.stats_out = rows;
-    a.H = H; a.BH = (int)BH; a.Lq = Lq; a.Lk = Lk; a.vec = vec;
-    few_shares(a);
+    a.vec = vec;
     if (a.shares > 1) {
       const size_t obytes = al256((size_t)a.shares * BH * Lq * D * 4);
       uint8_t* ws = static_cast<uint8_t*>(workspace(obytes + (size_t)a.shares * BH * Lq * 8, stream));
@@ -1356,22 +1357,23 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
   };
   auto join = [&]() {
     if (parts == 0) return;
-    int most = 0, L = 0;
+    int64_t blocks = 0;
     for (int i = 0; i < parts; ++i) {
-      most = joins.t[i].cuts > most ? joins.t[i].cuts : most;
-      L = joins.t[i].L > L ? joins.t[i].L : L;
+      const int rows = 16 / joins.t[i].threads();
+      const int64_t n = (BH * joins.t[i].L + rows - 1) / rows;
+      blocks = n > blocks ? n : blocks;
     }
     LaunchScope scope(kKSdpaSplit, stream);
-    if (most > 8) launch_chained(join_k<8>, dim3((unsigned)((BH * L + 1) / 2), parts), dim3(256), 0, stream, joins);
-    else launch_chained(join_k<1>, dim3((unsigned)((BH * L + 15) / 16), parts), dim3(256), 0, stream, joins);
+    launch_chained(join_k, dim3((unsigned)blocks, parts), dim3(256), 0, stream, joins);
   };
   auto bias_grad = [&](const float* part, int terms, int Lt) {
     LaunchScope scope(kKSdpaSplit, stream);
     launch_chained(bias_grad_k, dim3((Lk + 31) / 32, bias_batches * bias_heads), dim3(32, 8), 0, stream, part, terms, B, H,
                    bias_batches, bias_heads, Lk, Lt, dbias);
   };
-  if (Lq <= kFewRows) {
-    FewArgs a{};
+  FewArgs a{};
+  a.H = H; a.BH = (int)BH; a.Lq = Lq; a.Lk = Lk;
+  if (few(a)) {
     a.dout = rows_of(dout, strides); a.q = rows_of(q, strides + 3); a.k = rows_of(k, strides + 6);
     a.v = rows_of(v, strides + 9); a.out = rows_of(out, strides + 12);
     a.bias = bias;
@@ -1379,17 +1381,24 @@ int triposplat_b200_attention_backward(const float* dout, const float* q, const 
     a.stats = rows;
     a.dk = dk; a.kb = go[3]; a.kh = go[4]; a.kl = go[5];
     a.dv = dv; a.vb = go[6]; a.vh = go[7]; a.vl = go[8];
-    a.H = H; a.BH = (int)BH; a.Lq = Lq; a.Lk = Lk; a.vec = vec; a.vec_out = vec_out;
-    few_shares(a);
+    a.vec = vec; a.vec_out = vec_out;
     const size_t qbytes = al256((size_t)a.shares * BH * Lq * D * 4);
-    uint8_t* ws = static_cast<uint8_t*>(workspace(qbytes + (dbias ? (size_t)BH * Lk * 4 : 0), stream));
+    const size_t kbytes = a.groups > 1 ? al256((size_t)a.groups * BH * Lk * D * 4) : 0;
+    uint8_t* ws = static_cast<uint8_t*>(workspace(qbytes + 2 * kbytes + (dbias ? (size_t)a.groups * BH * Lk * 4 : 0), stream));
     if (!ws) return kWorkspace;
     a.dq = reinterpret_cast<float*>(ws);
-    a.db = dbias ? reinterpret_cast<float*>(ws + qbytes) : nullptr;
+    a.dk_part = reinterpret_cast<float*>(ws + qbytes);
+    a.dv_part = reinterpret_cast<float*>(ws + qbytes + kbytes);
+    a.db = dbias ? reinterpret_cast<float*>(ws + qbytes + 2 * kbytes) : nullptr;
+    if (a.groups > 1) a.vec_out = 1;  // into the partial sums, joined by a last kernel as dq's are
     few_bwd(a, stream);
     add_join(a.dq, a.shares, Lq, Lq, dq, go);
+    if (a.groups > 1) {
+      add_join(a.dk_part, a.groups, Lk, Lk, dk, go + 3);
+      add_join(a.dv_part, a.groups, Lk, Lk, dv, go + 6);
+    }
     join();
-    if (dbias) bias_grad(a.db, 1, Lk);
+    if (dbias) bias_grad(a.db, a.groups, Lk);
     return launch_status();
   }
   st = key_bias ? ensure_kernel<true>() : ensure_kernel<false>();

@@ -1,7 +1,8 @@
-// Attention of up to four query rows per head (a pooled token, a decoded one), forward and backward,
-// in fp32 on the CUDA cores.  With so few rows the work is reading K and V once (and, backward, writing
-// their gradients): the tensor-core path would first write both as fp16 pairs and read those back,
-// and walk them with one held tile per head.
+// Attention of up to four query rows per head (a pooled token, a decoded one), and of any small number of
+// queries and keys in groups of four rows, forward and backward, in fp32 on the CUDA cores.  With so
+// few rows the work is reading K and V once (and, backward, writing their gradients): the tensor-core
+// path would first write both as fp16 pairs and read those back, and walk them with one held tile
+// per head.  With several groups, each writes its part of dK and dV, joined like the shares of dQ.
 //
 // Four lanes per key, 16 of its 64 dimensions each; a score is 16 products per lane and two shuffles.
 // A block takes a share of a head's keys, four warps of eight keys at a time.  Forward: each group
@@ -31,7 +32,9 @@ struct FewArgs {
   float* dq;               // partial [shares, BH, Lq, 64]
   float* db;               // nullable: [BH, Lk]
   int64_t kb, kh, kl, vb, vh, vl;  // strides of dk, dv
+  float *dk_part, *dv_part;  // several groups: [groups, BH, Lk, 64] in place of dk, dv; db then [groups, BH, Lk]
   int H, BH, Lq, Lk, vec, vec_out, shares, span;
+  int groups;              // of NQ query rows, a block each (blockIdx.z)
 };
 
 // sum over the lanes of a warp that hold the same dimensions (lane mod 4)
@@ -54,11 +57,12 @@ __global__ void __launch_bounds__(kFewThreads) few_fwd_k(const FewArgs a) {
   grid_wait();
   const int bh = blockIdx.y, b = bh / a.H, h = bh - b * a.H;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lq = lane & 3;
+  const int r0 = blockIdx.z * NQ, rows = min(NQ, a.Lq - r0);
   float2 head = make_float2(0.0f, 1.0f);
   if (a.bias.p) head = a.head[bh * a.head_stride];
   for (int i = threadIdx.x; i < NQ * D; i += kFewThreads) {
     const int r = i / D, d = i - r * D;
-    qs[r][d] = r < a.Lq && head.y != 0.0f ? a.q.at(b, h, r)[d] * (0.125f * LOG2E) : 0.0f;
+    qs[r][d] = r < rows && head.y != 0.0f ? a.q.at(b, h, r0 + r)[d] * (0.125f * LOG2E) : 0.0f;
   }
   __syncthreads();
   float m[NQ], l[NQ], o[NQ][16];
@@ -122,7 +126,7 @@ __global__ void __launch_bounds__(kFewThreads) few_fwd_k(const FewArgs a) {
   __syncthreads();
   for (int i = threadIdx.x; i < NQ * D; i += kFewThreads) {
     const int r = i / D, d = i - r * D;
-    if (r >= a.Lq) continue;
+    if (r >= rows) continue;
     float top = -INFINITY, ls = 0.0f, os = 0.0f;
 #pragma unroll
     for (int w = 0; w < kFewThreads / 32; ++w) top = fmaxf(top, sm_m[w][r]);
@@ -134,15 +138,15 @@ __global__ void __launch_bounds__(kFewThreads) few_fwd_k(const FewArgs a) {
     }
     os = ls == 0.0f ? 0.0f : os / ls;
     if (a.shares > 1) {
-      const int64_t row = ((int64_t)blockIdx.x * a.BH + bh) * a.Lq + r;
+      const int64_t row = ((int64_t)blockIdx.x * a.BH + bh) * a.Lq + r0 + r;
       a.o[row * D + d] = os;
       if (d == 0) a.stats_out[row] = make_float2(top, ls);
     } else {
-      a.o[(((int64_t)b * a.Lq + r) * a.H + h) * D + d] = os;
-      if (d == 0) a.stats_out[(int64_t)bh * (a.Lq + 1) + r] = make_float2(top, ls);
+      a.o[(((int64_t)b * a.Lq + r0 + r) * a.H + h) * D + d] = os;
+      if (d == 0) a.stats_out[(int64_t)bh * (a.Lq + 1) + r0 + r] = make_float2(top, ls);
     }
   }
-  if (!a.bias.p && blockIdx.x == 0 && threadIdx.x == 0 && a.shares == 1)
+  if (!a.bias.p && blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0 && a.shares == 1)
     a.stats_out[(int64_t)bh * (a.Lq + 1) + a.Lq] = make_float2(0.0f, 1.0f);
 }
 
@@ -155,19 +159,20 @@ __global__ void __launch_bounds__(kFewThreads) few_bwd_k(const FewArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lq = lane & 3;
   const float2 head = a.bias.p ? a.head[bh * a.head_stride] : make_float2(0.0f, 1.0f);
   const float c = 0.125f * LOG2E * head.y;
+  const int r0 = blockIdx.z * NQ, rows = min(NQ, a.Lq - r0);
   static_assert(NQ <= kFewThreads / 32, "a warp per row");
   if (warp < NQ) {  // q, g = dO / l, delta = g . O, m
     const int r = warp;
     float delta = 0.0f, m = INFINITY;
     float q[2] = {0.0f, 0.0f}, g[2] = {0.0f, 0.0f};
-    if (r < a.Lq) {
-      const float2 ml = a.stats[(int64_t)bh * (a.Lq + 1) + r];
+    if (r < rows) {
+      const float2 ml = a.stats[(int64_t)bh * (a.Lq + 1) + r0 + r];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        q[u] = a.q.at(b, h, r)[lane + 32 * u];
+        q[u] = a.q.at(b, h, r0 + r)[lane + 32 * u];
         if (ml.y != 0.0f) {
-          g[u] = a.dout.at(b, h, r)[lane + 32 * u] / ml.y;
-          delta = fmaf(g[u], a.out.at(b, h, r)[lane + 32 * u], delta);
+          g[u] = a.dout.at(b, h, r0 + r)[lane + 32 * u] / ml.y;
+          delta = fmaf(g[u], a.out.at(b, h, r0 + r)[lane + 32 * u], delta);
         }
       }
       if (ml.y != 0.0f) m = ml.x;  // else +inf: e = 0 throughout
@@ -221,6 +226,11 @@ __global__ void __launch_bounds__(kFewThreads) few_bwd_k(const FewArgs a) {
     if (j < j1) {
       float* pk = a.dk + b * a.kb + h * a.kh + j * a.kl;
       float* pv = a.dv + b * a.vb + h * a.vh + j * a.vl;
+      const int64_t part = ((int64_t)blockIdx.z * a.BH + bh) * a.Lk + j;
+      if (a.groups > 1) {
+        pk = a.dk_part + part * D;
+        pv = a.dv_part + part * D;
+      }
 #pragma unroll
       for (int e = 0; e < 16; ++e) dk[e] *= 0.125f;
       if (a.vec_out) {
@@ -236,7 +246,7 @@ __global__ void __launch_bounds__(kFewThreads) few_bwd_k(const FewArgs a) {
           pv[col16(lq, e)] = dv[e];
         }
       }
-      if (a.db && (lane & 3) == 0) a.db[(int64_t)bh * a.Lk + j] = db;
+      if (a.db && (lane & 3) == 0) a.db[part] = db;
     }
   }
 #pragma unroll
@@ -249,27 +259,42 @@ __global__ void __launch_bounds__(kFewThreads) few_bwd_k(const FewArgs a) {
   __syncthreads();
   for (int i = threadIdx.x; i < NQ * D; i += kFewThreads) {
     const int r = i / D, d = i - r * D;
-    if (r >= a.Lq) continue;
+    if (r >= rows) continue;
     float s = 0.0f;
 #pragma unroll
     for (int w = 0; w < kFewThreads / 32; ++w) s += sm_q[w][r][d];
-    a.dq[(((int64_t)blockIdx.x * a.BH + bh) * a.Lq + r) * D + d] = s * 0.125f;
+    a.dq[(((int64_t)blockIdx.x * a.BH + bh) * a.Lq + r0 + r) * D + d] = s * 0.125f;
   }
 }
 
-// Keys per block so that the GPU has some eight blocks per SM, a multiple of the 32 that a block takes
-// at a time and no less than four times that.
+static int few_rows(int Lq) { return Lq >= 3 ? 4 : Lq; }
+
+// Groups of query rows, and keys per block so that the GPU has some eight blocks per SM, a multiple of the 32 that a
+// block takes at a time and no less than four times that.
 static void few_shares(FewArgs& a) {
-  const int64_t want = ((int64_t)sm_count() * 8 + a.BH - 1) / a.BH;
+  a.groups = (a.Lq + few_rows(a.Lq) - 1) / few_rows(a.Lq);
+  const int64_t blocks = (int64_t)a.BH * a.groups, want = ((int64_t)sm_count() * 8 + blocks - 1) / blocks;
   const int64_t span = (a.Lk + want - 1) / want;
   a.span = (int)((span < 128 ? 128 : span + 31) / 32 * 32);
   a.shares = (a.Lk + a.span - 1) / a.span;
 }
 
+// Whether a call takes this path: up to four query rows, or so little work that the tensor-core path (29 to 36 us for
+// forward and backward of anything small) is all starts and ends.  This one takes some 17 us, 1.6 for every 100
+// blocks and 1 for every 10,000 pairs of a query and a key; measured, here and there: 4 heads 65 x 17 17.5 and 32, 4 heads
+// 200 x 20 17 and 35, 8 heads 16 x 1000 29 and 37, 32 heads 65 x 17 27 and 33, 32 heads 20 x 200 37 and 33, 4 heads 1000 x 16
+// 43 and 37, 32 heads 90 x 90 50 and 34.
+static bool few(FewArgs& a) {
+  if (a.Lq > kFewRows && (int64_t)a.BH * a.Lq > 140000) return false;
+  few_shares(a);
+  if (a.Lq <= kFewRows) return true;
+  return (int64_t)a.BH * a.Lq * a.Lk + 160ll * a.BH * a.groups * a.shares <= 140000;
+}
+
 // chained: behind the bias's rows
 static void few_fwd(const FewArgs& a, bool chained, cudaStream_t stream) {
   LaunchScope scope(kKSdpaAttn, stream);
-  const dim3 grid(a.shares, a.BH);
+  const dim3 grid(a.shares, a.BH, a.groups);
   auto kernel = a.Lq == 1 ? few_fwd_k<1> : (a.Lq == 2 ? few_fwd_k<2> : few_fwd_k<4>);
   if (chained) launch_chained(kernel, grid, dim3(kFewThreads), 0, stream, a);
   else kernel<<<grid, kFewThreads, 0, stream>>>(a);
@@ -277,8 +302,6 @@ static void few_fwd(const FewArgs& a, bool chained, cudaStream_t stream) {
 
 static void few_bwd(const FewArgs& a, cudaStream_t stream) {
   LaunchScope scope(kKSdpaAttn, stream);
-  const dim3 grid(a.shares, a.BH);
-  if (a.Lq == 1) few_bwd_k<1><<<grid, kFewThreads, 0, stream>>>(a);
-  else if (a.Lq == 2) few_bwd_k<2><<<grid, kFewThreads, 0, stream>>>(a);
-  else few_bwd_k<4><<<grid, kFewThreads, 0, stream>>>(a);
+  auto kernel = a.Lq == 1 ? few_bwd_k<1> : (a.Lq == 2 ? few_bwd_k<2> : few_bwd_k<4>);
+  kernel<<<dim3(a.shares, a.BH, a.groups), kFewThreads, 0, stream>>>(a);
 }
