@@ -482,7 +482,7 @@ int triposplat_b200_axis_rope_backward(const void* dy, const void* x, const void
  * stats [B, H, Lq + 1, 2] for the backward pass (a row's reference maximum in log2 units and
  * its sum; last, the largest bias and whether the scores count beside it).  A key whose bias is
  * -inf does not exist (its K and V may hold anything; whole tiles of 128 such keys at either end of
- * a row cost nothing); a row without keys is zeros.  Up to four queries per head, and calls of few
+ * a row cost nothing); a row without keys is zeros.  Up to eight queries per head, and calls of few
  * queries and keys, take fp32 kernels that read K and V as they are.  The scores' accuracy is that of
  * triposplat_sdpa_f32_avx512_exact_q8t512. */
 int triposplat_b200_attention_forward(const float* q, const float* k, const float* v,

@@ -1,4 +1,4 @@
-// Attention of up to four query rows per head (a pooled token, a decoded one), and of any small number of
+// Attention of up to eight query rows per head (a pooled token, a decoded one), and of any small number of
 // queries and keys in groups of four rows, forward and backward, in fp32 on the CUDA cores.  With so
 // few rows the work is reading K and V once (and, backward, writing their gradients): the tensor-core
 // path would first write both as fp16 pairs and read those back, and walk them with one held tile
@@ -18,7 +18,7 @@
 //
 // Included by sdpa_backward.cu, whose Rows, Bias and helpers it uses.
 
-constexpr int kFewRows = 4;
+constexpr int kFewRows = 8;
 constexpr int kFewThreads = 128;
 
 struct FewArgs {
@@ -34,7 +34,7 @@ struct FewArgs {
   int64_t kb, kh, kl, vb, vh, vl;  // strides of dk, dv
   float *dk_part, *dv_part;  // several groups: [groups, BH, Lk, 64] in place of dk, dv; db then [groups, BH, Lk]
   int H, BH, Lq, Lk, vec, vec_out, shares, span;
-  int groups;              // of NQ query rows, a block each (blockIdx.z)
+  int rows, groups;        // groups of NQ = rows query rows, a block each (blockIdx.z)
 };
 
 // sum over the lanes of a warp that hold the same dimensions (lane mod 4)
@@ -160,9 +160,7 @@ __global__ void __launch_bounds__(kFewThreads) few_bwd_k(const FewArgs a) {
   const float2 head = a.bias.p ? a.head[bh * a.head_stride] : make_float2(0.0f, 1.0f);
   const float c = 0.125f * LOG2E * head.y;
   const int r0 = blockIdx.z * NQ, rows = min(NQ, a.Lq - r0);
-  static_assert(NQ <= kFewThreads / 32, "a warp per row");
-  if (warp < NQ) {  // q, g = dO / l, delta = g . O, m
-    const int r = warp;
+  for (int r = warp; r < NQ; r += kFewThreads / 32) {  // a warp per row: q, g = dO / l, delta = g . O, m
     float delta = 0.0f, m = INFINITY;
     float q[2] = {0.0f, 0.0f}, g[2] = {0.0f, 0.0f};
     if (r < rows) {
@@ -267,41 +265,49 @@ __global__ void __launch_bounds__(kFewThreads) few_bwd_k(const FewArgs a) {
   }
 }
 
-static int few_rows(int Lq) { return Lq >= 3 ? 4 : Lq; }
-
 // Groups of query rows, and keys per block so that the GPU has some eight blocks per SM, a multiple of the 32 that a
 // block takes at a time and no less than four times that.
-static void few_shares(FewArgs& a) {
-  a.groups = (a.Lq + few_rows(a.Lq) - 1) / few_rows(a.Lq);
+static void few_shares(FewArgs& a, int rows) {
+  a.rows = rows;
+  a.groups = (a.Lq + rows - 1) / rows;
   const int64_t blocks = (int64_t)a.BH * a.groups, want = ((int64_t)sm_count() * 8 + blocks - 1) / blocks;
   const int64_t span = (a.Lk + want - 1) / want;
   a.span = (int)((span < 128 ? 128 : span + 31) / 32 * 32);
   a.shares = (a.Lk + a.span - 1) / a.span;
 }
 
-// Whether a call takes this path: up to four query rows, or so little work that the tensor-core path (29 to 36 us for
+// Whether a call takes this path: up to eight query rows, or so little work that the tensor-core path (29 to 36 us for
 // forward and backward of anything small) is all starts and ends.  This one takes some 17 us, 1.6 for every 100
 // blocks and 1 for every 10,000 pairs of a query and a key; measured, here and there: 4 heads 65 x 17 17.5 and 32, 4 heads
-// 200 x 20 17 and 35, 8 heads 16 x 1000 29 and 37, 32 heads 65 x 17 27 and 33, 32 heads 20 x 200 37 and 33, 4 heads 1000 x 16
-// 43 and 37, 32 heads 90 x 90 50 and 34.
+// 200 x 20 17 and 35, 8 heads 16 x 1000 29 and 37, 32 heads 65 x 17 27 and 33, 32 heads 20 x 200 37 and 33, 4 heads
+// 1000 x 16 43 and 37, 32 heads 90 x 90 50 and 34.  Five to eight rows of more than that are one group of eight (few
+// registers left for loads in flight, but K and V are read once): 32 heads 8 x 8193 225 us, there 290, 8 heads 8 x 3000 40
+// and 55, 32 heads 8 x 1000 39 and 62; of less, 8 heads 8 x 300, 33 us, as two groups of four 23.
 static bool few(FewArgs& a) {
-  if (a.Lq > kFewRows && (int64_t)a.BH * a.Lq > 140000) return false;
-  few_shares(a);
-  if (a.Lq <= kFewRows) return true;
-  return (int64_t)a.BH * a.Lq * a.Lk + 160ll * a.BH * a.groups * a.shares <= 140000;
+  if (a.Lq <= 4) {
+    few_shares(a, a.Lq == 3 ? 4 : a.Lq);
+    return true;
+  }
+  if ((int64_t)a.BH * a.Lq <= 140000) {
+    few_shares(a, 4);
+    if ((int64_t)a.BH * a.Lq * a.Lk + 160ll * a.BH * a.groups * a.shares <= 140000) return true;
+  }
+  if (a.Lq > kFewRows) return false;
+  few_shares(a, 8);
+  return true;
 }
 
 // chained: behind the bias's rows
 static void few_fwd(const FewArgs& a, bool chained, cudaStream_t stream) {
   LaunchScope scope(kKSdpaAttn, stream);
   const dim3 grid(a.shares, a.BH, a.groups);
-  auto kernel = a.Lq == 1 ? few_fwd_k<1> : (a.Lq == 2 ? few_fwd_k<2> : few_fwd_k<4>);
+  auto kernel = a.rows == 1 ? few_fwd_k<1> : (a.rows == 2 ? few_fwd_k<2> : (a.rows == 4 ? few_fwd_k<4> : few_fwd_k<8>));
   if (chained) launch_chained(kernel, grid, dim3(kFewThreads), 0, stream, a);
   else kernel<<<grid, kFewThreads, 0, stream>>>(a);
 }
 
 static void few_bwd(const FewArgs& a, cudaStream_t stream) {
   LaunchScope scope(kKSdpaAttn, stream);
-  auto kernel = a.Lq == 1 ? few_bwd_k<1> : (a.Lq == 2 ? few_bwd_k<2> : few_bwd_k<4>);
+  auto kernel = a.rows == 1 ? few_bwd_k<1> : (a.rows == 2 ? few_bwd_k<2> : (a.rows == 4 ? few_bwd_k<4> : few_bwd_k<8>));
   kernel<<<dim3(a.shares, a.BH, a.groups), kFewThreads, 0, stream>>>(a);
 }
