@@ -650,6 +650,11 @@ __device__ __forceinline__ float relative_bias(float v, float mx) {
   return v == -INFINITY ? v : (d < -1.0e6f ? -1.0e6f : d);
 }
 
+// A row's largest bias and whether the scores count beside it (0 beyond 2^60 in magnitude).
+__device__ __forceinline__ float2 bias_head(float mx) {
+  return make_float2(mx, mx > -INFINITY && fabsf(mx) > 0x1p60f ? 0.0f : 1.0f);
+}
+
 // Which bias row (b, h) reads: [bias_b, bias_h, Lk] with 1 for a shared dimension.
 struct Bias {
   const float* p;
@@ -674,8 +679,7 @@ __device__ __forceinline__ int2 tile_range(int lo, int hi, int2* sm) {
   return hi < 0 ? make_int2(0, 0) : make_int2(lo / HELD, hi / HELD + 1);
 }
 
-// One block per (b, h): the row's largest bias, where it leaves the scores weight (head = 0 beyond
-// 2^60 in magnitude), both behind the statistics for the backward pass, and (out not null) the
+// One block per (b, h): the row's head, behind the statistics for the backward pass, and (out not null) the
 // relative bias and the range of tiles with a key.
 __global__ void __launch_bounds__(256) bias_rows_k(Bias bias, int H, float* __restrict__ out, int2* __restrict__ tiles,
                                                    float2* head, int64_t head_stride) {
@@ -701,7 +705,7 @@ __global__ void __launch_bounds__(256) bias_rows_k(Bias bias, int H, float* __re
   const int2 range = tile_range(lo, hi, sm_range);  // also orders sm
 #pragma unroll
   for (int k = 0; k < 8; ++k) mx = fmaxf(mx, sm[k]);
-  if (threadIdx.x == 0) head[bh * head_stride] = make_float2(mx, mx > -INFINITY && fabsf(mx) > 0x1p60f ? 0.0f : 1.0f);
+  if (threadIdx.x == 0) head[bh * head_stride] = bias_head(mx);
   if (!out) return;
   if (threadIdx.x == 0) tiles[bh] = range;
   for (int j = threadIdx.x; j < bias.L; j += 256) out[(int64_t)bh * bias.L + j] = relative_bias(src[j], mx);
@@ -1290,8 +1294,10 @@ int triposplat_b200_attention_forward(const float* q, const float* k, const floa
       a.o = reinterpret_cast<float*>(ws);
       a.stats_out = reinterpret_cast<float2*>(ws + obytes);
     }
-    if (key_bias) bias_rows(nullptr, nullptr);
-    few_fwd(a, key_bias != nullptr, stream);
+    const bool apart = key_bias && Lk > kFewBias;
+    if (apart) bias_rows(nullptr, nullptr);
+    else if (key_bias) a.head_out = rows + Lq;
+    few_fwd(a, apart, stream);
     if (a.shares > 1) join(a.o, a.stats_out, a.shares, BH * Lq * D, BH * Lq, Lq, 1, key_bias == nullptr);
     return launch_status();
   }

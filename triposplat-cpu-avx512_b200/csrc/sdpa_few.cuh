@@ -20,11 +20,15 @@
 
 constexpr int kFewRows = 8;
 constexpr int kFewThreads = 128;
+// Keys up to which the forward blocks look for a bias row's largest value themselves, instead of a launch of its own:
+// 2 us less of 20 to 30 (32 heads 1 x 2000 31 and 33); every block reads the row, so long rows keep the launch.
+constexpr int kFewBias = 2048;
 
 struct FewArgs {
   Rows q, k, v, out, dout;
   Bias bias;               // .p null: none
   const float2* head;      // [BH] head_stride apart: (largest bias, weight of the scores); only with a bias
+  float2* head_out;        // forward: where not null, each block finds its row's head, and writes it here
   int64_t head_stride;
   const float2* stats;     // backward: [BH, Lq + 1]
   float *o, *dk, *dv;      // forward: [B, Lq, H, 64] or partial [shares, BH, Lq, 64]; backward: with strides
@@ -59,7 +63,23 @@ __global__ void __launch_bounds__(kFewThreads) few_fwd_k(const FewArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lq = lane & 3;
   const int r0 = blockIdx.z * NQ, rows = min(NQ, a.Lq - r0);
   float2 head = make_float2(0.0f, 1.0f);
-  if (a.bias.p) head = a.head[bh * a.head_stride];
+  if (a.bias.p && a.head_out) {
+    __shared__ float sm_b[kFewThreads / 32];
+    const float* row = a.bias.row(b, h);
+    float mx = -INFINITY;
+#pragma unroll 8
+    for (int j = threadIdx.x; j < a.Lk; j += kFewThreads) mx = fmaxf(mx, row[j]);
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
+    if (lane == 0) sm_b[warp] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kFewThreads / 32; ++w) mx = fmaxf(mx, sm_b[w]);
+    head = bias_head(mx);
+    if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) a.head_out[bh * a.head_stride] = head;
+  } else if (a.bias.p) {
+    head = a.head[bh * a.head_stride];
+  }
   for (int i = threadIdx.x; i < NQ * D; i += kFewThreads) {
     const int r = i / D, d = i - r * D;
     qs[r][d] = r < rows && head.y != 0.0f ? a.q.at(b, h, r0 + r)[d] * (0.125f * LOG2E) : 0.0f;
